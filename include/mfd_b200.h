@@ -27,7 +27,7 @@ enum mfd_status {
     MFD_ERR_CAPACITY = 4     /* a device-side capacity check tripped (reported through a status word) */
 };
 
-enum mfd_dtype { MFD_F32 = 0, MFD_BF16 = 1, MFD_I32 = 2, MFD_I64 = 3 };
+enum mfd_dtype { MFD_F32 = 0, MFD_BF16 = 1, MFD_I32 = 2, MFD_I64 = 3, MFD_I8 = 4, MFD_E4M3 = 5 };
 
 /* Thread-local message of the last failed call ("" if none). */
 const char* mfd_last_error(void);
@@ -307,6 +307,89 @@ int mfd_gdn_commit(const uint64_t* states, int state_dtype, const uint64_t* u, c
  */
 int mfd_conv_commit(const uint64_t* conv_states, const uint64_t* x, int64_t elem_bytes, int64_t layers,
                     int64_t conv_dim, int64_t kernel, const int32_t* window, void* stream);
+
+/*
+ * 8-bit paged K/V cache of one layer.  k_cache, v_cache: pages of page_size (16, 32, 64 or 128) tokens for every KV
+ * head, row (page p, KV head h, token t) at byte offset p * sc_p + h * sc_h + t * sc_t (K and V alike; 128 contiguous
+ * codes a row, strides and bases multiples of 16); code_dtype MFD_I8 or MFD_E4M3.  k_scale, v_scale
+ * [num_pages, Hkv] float32: a value is code * scale.  Request b holds seq_lens[b] tokens (int32, on the device),
+ * token j in page page_table[b * table_stride + j / page_size] (int32), slot j % page_size.  Lengths are clamped to
+ * [0, max_pages * page_size] and page ids to [0, num_pages), so no table makes a kernel read outside the cache.
+ */
+
+/*
+ * Quantise new rows into the cache.  k_new, v_new: bf16 rows (b, i, h) at sn_b, sn_n, sn_h elements (K and V alike, 128
+ * contiguous, multiples of 8), i < n.  Request b appends rows path[b * path_stride + r], r < rows (int64, null: row r
+ * itself); the list ends at its first entry outside [0, n) or at counts[b] (int32, null: rows).  A page's scale
+ * becomes max(its old scale if it already holds tokens of the request, max |finite new value| * r, 2^-100), r the
+ * float32 nearest to 1 / 127 (int8) or 1 / 448 (e4m3); codes are value / scale rounded to nearest even; tokens already in the page are rounded
+ * again when its scale grows.  An infinite value becomes +-127 or +-448, NaN becomes 0, and neither counts for the scale.
+ * Every product, quotient and rounding is the IEEE float32 one, so the codes do not depend on the launch.  new_lens
+ * [bs] int32 (must not be seq_lens) receives seq_lens + the rows appended.  Rows past max_pages * page_size, and rows
+ * of a page whose table entry is outside [0, num_pages), are dropped and status (optional device int) receives
+ * MFD_ERR_CAPACITY (the length then stops at the capacity).  A page that is written belongs to one request.
+ */
+int mfd_kv8_append(void* k_cache, void* v_cache, int64_t sc_p, int64_t sc_h, int64_t sc_t, int code_dtype,
+                   float* k_scale, float* v_scale, int64_t num_pages, int64_t page_size, const int32_t* page_table,
+                   int64_t table_stride, int64_t max_pages, const int32_t* seq_lens, const void* k_new,
+                   const void* v_new, int64_t sn_b, int64_t sn_n, int64_t sn_h, int64_t n, const int64_t* path,
+                   int64_t path_stride, int64_t rows, const int32_t* counts, int64_t bs, int64_t num_kv_heads,
+                   int64_t head_dim, int32_t* new_lens, int* status, void* stream);
+
+/*
+ * Attention of n query nodes per request over the cached tokens (all visible) and the nodes' own keys.  q, out: bf16
+ * rows (b, i, head) at sq_*, so_* elements (multiples of 8, 128 contiguous); k_new, v_new as for mfd_kv8_append (null:
+ * no keys of their own); node i sees node j where bit j of anc_bits[(b * n + i) * anc_words] is set (null: j <= i).
+ * lse [bs, n, H] float32 (optional): the natural log of the sum of exp(score * scale).  A row that sees nothing gives
+ * zeros and lse -inf.  A non-finite key or value a row does not see has no effect on it.  n = 1 is a decode step.
+ * Limits: head_dim 128, H a multiple of Hkv, n <= 4096.
+ * Workspace: mfd_kv8_attention_workspace() bytes, zeroed before its first use, any sizes in turn; its first int32 is a
+ * sticky device status, 1 once a bounded wait in the kernel gave up.  Tickets: mfd_kv8_attention_tickets(bs, n, H,
+ * Hkv) zeroed words of a ticket-only buffer, left zero again.
+ */
+size_t mfd_kv8_attention_workspace(int64_t bs, int64_t n, int64_t num_heads, int64_t num_kv_heads);
+int64_t mfd_kv8_attention_tickets(int64_t bs, int64_t n, int64_t num_heads, int64_t num_kv_heads);
+int mfd_kv8_attention(const void* q, int64_t sq_b, int64_t sq_n, int64_t sq_h, const void* k_cache,
+                      const void* v_cache, int64_t sc_p, int64_t sc_h, int64_t sc_t, int code_dtype,
+                      const float* k_scale, const float* v_scale, int64_t num_pages, int64_t page_size,
+                      const int32_t* page_table, int64_t table_stride, int64_t max_pages, const int32_t* seq_lens,
+                      const void* k_new, const void* v_new, int64_t sn_b, int64_t sn_n, int64_t sn_h,
+                      const uint64_t* anc_bits, int64_t anc_words, int64_t bs, int64_t n, int64_t num_heads,
+                      int64_t num_kv_heads, int64_t head_dim, float scale, void* out, int64_t so_b, int64_t so_n,
+                      int64_t so_h, float* lse, void* workspace, size_t workspace_bytes, unsigned int* tickets,
+                      int64_t tickets_len, void* stream);
+
+/*
+ * Attention weight per page, over the query rows that were accepted:
+ *   out[b, p] = decay * mass[b, p] + sum over heads, listed nodes i and tokens j of page p of
+ *               exp(q_i . k_j * scale - lse[b, i, head])      for the request's pages, 0 after them.
+ * q as above, lse [bs, n, H] float32 from mfd_kv8_attention (-inf: the row weighs nothing); path, rows, counts as for
+ * mfd_kv8_append (null path: nodes 0 .. counts - 1).  mass, out [bs, max_pages] float32 with row stride mass_stride
+ * (out may be mass).  The sums run in a fixed order.  Workspace: mfd_kv8_page_weights_workspace bytes; tickets: bs.
+ */
+size_t mfd_kv8_page_weights_workspace(int64_t bs, int64_t max_pages, int64_t page_size, int64_t num_kv_heads);
+int mfd_kv8_page_weights(const void* q, int64_t sq_b, int64_t sq_n, int64_t sq_h, const float* lse,
+                         const void* k_cache, int64_t sc_p, int64_t sc_h, int64_t sc_t, int code_dtype,
+                         const float* k_scale, int64_t num_pages, int64_t page_size, const int32_t* page_table,
+                         int64_t table_stride, int64_t max_pages, const int32_t* seq_lens, const int64_t* path,
+                         int64_t path_stride, int64_t rows, const int32_t* counts, int64_t bs, int64_t n,
+                         int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, float scale, float decay,
+                         const float* mass, float* out, int64_t mass_stride, void* workspace, size_t workspace_bytes,
+                         unsigned int* tickets, int64_t tickets_len, void* stream);
+
+/*
+ * Shorten every request that holds more than keep_pages pages: its first sink_pages and last recent_pages pages stay,
+ * and of the others those of the largest mass, keep_pages in all (equal masses: the earlier page stays; NaN counts as
+ * the least).  table_out, mass_out [bs, max_pages] receive the pages that stay, in order (then -1 and 0), freed the
+ * pages dropped, in order (then -1), freed_counts [bs] their number, new_lens [bs] the lengths left; the other
+ * requests come out as they are.  page_table, mass, table_out, mass_out, freed have row stride max_pages and overlap
+ * nowhere.  recent_pages >= 1 (the open page stays), sink_pages + recent_pages <= keep_pages.  Nothing of the cache
+ * moves: whole pages leave, with their scales.
+ */
+int mfd_kv8_evict(const int32_t* page_table, const float* mass, const int32_t* seq_lens, int64_t bs,
+                  int64_t max_pages, int64_t page_size, int64_t keep_pages, int64_t sink_pages, int64_t recent_pages,
+                  int32_t* table_out, float* mass_out, int32_t* new_lens, int32_t* freed, int32_t* freed_counts,
+                  void* stream);
 
 #ifdef __cplusplus
 }

@@ -67,10 +67,25 @@ _SIGS = {
                                  c_vp]),
     "mfd_gdn_commit": (c_int, [c_vp, c_int, c_vp, c_vp, c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64,
                                c_vp]),
+    "mfd_kv8_append": (c_int, [c_vp, c_vp, c_i64, c_i64, c_i64, c_int, c_vp, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64,
+                               c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64,
+                               c_i64, c_vp, c_vp, c_vp]),
+    "mfd_kv8_attention_workspace": (c_size, [c_i64, c_i64, c_i64, c_i64]),
+    "mfd_kv8_attention_tickets": (c_i64, [c_i64, c_i64, c_i64, c_i64]),
+    "mfd_kv8_attention": (c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_int, c_vp, c_vp, c_i64,
+                                  c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64,
+                                  c_i64, c_i64, c_i64, c_i64, c_f32, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_size,
+                                  c_vp, c_i64, c_vp]),
+    "mfd_kv8_page_weights_workspace": (c_size, [c_i64, c_i64, c_i64, c_i64]),
+    "mfd_kv8_page_weights": (c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_int, c_vp, c_i64,
+                                     c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64,
+                                     c_i64, c_i64, c_f32, c_f32, c_vp, c_vp, c_i64, c_vp, c_size, c_vp, c_i64, c_vp]),
+    "mfd_kv8_evict": (c_int, [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp,
+                              c_vp, c_vp]),
     "mfd_conv_commit": (c_int, [c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_vp]),
 }
 
-MFD_F32, MFD_BF16, MFD_I32, MFD_I64 = 0, 1, 2, 3
+MFD_F32, MFD_BF16, MFD_I32, MFD_I64, MFD_I8, MFD_E4M3 = 0, 1, 2, 3, 4, 5
 
 
 def exported_symbols() -> list[str]:
@@ -126,6 +141,26 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
 
 def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def device_index(first: torch.Tensor, *rest: torch.Tensor | None) -> int:
+    """require_cuda for calls whose host time matters: the CUDA device index all the tensors share, without the
+    runtime queries (a CUDA tensor implies a device)."""
+    idx = first.get_device()
+    if idx < 0:
+        require_cuda(first)
+    for t in rest:
+        if t is not None and t.get_device() != idx:
+            require_cuda(first, t)
+    return idx
+
+
+def raw_stream(idx: int) -> int:
+    """The current stream of CUDA device `idx` as an integer."""
+    return _raw_stream(idx) if _raw_stream is not None else torch.cuda.current_stream(idx).cuda_stream
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

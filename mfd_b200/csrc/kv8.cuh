@@ -1,0 +1,209 @@
+// kv8.cuh -- what the kernels of the 8-bit paged K/V cache share: code conversions, page addressing, the tensor
+// instruction of the register kernels, and the limits of the accepted-path lists.
+//
+// A cached value is code * scale with one float32 scale per (page, KV head, tensor).  Both code types are exact in
+// float16 and in bf16 (int8: |c| <= 128; e4m3: 3 fraction bits, 2^-9 .. 448), so products of 16-bit operands lose
+// nothing and the page's scale multiplies a finished dot product (K) or is folded into the softmax weight (V).
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace mfd {
+namespace kv8 {
+
+constexpr int kD = 128;                           // head dim: codes per row
+constexpr float kScaleFloor = 7.888609052210118e-31f;  // 2^-100, the least scale of a page
+
+// One cache tensor pair of a layer; strides in bytes (= codes).
+struct Cache {
+    const uint8_t* k;
+    const uint8_t* v;
+    int64_t sc_p, sc_h, sc_t;
+    const float* k_scale;  // [num_pages, Hkv]
+    const float* v_scale;
+    int64_t num_pages;
+    int page, page_shift;  // tokens per page (a power of two) and its log2
+    const int32_t* table;
+    int64_t table_stride;
+    int max_pages;
+    const int32_t* lens;
+    int Hkv;
+};
+
+__device__ __forceinline__ int seq_len(const Cache& c, int b) {
+    const int cap = c.max_pages << c.page_shift;
+    return min(max(__ldg(c.lens + b), 0), cap);
+}
+// a page id as read from the table, clamped to the pool
+__device__ __forceinline__ int page_id(const Cache& c, int b, int p) {
+    return min(max(__ldg(c.table + (int64_t)b * c.table_stride + p), 0), (int)c.num_pages - 1);
+}
+
+// four codes of a word as two float16 pairs: (bytes 0, 1) and (bytes 2, 3)
+template <bool FP8>
+__device__ __forceinline__ void halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if (FP8) {
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+            : "=r"(lo), "=r"(hi)
+            : "r"(w));
+    } else {
+        // c + 128 as the low byte of the float16 1024 (bits 0x6400, spacing 1), less 1152: exact
+        w ^= 0x80808080u;
+        const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+        uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+        const __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), off);
+        const __half2 y = __hsub2(*reinterpret_cast<__half2*>(&b), off);
+        lo = *reinterpret_cast<const uint32_t*>(&x);
+        hi = *reinterpret_cast<const uint32_t*>(&y);
+    }
+}
+
+// the same as two bf16 pairs
+template <bool FP8>
+__device__ __forceinline__ void bfloats(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if (FP8) {  // through float16 (a NaN code stays NaN)
+        uint32_t a, b;
+        halves<true>(w, a, b);
+        const float2 x = __half22float2(*reinterpret_cast<__half2*>(&a)), y = __half22float2(*reinterpret_cast<__half2*>(&b));
+        const __nv_bfloat162 u = __floats2bfloat162_rn(x.x, x.y), v = __floats2bfloat162_rn(y.x, y.y);
+        lo = *reinterpret_cast<const uint32_t*>(&u);
+        hi = *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+        // the low seven bits on the bf16 128 (bits 0x4300, spacing 1), less 128 or, with the sign bit, 256: exact
+        const uint32_t x = __byte_perm(w, 0x43434343u, 0x4140), y = __byte_perm(w, 0x43434343u, 0x4342);
+        uint32_t xa = x & 0xff7fff7fu, xb = x & 0xff80ff80u, ya = y & 0xff7fff7fu, yb = y & 0xff80ff80u;
+        const __nv_bfloat162 u = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&xa), *reinterpret_cast<__nv_bfloat162*>(&xb));
+        const __nv_bfloat162 v = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&ya), *reinterpret_cast<__nv_bfloat162*>(&yb));
+        lo = *reinterpret_cast<const uint32_t*>(&u);
+        hi = *reinterpret_cast<const uint32_t*>(&v);
+    }
+}
+
+// a pair of weights as bf16 hi + lo (16 bits of each): hi is the rounded weight, lo what it left
+__device__ __forceinline__ void split_bf16(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    const __nv_bfloat162 r = __floats2bfloat162_rn(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
+    lo = *reinterpret_cast<const uint32_t*>(&r);
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// bf16 pair -> the two floats
+__device__ __forceinline__ float2 bf2(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// the power of two 2^-e that brings a row of largest magnitude mx into (-2, 2), and 2^e.  Both are exact, so a bf16
+// query row becomes float16 without loss except below 2^-24 of its largest element, whose products vanish against
+// the row's own rounding.  (A zero or non-finite row is left as it is.)
+__device__ __forceinline__ void row_power(float mx, float& down, float& up) {
+    int e = (int)((__float_as_uint(mx) >> 23) & 0xffu) - 127;
+    if (mx == 0.f || e == 128) e = 0;
+    e = max(e, -126);
+    down = e == 127 ? 5.877471754111438e-39f : __uint_as_float((uint32_t)(127 - e) << 23);  // (2^-127 is subnormal)
+    up = __uint_as_float((uint32_t)(max(e + 127, 1)) << 23);
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint4 ldg_stream_u4(const void* p) {
+    uint4 r;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+                 : "l"(p));
+    return r;
+}
+
+// Rows a request lists: counts[b] (or `rows`), cut at the first path entry outside [0, n).  Called by whole warps.
+__device__ __forceinline__ int listed_rows(const int64_t* path, int64_t path_stride, int rows, const int32_t* counts,
+                                           int n, int b) {
+    int c = counts ? min(max(__ldg(counts + b), 0), rows) : rows;
+    if (!path) return min(c, n);
+    const int lane = threadIdx.x & 31;
+    for (int i = 0; i < c; i += 32) {
+        int64_t e = 0;
+        if (i + lane < c) e = __ldg((const long long*)path + (int64_t)b * path_stride + i + lane);
+        const uint32_t bad = __ballot_sync(MFD_FULL_MASK, e < 0 || e >= n);
+        if (bad) {
+            c = i + __ffs(bad) - 1;
+            break;
+        }
+    }
+    return c;
+}
+
+// Work laid end to end over the requests, f(b) of it for request b; every warp computes where it is by itself.
+// warp-wide sum over requests of f(b)
+template <class F>
+__device__ __forceinline__ int64_t over_requests(int bs, F f) {
+    int64_t sum = 0;
+    for (int b0 = 0; b0 < bs; b0 += 32) {
+        const int b = b0 + (threadIdx.x & 31);
+        const unsigned v = b < bs ? (unsigned)f(b) : 0u;
+        sum += __reduce_add_sync(MFD_FULL_MASK, v);
+    }
+    return sum;
+}
+// the request whose range [before, before + f(b)) contains x, and before
+template <class F>
+__device__ __forceinline__ int find_request(int bs, int64_t x, F f, int64_t& before) {
+    before = 0;
+    for (int b0 = 0; b0 < bs; b0 += 32) {
+        const int lane = threadIdx.x & 31, b = b0 + lane;
+        const int64_t v = b < bs ? f(b) : 0;
+        int64_t inc = v;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int64_t o = __shfl_up_sync(MFD_FULL_MASK, inc, d);
+            if (lane >= d) inc += o;
+        }
+        const uint32_t hit = __ballot_sync(MFD_FULL_MASK, before + inc > x);
+        if (hit) {
+            const int l = __ffs(hit) - 1;
+            before += __shfl_sync(MFD_FULL_MASK, inc - v, l);
+            return b0 + l;
+        }
+        before += __shfl_sync(MFD_FULL_MASK, inc, 31);
+    }
+    return -1;
+}
+
+__device__ __forceinline__ float quad_max(float v) {
+    v = fmaxf(v, __shfl_xor_sync(MFD_FULL_MASK, v, 1));
+    return fmaxf(v, __shfl_xor_sync(MFD_FULL_MASK, v, 2));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+    v += __shfl_xor_sync(MFD_FULL_MASK, v, 1);
+    return v + __shfl_xor_sync(MFD_FULL_MASK, v, 2);
+}
+// SMs of the current device, and the opt-in to a kernel's dynamic shared memory, asked of the driver once per device
+int sm_count();
+cudaError_t opt_in_smem(const void* kernel, int bytes, bool (&done)[64]);
+
+// host checks shared by the entry points; false after set_error
+bool check_cache(const char* who, const void* k, const void* v, int64_t sc_p, int64_t sc_h, int64_t sc_t,
+                 int code_dtype, int64_t num_pages, int64_t page_size, const int32_t* table, int64_t max_pages,
+                 const int32_t* lens, int64_t bs, int64_t hkv, int64_t head_dim, int* status);
+
+}  // namespace kv8
+}  // namespace mfd

@@ -1,0 +1,87 @@
+// kv8_attention.cu -- C entry point of the attention over the 8-bit paged cache: checks, and which kernel takes the
+// rows.
+#include "kv8_attention.cuh"
+
+using namespace mfd;
+
+static int kv8_rows_total(int64_t n, int64_t H, int64_t Hkv) { return (int)(n * (H / Hkv)); }
+
+static bool kv8_sizes_ok(int64_t bs, int64_t n, int64_t H, int64_t Hkv) {
+    return bs >= 0 && n > 0 && n <= 4096 && H > 0 && Hkv > 0 && H % Hkv == 0 && H <= 16384;
+}
+
+extern "C" size_t mfd_kv8_attention_workspace(int64_t bs, int64_t n, int64_t num_heads, int64_t num_kv_heads) {
+    if (!kv8_sizes_ok(bs, n, num_heads, num_kv_heads)) return 0;
+    return 512 + kv8::rows_workspace(kv8::sm_count());
+}
+
+extern "C" int64_t mfd_kv8_attention_tickets(int64_t bs, int64_t n, int64_t num_heads, int64_t num_kv_heads) {
+    if (!kv8_sizes_ok(bs, n, num_heads, num_kv_heads)) return 0;
+    return kv8::rows_tickets(bs, num_kv_heads, kv8_rows_total(n, num_heads, num_kv_heads));
+}
+
+extern "C" int mfd_kv8_attention(const void* q, int64_t sq_b, int64_t sq_n, int64_t sq_h, const void* k_cache,
+                                 const void* v_cache, int64_t sc_p, int64_t sc_h, int64_t sc_t, int code_dtype,
+                                 const float* k_scale, const float* v_scale, int64_t num_pages, int64_t page_size,
+                                 const int32_t* page_table, int64_t table_stride, int64_t max_pages,
+                                 const int32_t* seq_lens, const void* k_new, const void* v_new, int64_t sn_b,
+                                 int64_t sn_n, int64_t sn_h, const uint64_t* anc_bits, int64_t anc_words, int64_t bs,
+                                 int64_t n, int64_t num_heads, int64_t num_kv_heads, int64_t head_dim, float scale,
+                                 void* out, int64_t so_b, int64_t so_n, int64_t so_h, float* lse, void* workspace,
+                                 size_t workspace_bytes, unsigned int* tickets, int64_t tickets_len, void* stream) {
+    const char* who = "mfd_kv8_attention";
+    int st;
+    if (!kv8::check_cache(who, k_cache, v_cache, sc_p, sc_h, sc_t, code_dtype, num_pages, page_size, page_table,
+                          max_pages, seq_lens, bs, num_kv_heads, head_dim, &st))
+        return st;
+    if (!q || !out || !k_scale || !v_scale || !workspace || !tickets || (k_new == nullptr) != (v_new == nullptr)) {
+        set_error("%s: null pointer", who);
+        return MFD_ERR_INVALID;
+    }
+    if (n <= 0 || num_heads <= 0 || num_heads % num_kv_heads || (anc_bits && anc_words < (n + 63) / 64)) {
+        set_error("%s: invalid sizes (n %lld, %lld query heads over %lld KV heads, %lld mask words)", who, (long long)n,
+                  (long long)num_heads, (long long)num_kv_heads, (long long)anc_words);
+        return MFD_ERR_INVALID;
+    }
+    if (!kv8_sizes_ok(bs, n, num_heads, num_kv_heads)) {
+        set_error("%s: more than 4096 nodes or 16384 heads", who);
+        return MFD_ERR_UNSUPPORTED;
+    }
+    if (sq_b % 8 || sq_n % 8 || sq_h % 8 || so_b % 8 || so_n % 8 || so_h % 8 || (uintptr_t)q % 16 ||
+        (uintptr_t)out % 16 || (k_new && (sn_b % 8 || sn_n % 8 || sn_h % 8 || (uintptr_t)k_new % 16 || (uintptr_t)v_new % 16))) {
+        set_error("%s: rows need strides that are multiples of 8 elements and 16-byte aligned bases", who);
+        return MFD_ERR_INVALID;
+    }
+    const int64_t base = ((uintptr_t)workspace + 255) / 256 * 256 - (uintptr_t)workspace;
+    if (workspace_bytes < mfd_kv8_attention_workspace(bs, n, num_heads, num_kv_heads) ||
+        tickets_len < mfd_kv8_attention_tickets(bs, n, num_heads, num_kv_heads)) {
+        set_error("%s: workspace or tickets too small", who);
+        return MFD_ERR_INVALID;
+    }
+    if (bs == 0) return MFD_OK;
+    kv8::AttnParams p;
+    p.c.k = (const uint8_t*)k_cache, p.c.v = (const uint8_t*)v_cache;
+    p.c.sc_p = sc_p, p.c.sc_h = sc_h, p.c.sc_t = sc_t;
+    p.c.k_scale = k_scale, p.c.v_scale = v_scale;
+    p.c.num_pages = num_pages;
+    p.c.page = (int)page_size, p.c.page_shift = __builtin_ctz((unsigned)page_size);
+    p.c.table = page_table, p.c.table_stride = table_stride, p.c.max_pages = (int)max_pages;
+    p.c.lens = seq_lens;
+    p.c.Hkv = (int)num_kv_heads;
+    p.fp8 = code_dtype == MFD_E4M3;
+    p.q = (const __nv_bfloat16*)q, p.sq_b = sq_b, p.sq_n = sq_n, p.sq_h = sq_h;
+    p.kn = (const __nv_bfloat16*)k_new, p.vn = (const __nv_bfloat16*)v_new;
+    p.sn_b = sn_b, p.sn_n = sn_n, p.sn_h = sn_h;
+    p.anc = anc_bits, p.words = (int)anc_words;
+    p.bs = (int)bs, p.n = (int)n, p.H = (int)num_heads, p.G = (int)(num_heads / num_kv_heads);
+    p.nn = k_new ? (int)n : 0;
+    p.row0 = 0, p.rows = kv8_rows_total(n, num_heads, num_kv_heads);
+    p.scale_log2 = scale * kLog2e;
+    p.out = (__nv_bfloat16*)out, p.so_b = so_b, p.so_n = so_n, p.so_h = so_h;
+    p.lse = lse;
+    char* ws = (char*)workspace + base;
+    p.status = (int*)ws;
+    p.part = (float*)(ws + 256);
+    p.tickets = tickets;
+    return kv8::launch_rows(p, kv8::sm_count(), (cudaStream_t)stream);
+}

@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._lib import MFD_BF16, MFD_F32, MFD_I32, MFD_I64, Workspace, check, ptr, require_cuda, stream_ptr
+from ._lib import MFD_BF16, MFD_E4M3, MFD_F32, MFD_I8, MFD_I32, MFD_I64, Workspace, check, device_index, ptr, raw_stream, require_cuda, stream_ptr
 
 
 def _ids_code(dtype: torch.dtype) -> int:
@@ -586,3 +586,227 @@ def conv_commit(conv_states, xs, window) -> None:
     rc = _lib.lib().mfd_conv_commit(pa.data_ptr(), pa.data_ptr() + 8 * nl, conv_states[0].element_size(), nl,
                                     conv_dim, kernel, win.data_ptr(), stream_ptr(dev))
     check(rc, "mfd_conv_commit")
+
+
+# ----------------------------------------------------------------------------------------------- 8-bit paged K/V cache
+
+_KV8_CODES = {torch.int8: MFD_I8, torch.float8_e4m3fn: MFD_E4M3}
+
+
+def _kv8_check(what: str, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens):
+    """The cache's checks; its shape, strides and code type."""
+    shape, strides = k_cache.shape, k_cache.stride()
+    code = _KV8_CODES.get(k_cache.dtype)
+    if code is None:
+        raise RuntimeError(f"{what}: cache codes must be int8 or float8_e4m3fn, got {k_cache.dtype}")
+    if len(shape) != 4 or strides[3] != 1:
+        raise RuntimeError(f"{what}: caches must be [pages, KV heads, page_size, D] with a contiguous last dim")
+    if v_cache is not k_cache and (v_cache.shape != shape or v_cache.dtype != k_cache.dtype
+                                   or v_cache.stride() != strides):
+        raise RuntimeError(f"{what}: k_cache and v_cache need the same dtype, shape and strides")
+    for s in (k_scale, v_scale) if v_scale is not k_scale else (k_scale,):
+        if s.dtype != torch.float32 or s.shape != shape[:2] or not s.is_contiguous():
+            raise RuntimeError(f"{what}: scales must be contiguous float32 [pages, KV heads]")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1:
+        raise RuntimeError(f"{what}: page_table must be int32 [bs, max_pages] with a contiguous last dim")
+    if seq_lens.dtype != torch.int32 or seq_lens.shape != page_table.shape[:1] or not seq_lens.is_contiguous():
+        raise RuntimeError(f"{what}: seq_lens must be contiguous int32 [bs]")
+    return shape, strides, code
+
+
+def _kv8_rows(what: str, rows: torch.Tensor, name: str, shape):
+    """Checks rows [bs, n, heads, D]; their strides."""
+    if rows.dtype != torch.bfloat16 or rows.shape != shape:
+        raise RuntimeError(f"{what}: {name} must be bfloat16 {tuple(shape)}, got {rows.dtype} {tuple(rows.shape)}")
+    strides = rows.stride()
+    if strides[3] != 1:
+        raise RuntimeError(f"{what}: {name} needs a contiguous last dim")
+    return strides
+
+
+def _kv8_new(what: str, k_new: torch.Tensor, v_new: torch.Tensor, shape):
+    strides = _kv8_rows(what, k_new, "k_new", shape)
+    if _kv8_rows(what, v_new, "v_new", shape) != strides:
+        raise RuntimeError(f"{what}: k_new and v_new need the same strides")
+    return strides
+
+
+def _kv8_path(what: str, bs: int, n: int, path, counts):
+    if path is not None and (path.dtype != torch.int64 or path.dim() != 2 or path.shape[0] != bs
+                             or path.stride(1) != 1):
+        raise RuntimeError(f"{what}: path must be int64 [bs, rows] with a contiguous last dim")
+    if counts is not None and (counts.dtype != torch.int32 or counts.shape != (bs,) or not counts.is_contiguous()):
+        raise RuntimeError(f"{what}: counts must be contiguous int32 [bs]")
+    return (path.stride(0), path.shape[1]) if path is not None else (0, n)
+
+
+def kv8_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+               k_new: torch.Tensor, v_new: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+               path: torch.Tensor | None = None, counts: torch.Tensor | None = None,
+               new_lens: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """Quantise rows of k_new, v_new [bs, n, Hkv, 128] bf16 into the pages of an 8-bit cache, in place.
+
+    k_cache, v_cache [pages, Hkv, page_size, 128] int8 or float8_e4m3fn; k_scale, v_scale [pages, Hkv] f32: a value is
+    code * scale.  page_table int32 [bs, max_pages], seq_lens int32 [bs] (before the call).  Request b appends the
+    nodes path[b, :counts[b]] (path int64 [bs, rows], as accept's "accepted", ended by -1; None: rows 0 .. counts - 1;
+    counts as accept's "commit_lens"; None: all).  Returns the new lengths (a tensor of their own)."""
+    dev = device_index(k_cache, v_cache, k_scale, v_scale, k_new, v_new, page_table, seq_lens, path, counts, new_lens,
+                       status)
+    (pages, hkv, page, d), sc, code = _kv8_check("kv8_append", k_cache, v_cache, k_scale, v_scale, page_table, seq_lens)
+    bs, width = page_table.shape
+    n = k_new.shape[1]
+    sn = _kv8_new("kv8_append", k_new, v_new, (bs, n, hkv, d))
+    path_stride, rows = _kv8_path("kv8_append", bs, n, path, counts)
+    if new_lens is None:
+        new_lens = torch.empty_like(seq_lens)
+    elif new_lens.dtype != torch.int32 or new_lens.shape != seq_lens.shape or not new_lens.is_contiguous():
+        raise RuntimeError("kv8_append: new_lens must be contiguous int32 [bs]")
+    rc = _lib.lib().mfd_kv8_append(k_cache.data_ptr(), v_cache.data_ptr(), sc[0], sc[1], sc[2], code,
+                                   k_scale.data_ptr(), v_scale.data_ptr(), pages, page, page_table.data_ptr(),
+                                   page_table.stride(0), width, seq_lens.data_ptr(), k_new.data_ptr(),
+                                   v_new.data_ptr(), sn[0], sn[1], sn[2], n, ptr(path), path_stride, rows, ptr(counts),
+                                   bs, hkv, d, new_lens.data_ptr(), ptr(status), raw_stream(dev))
+    check(rc, "mfd_kv8_append")
+    return new_lens
+
+
+_KV8_WORK: dict = {}
+
+
+def _kv8_scratch(dev: torch.device, stream: int, purpose: str, nbytes: int, tickets: int):
+    """Workspace and zeroed ticket words of one stream: calls on different streams may overlap on the GPU, so the
+    operators of the 8-bit cache share neither between streams."""
+    return (Workspace.get(dev, (purpose, stream), nbytes),
+            Workspace.get(dev, (purpose, "tickets", stream), 4 * tickets))
+
+
+def kv8_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                  v_scale: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, scale: float,
+                  k_new: torch.Tensor | None = None, v_new: torch.Tensor | None = None,
+                  anc: torch.Tensor | None = None, out: torch.Tensor | None = None, return_lse: bool = False):
+    """Attention of q [bs, n, H, 128] bf16 over an 8-bit cache (see kv8_append) and the nodes' own keys.
+
+    Every node sees all seq_lens[b] cached tokens and, of k_new, v_new [bs, n, Hkv, 128] bf16, the nodes whose bits are
+    set in its row of anc [bs, n, words] int64 (ancestor-or-self bitsets, mfd_build_trees; None: nodes up to itself).
+    n = 1 is a decode step.  Returns out [bs, n, H, 128] bf16, or (out, lse) with lse f32 [bs, n, H] the natural
+    log-sum-exp of every row's scaled scores.  Rows that see nothing give 0 and -inf."""
+    dev = device_index(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, k_new, v_new, anc, out)
+    (pages, hkv, page, d), sc, code = _kv8_check("kv8_attention", k_cache, v_cache, k_scale, v_scale, page_table,
+                                                 seq_lens)
+    bs, width = page_table.shape
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != bs or shape[3] != d:
+        raise RuntimeError(f"kv8_attention: q must be [bs, n, H, D] for {bs} requests, D = {d}; got {tuple(shape)}")
+    _, n, H, _ = shape
+    sq = _kv8_rows("kv8_attention", q, "q", shape)
+    sn, kn, vn = (0, 0, 0), None, None
+    if k_new is not None and v_new is not None:
+        sn, kn, vn = _kv8_new("kv8_attention", k_new, v_new, (bs, n, hkv, d)), k_new.data_ptr(), v_new.data_ptr()
+    elif k_new is not v_new:
+        raise RuntimeError("kv8_attention: k_new and v_new come together")
+    ab, words = None, 0
+    if anc is not None:
+        if anc.dtype != torch.int64 or anc.dim() != 3 or anc.shape[:2] != shape[:2] or not anc.is_contiguous():
+            raise RuntimeError("kv8_attention: anc must be contiguous int64 [bs, n, words]")
+        ab, words = anc.data_ptr(), anc.shape[2]
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
+    so = _kv8_rows("kv8_attention", out, "out", shape)
+    lse = torch.empty(shape[:3], dtype=torch.float32, device=q.device) if return_lse else None
+    L = _lib.lib()
+    key = (dev, bs, n, H, hkv)
+    need = _KV8_WORK.get(key)
+    if need is None:
+        with torch.cuda.device(dev):
+            need = (L.mfd_kv8_attention_workspace(bs, n, H, hkv), L.mfd_kv8_attention_tickets(bs, n, H, hkv))
+        if len(_KV8_WORK) >= 4096:
+            _KV8_WORK.clear()
+        _KV8_WORK[key] = need
+    stream = raw_stream(dev)
+    ws, tk = _kv8_scratch(q.device, stream, "kv8_attn", *need)
+    rc = L.mfd_kv8_attention(q.data_ptr(), sq[0], sq[1], sq[2], k_cache.data_ptr(), v_cache.data_ptr(), sc[0], sc[1],
+                             sc[2], code, k_scale.data_ptr(), v_scale.data_ptr(), pages, page, page_table.data_ptr(),
+                             page_table.stride(0), width, seq_lens.data_ptr(), kn, vn, sn[0], sn[1], sn[2], ab, words,
+                             bs, n, H, hkv, d, scale, out.data_ptr(), so[0], so[1], so[2], ptr(lse), ws.data_ptr(),
+                             ws.numel(), tk.data_ptr(), tk.numel() // 4, stream)
+    check(rc, "mfd_kv8_attention")
+    return (out, lse) if return_lse else out
+
+
+def kv8_attention_status(device=None) -> int:
+    """The sticky status word of kv8_attention's workspace for the current stream: 0, or 1 once a bounded wait in a
+    kernel gave up.  0 when no such call has run on the stream."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    idx = dev.index if dev.index is not None else torch.cuda.current_device()
+    ws = Workspace._cache.get((idx, ("kv8_attn", stream_ptr(dev))))
+    if ws is None:
+        return 0
+    off = (-ws.data_ptr()) % 256
+    return int(ws[off:off + 4].view(torch.int32).item())
+
+
+def kv8_page_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Tensor,
+                     page_table: torch.Tensor, seq_lens: torch.Tensor, scale: float, mass: torch.Tensor,
+                     path: torch.Tensor | None = None, counts: torch.Tensor | None = None, decay: float = 1.0,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """The attention weight each cached page received from the listed nodes of q [bs, n, H, 128], added to its mass:
+    out = decay * mass + sum of exp(q . k * scale - lse) over heads, nodes path[b, :counts[b]] (as in kv8_append) and
+    the page's tokens; 0 past a request's pages.  lse f32 [bs, n, H] from kv8_attention on the same cache (before the
+    nodes are appended); mass f32 [bs, max_pages]; out may be mass.  The sums run in a fixed order."""
+    dev = device_index(q, lse, k_cache, k_scale, page_table, seq_lens, mass, path, counts, out)
+    (pages, hkv, page, d), sc, code = _kv8_check("kv8_page_weights", k_cache, k_cache, k_scale, k_scale, page_table,
+                                                 seq_lens)
+    table_shape = page_table.shape
+    bs, width = table_shape
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != bs or shape[3] != d:
+        raise RuntimeError(f"kv8_page_weights: q must be [bs, n, H, D] for {bs} requests, D = {d}; got {tuple(shape)}")
+    _, n, H, _ = shape
+    sq = _kv8_rows("kv8_page_weights", q, "q", shape)
+    if lse.dtype != torch.float32 or lse.shape != shape[:3] or not lse.is_contiguous():
+        raise RuntimeError("kv8_page_weights: lse must be contiguous float32 [bs, n, H]")
+    path_stride, rows = _kv8_path("kv8_page_weights", bs, n, path, counts)
+    if mass.dtype != torch.float32 or mass.shape != table_shape or not mass.is_contiguous():
+        raise RuntimeError("kv8_page_weights: mass must be contiguous float32 [bs, max_pages]")
+    if out is None:
+        out = torch.empty_like(mass)
+    elif out.dtype != torch.float32 or out.shape != table_shape or not out.is_contiguous():
+        raise RuntimeError("kv8_page_weights: out must be contiguous float32 [bs, max_pages]")
+    L = _lib.lib()
+    stream = raw_stream(dev)
+    ws, tk = _kv8_scratch(q.device, stream, "kv8_weights", L.mfd_kv8_page_weights_workspace(bs, width, page, hkv), bs)
+    rc = L.mfd_kv8_page_weights(q.data_ptr(), sq[0], sq[1], sq[2], lse.data_ptr(), k_cache.data_ptr(), sc[0], sc[1],
+                                sc[2], code, k_scale.data_ptr(), pages, page, page_table.data_ptr(),
+                                page_table.stride(0), width, seq_lens.data_ptr(), ptr(path), path_stride, rows,
+                                ptr(counts), bs, n, H, hkv, d, scale, decay, mass.data_ptr(), out.data_ptr(), width,
+                                ws.data_ptr(), ws.numel(), tk.data_ptr(), tk.numel() // 4, stream)
+    check(rc, "mfd_kv8_page_weights")
+    return out
+
+
+def kv8_evict(page_table: torch.Tensor, mass: torch.Tensor, seq_lens: torch.Tensor, page_size: int, keep_pages: int,
+              sink_pages: int, recent_pages: int):
+    """Shorten every request of more than keep_pages pages: its first sink_pages and last recent_pages (>= 1) pages
+    stay, and of the others those of the largest mass (ties: the earlier page), keep_pages in all.
+
+    page_table int32 and mass f32 [bs, max_pages], seq_lens int32 [bs].  Returns new tensors (page_table, mass,
+    seq_lens, freed, freed_counts): table and mass compacted in order (-1 and 0 after them), freed int32 [bs,
+    max_pages] the dropped page ids in order (-1 after them), freed_counts int32 [bs].  No cache byte moves."""
+    dev = device_index(page_table, mass, seq_lens)
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous():
+        raise RuntimeError("kv8_evict: page_table must be contiguous int32 [bs, max_pages]")
+    if mass.dtype != torch.float32 or mass.shape != page_table.shape or not mass.is_contiguous():
+        raise RuntimeError("kv8_evict: mass must be contiguous float32 [bs, max_pages]")
+    if seq_lens.dtype != torch.int32 or seq_lens.shape != page_table.shape[:1] or not seq_lens.is_contiguous():
+        raise RuntimeError("kv8_evict: seq_lens must be contiguous int32 [bs]")
+    bs, width = page_table.shape
+    table = torch.empty_like(page_table)
+    kept = torch.empty_like(mass)
+    freed = torch.empty_like(page_table)
+    lens = torch.empty_like(seq_lens)
+    counts = torch.empty_like(seq_lens)
+    rc = _lib.lib().mfd_kv8_evict(page_table.data_ptr(), mass.data_ptr(), seq_lens.data_ptr(), bs, width, page_size,
+                                  keep_pages, sink_pages, recent_pages, table.data_ptr(), kept.data_ptr(),
+                                  lens.data_ptr(), freed.data_ptr(), counts.data_ptr(), raw_stream(dev))
+    check(rc, "mfd_kv8_evict")
+    return table, kept, lens, freed, counts
