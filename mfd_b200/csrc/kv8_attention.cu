@@ -6,13 +6,17 @@ using namespace mfd;
 
 static int kv8_rows_total(int64_t n, int64_t H, int64_t Hkv) { return (int)(n * (H / Hkv)); }
 
+// Rows of a (request, KV head) up to which the register kernel takes them all.
+constexpr int kRowsAlone = 16;
+
 static bool kv8_sizes_ok(int64_t bs, int64_t n, int64_t H, int64_t Hkv) {
     return bs >= 0 && n > 0 && n <= 4096 && H > 0 && Hkv > 0 && H % Hkv == 0 && H <= 16384;
 }
 
 extern "C" size_t mfd_kv8_attention_workspace(int64_t bs, int64_t n, int64_t num_heads, int64_t num_kv_heads) {
     if (!kv8_sizes_ok(bs, n, num_heads, num_kv_heads)) return 0;
-    return 512 + kv8::rows_workspace(kv8::sm_count());
+    const size_t rows = kv8::rows_workspace(kv8::sm_count()), tc = kv8::tc_workspace(kv8::sm_count());
+    return 512 + (kv8_rows_total(n, num_heads, num_kv_heads) <= kRowsAlone || rows > tc ? rows : tc);
 }
 
 extern "C" int64_t mfd_kv8_attention_tickets(int64_t bs, int64_t n, int64_t num_heads, int64_t num_kv_heads) {
@@ -83,5 +87,15 @@ extern "C" int mfd_kv8_attention(const void* q, int64_t sq_b, int64_t sq_n, int6
     p.status = (int*)ws;
     p.part = (float*)(ws + 256);
     p.tickets = tickets;
-    return kv8::launch_rows(p, kv8::sm_count(), (cudaStream_t)stream);
+    const int sms = kv8::sm_count(), rows = p.rows;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (rows <= kRowsAlone) return kv8::launch_rows(p, sms, s);
+    // pairs of 128-row tiles; a remainder of a few rows goes to the register kernel instead of a tile of padding
+    const int rest = rows % 256;
+    const bool tail = rows > 256 && rest > 0 && rest <= kRowsAlone;
+    if (tail) p.rows = rows - rest;
+    st = kv8::launch_tc(p, rows > 128, sms, s);
+    if (st != MFD_OK || !tail) return st;
+    p.row0 = rows - rest, p.rows = rows;
+    return kv8::launch_rows(p, sms, s);
 }

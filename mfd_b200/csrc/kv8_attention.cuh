@@ -33,6 +33,10 @@ int launch_rows(const AttnParams& p, int sms, cudaStream_t stream);
 int64_t rows_tickets(int64_t bs, int64_t hkv, int64_t rows);
 size_t rows_workspace(int sms);
 
+// the same with the tensor-core kernel (tiles of 128 rows; pair: two tiles a CTA), and its combination of pieces
+int launch_tc(const AttnParams& p, bool pair, int sms, cudaStream_t stream);
+size_t tc_workspace(int sms);
+
 // 64 visibility bits of own keys [64 w, 64 w + 64) for a node
 __device__ __forceinline__ uint64_t visible_word(const AttnParams& p, int b, int node, int w) {
     const int left = p.nn - 64 * w;

@@ -1,0 +1,734 @@
+// kv8_attention_tc.cu -- attention of many query rows (trees, long drafts) over the 8-bit paged cache on the
+// 5th-generation tensor cores (tcgen05 + TMEM).
+//
+// The mathematics is that of kv8_attention_rows.cu, with every operand in bf16 (the codes, the queries and the nodes'
+// own keys and values are exact there; the weights go in as hi + lo, 16 bits of each):
+//   S = Q K8^T,  w = sk scale log2(e) S + log2(sv),  P = 2^(w - m) = P_hi + P_lo,  O = P_hi V8 + P_lo V8,
+//   l = sum P / sv,  out = O / l.
+//
+// Rows r = node * G + g of a (request, KV head) in tiles of 128 (one row per TMEM lane).  Two softmax groups of four
+// warps, each with its own S buffer and O accumulator in TMEM, so one group's softmax runs while the other's products
+// do:
+//   PAIR   a CTA takes two row tiles; each key tile, converted once, feeds 256 rows (group t = row tile t)
+//   single a CTA takes one row tile; group t takes every other key tile and the two (m, l, O) merge at the end
+// In both, step s is group s & 1; the products run PV(s), S(s + 2) in order.
+//
+// Warp roles (448 threads, one CTA an SM):
+//   warps 0-7    softmax, thread = row; 128 scores read from TMEM twice (maximum, then weights) instead of held
+//   warps 8-11   converters: raw codes -> bf16 tiles in the 128-byte-swizzled operand layout; the nodes' own keys are
+//                copied there (past the end of a request: zeros, whatever the page holds)
+//   warp 12      producer: page ids and scales, one TMA load per page and tensor into the raw ring (no multicast)
+//   warp 13      MMA issuer
+// Shared memory: Q (32 KB a row tile), K tile 32 KB, V tiles 2 x 32 KB, raw ring 32 KB a stage.  K needs one buffer: it
+// is free from the last S of its tile to the end of the next PV, and the PV of hi + lo is the longer product.
+//
+// Bound: the tensor pipe and shared memory together.  A key tile of 128 costs a pair of row tiles 4 S and 8 PV
+// products of 128 x 128 x 64, 3072 cycles of the tensor pipe at its bf16 rate, and about the same of the
+// 128 B/clk shared-memory port (operands 256 KB, conversion 96 KB, raw codes 32 KB); the exponentials are 2048.
+//
+// Split: as in kv8_attention_rows.cu, in key tiles of 128: equal ranges of all units' tiles laid end to end, or at most
+// one piece a CTA when there are few units.  Pieces leave (m, l, O) and kv8_combine_kernel adds them in order, spread
+// over the GPU (one CTA reading all pieces of 256 rows would take longer than the attention at batch 1).
+//
+// Every mbarrier wait is bounded; a CTA whose wait gave up records status 1, stops and releases its TMEM.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include "kv8_attention.cuh"
+#include "tcgen05.cuh"
+
+namespace mfd {
+namespace kv8 {
+
+namespace {
+
+constexpr int kTcThreads = 448;
+constexpr int kKt = 128;                 // keys per tile
+constexpr int kTileBytes = kKt * kD * 2;  // 32 KB: a bf16 tile, [2 d-halves][128 rows][128 B]
+constexpr int kRawBytes = 2 * kKt * kD;   // 32 KB: the codes of K and V
+constexpr int kRing = 8;                 // tiles of page constants kept
+constexpr uint32_t kTries = 1u << 20;
+
+template <bool PAIR>
+struct Layout {
+    static constexpr int kRowTiles = PAIR ? 2 : 1;
+    static constexpr int kStages = PAIR ? 2 : 3;
+    static constexpr int kOffQ = 0;
+    static constexpr int kOffK = kOffQ + kRowTiles * kTileBytes;
+    static constexpr int kOffV = kOffK + kTileBytes;
+    static constexpr int kOffRaw = kOffV + 2 * kTileBytes;
+    static constexpr int kOffConst = kOffRaw + kStages * kRawBytes;  // [kRing][8 groups][4] floats: c, d, 1 / sv
+    static constexpr int kOffBar = kOffConst + kRing * 8 * 4 * 4;
+    static constexpr int kUsed = kOffBar + 512;
+    static constexpr int kBytes = kUsed + 1024;  // the base is aligned to 1024 by hand
+    static_assert(kBytes <= 227 * 1024, "shared memory");
+    // barriers
+    static constexpr int kQFull = 0;
+    static constexpr int kRawFull = 1;
+    static constexpr int kRawEmpty = kRawFull + kStages;
+    static constexpr int kKFull = kRawEmpty + kStages;
+    static constexpr int kKEmpty = kKFull + 1;
+    static constexpr int kVFull = kKEmpty + 1;
+    static constexpr int kVEmpty = kVFull + 2;
+    static constexpr int kSFull = kVEmpty + 2;
+    static constexpr int kPFull = kSFull + 2;
+    static constexpr int kPV = kPFull + 2;
+    static constexpr int kBars = kPV + 2;
+    static_assert(8 * kBars + 32 <= 512, "barriers");
+};
+
+constexpr int kSlotRows(bool pair) { return pair ? 256 : 128; }
+// floats of a partial: m, l per row, then O as float4 chunks, chunk-major (a warp stores 512 contiguous bytes)
+constexpr int64_t kSlotFloats(bool pair) { return (int64_t)kSlotRows(pair) * (2 + kD); }
+
+__device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int head, int page) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
+        "%5}], [%6];" ::"r"(dst),
+        "l"(map), "r"(0), "r"(0), "r"(head), "r"(page), "r"(smem_addr(bar))
+        : "memory");
+}
+
+// The pieces of the work, shared by the attention and the combination.
+struct Work {
+    int64_t total, per;
+    bool split;
+    int RB, per_req;
+};
+__device__ __forceinline__ int tiles_of(const AttnParams& p, int b) {
+    return max(1, (seq_len(p.c, b) + kKt - 1) / kKt + (p.nn + kKt - 1) / kKt);
+}
+__device__ __forceinline__ Work make_work(const AttnParams& p, int rows_per_unit, int ctas) {
+    Work w;
+    w.RB = (p.rows - p.row0 + rows_per_unit - 1) / rows_per_unit;
+    w.per_req = p.c.Hkv * w.RB;
+    const int64_t units = (int64_t)p.bs * w.per_req;
+    w.total = over_requests(p.bs, [&](int b) { return tiles_of(p, b); }) * w.per_req;
+    w.split = units * 2 <= (int64_t)ctas;
+    w.per = w.split ? (w.total + ctas - units - 1) / (ctas - units) : (w.total + ctas - 1) / ctas;
+    if (w.per < 1) w.per = 1;
+    return w;
+}
+
+struct Piece {
+    int b, hk, rb, t0, t1, tiles, slot, pieces;
+};
+// the piece of CTA `cta` that starts at `pos` (range mode: a tile index; split mode: the piece index); moves pos on
+__device__ __forceinline__ bool next_piece(const AttnParams& p, const Work& w, int cta, int64_t& pos, int64_t end,
+                                           Piece& pc) {
+    if (pos >= end) return false;
+    int64_t before;
+    if (w.split) {
+        pc.b = find_request(p.bs, pos, [&](int b) { return (int64_t)w.per_req * ((tiles_of(p, b) + w.per - 1) / w.per); },
+                            before);
+        if (pc.b < 0) return false;
+        pc.tiles = tiles_of(p, pc.b);
+        pc.pieces = (int)((pc.tiles + w.per - 1) / w.per);
+        const int64_t off = pos - before;
+        const int u = (int)(off / pc.pieces), i = (int)(off % pc.pieces);
+        pc.hk = u / w.RB, pc.rb = u % w.RB;
+        pc.t0 = (int)(i * w.per), pc.t1 = (int)min((int64_t)pc.tiles, (i + 1) * w.per);
+        pc.slot = 2 * cta;
+        pos = end;
+    } else {
+        pc.b = find_request(p.bs, pos, [&](int b) { return (int64_t)w.per_req * tiles_of(p, b); }, before);
+        if (pc.b < 0) return false;
+        pc.tiles = tiles_of(p, pc.b);
+        const int64_t off = pos - before;
+        const int u = (int)(off / pc.tiles);
+        pc.hk = u / w.RB, pc.rb = u % w.RB;
+        pc.t0 = (int)(off % pc.tiles);
+        pc.t1 = (int)min((int64_t)pc.tiles, pc.t0 + (end - pos));
+        const int64_t lo = pos - pc.t0;
+        pc.pieces = (int)((lo + pc.tiles - 1) / w.per - lo / w.per) + 1;
+        pc.slot = 2 * cta + (pos == (int64_t)cta * w.per ? 0 : 1);
+        pos += pc.t1 - pc.t0;
+    }
+    return true;
+}
+
+template <int N>
+__device__ __forceinline__ void bar_sync(int id) {
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
+}
+
+template <bool FP8, bool PAIR>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    kv8_tc_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const AttnParams p) {
+    using L = Layout<PAIR>;
+    constexpr int kStages = L::kStages;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    const uint32_t pad = (1024u - (smem_addr(smem_raw) & 1023u)) & 1023u;
+    unsigned char* smem = smem_raw + pad;
+    const uint32_t sbase = smem_addr(smem);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffBar + 8 * L::kBars);
+    volatile int* s_failed = reinterpret_cast<volatile int*>(smem + L::kOffBar + 8 * L::kBars + 4);
+    volatile int* s_odd = s_failed + 1;  // a non-finite own value was met in this piece
+    float4* consts = reinterpret_cast<float4*>(smem + L::kOffConst);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        mbar_init(&bars[L::kQFull], 8);
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&bars[L::kRawFull + i], 32);
+            mbar_init(&bars[L::kRawEmpty + i], 4);
+        }
+        mbar_init(&bars[L::kKFull], 4);
+        mbar_init(&bars[L::kKEmpty], 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars[L::kVFull + i], 4);
+            mbar_init(&bars[L::kVEmpty + i], 1);
+            mbar_init(&bars[L::kSFull + i], 1);
+            mbar_init(&bars[L::kPFull + i], 4);
+            mbar_init(&bars[L::kPV + i], 1);
+        }
+        *s_failed = 0;
+        *s_odd = 0;
+        mbar_fence_init();
+    }
+    if (warp == 13) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    // TMEM columns: O of group t at 128 t, S of group t at 256 + 128 t
+    const Work w = make_work(p, 128 * L::kRowTiles, gridDim.x);
+    int64_t pos = w.split ? blockIdx.x : (int64_t)blockIdx.x * w.per;
+    const int64_t end = w.split ? pos + 1 : min(w.total, pos + w.per);
+
+    // counters that run on over the CTA's pieces (barrier phases)
+    uint32_t n_piece = 0, n_raw = 0, n_k = 0, n_v = 0, n_s[2] = {0u, 0u};
+    uint32_t issued = 0;  // producer: raw stages filled
+    bool ok = true;
+    Piece pc;
+    while (next_piece(p, w, blockIdx.x, pos, end, pc)) {
+        const int len = seq_len(p.c, pc.b);
+        const int tp = (len + kKt - 1) / kKt;  // tiles of cached tokens, then own keys
+        const int tn = (p.nn + kKt - 1) / kKt;
+        const int t1 = min(pc.t1, tp + tn);      // (a unit without keys has one empty tile: nothing runs)
+        const int ntiles = max(0, t1 - pc.t0);
+        const int row_base = p.row0 + pc.rb * 128 * L::kRowTiles;
+        const int ntl = PAIR ? (p.rows - row_base > 128 ? 2 : 1) : 1;  // row tiles in use
+        const bool alternate = !PAIR || ntl == 1;  // key tiles alternate between the groups, which share the rows
+        const int nsteps = alternate ? ntiles : 2 * ntiles;
+
+        if (warp < 8) {
+            // ------------------------------------------------------------ queries into their operand layout
+            for (int e = tid; e < ntl * 128 * 16; e += 256) {
+                const int r = e >> 4, c = e & 15, row = row_base + r;
+                uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                if (row < p.rows)
+                    x = __ldg(reinterpret_cast<const uint4*>(p.q + (int64_t)pc.b * p.sq_b + (int64_t)(row / p.G) * p.sq_n +
+                                                             (int64_t)(pc.hk * p.G + row % p.G) * p.sq_h + c * 8));
+                *reinterpret_cast<uint4*>(smem + L::kOffQ + (r >> 7) * kTileBytes +
+                                          sw128_offset(r & 127, c * 8, 128)) = x;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars[L::kQFull]);
+
+            // ------------------------------------------------------------ softmax
+            const int grp = warp >> 2, quarter = warp & 3;
+            const int rt = quarter * 32 + lane;
+            const int row = row_base + (alternate ? 0 : 128 * grp) + rt;
+            const bool live = row < p.rows;
+            const bool quarter_live = row - lane < p.rows;
+            const int node = live ? row / p.G : 0;
+            const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+            const uint32_t s_tm = tmem + lane_off + 256 + 128 * grp, o_tm = tmem + lane_off + 128 * grp;
+            float m = -INFINITY, l = 0.f;
+            int done = 0;  // steps of this group
+            for (int s = grp; s < nsteps; s += 2, ++done) {
+                const int tile = pc.t0 + (alternate ? s : s >> 1);
+                ok = __all_sync(MFD_FULL_MASK, ok & mbar_wait(&bars[L::kSFull + grp], (n_s[grp] + done) & 1, kTries));
+                tc_fence_after();
+                if (quarter_live && ok) {
+                    const float4* cst = consts + (size_t)((n_raw + tile - pc.t0) & (kRing - 1)) * 8;
+                    // visibility of the tile's keys, 32 a word
+                    uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+                    bool masked = false;
+                    if (tile < tp) {
+                        const int valid = len - tile * kKt;
+                        if (valid < kKt) {
+                            masked = true;
+#pragma unroll
+                            for (int c = 0; c < 4; ++c)
+                                vis[c] = valid >= 32 * c + 32 ? ~0u : (valid <= 32 * c ? 0u : (1u << (valid - 32 * c)) - 1u);
+                        }
+                    } else {
+                        masked = true;
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const uint64_t v = live ? visible_word(p, pc.b, node, 2 * (tile - tp) + c) : 0ull;
+                            vis[2 * c] = (uint32_t)v;
+                            vis[2 * c + 1] = (uint32_t)(v >> 32);
+                        }
+                    }
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t u[1][32];
+                        tmem_ld32_issue(s_tm + 32 * c, u[0]);
+                        tmem_ld_wait(u);
+                        if (masked) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (!((vis[c] >> j) & 1u)) u[0][j] = 0xff800000u;
+                        }
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {  // 16 keys: one page
+                            float a[6];
+#pragma unroll
+                            for (int j = 0; j < 5; ++j)
+                                a[j] = fmax3(__uint_as_float(u[0][16 * q + 3 * j]), __uint_as_float(u[0][16 * q + 3 * j + 1]),
+                                             __uint_as_float(u[0][16 * q + 3 * j + 2]));
+                            a[5] = __uint_as_float(u[0][16 * q + 15]);
+                            const float g = fmax3(fmax3(a[0], a[1], a[2]), fmax3(a[3], a[4], a[5]), -INFINITY);
+                            const float4 k = cst[2 * c + q];
+                            mx = fmaxf(mx, g == -INFINITY ? g : fmaf(g, k.x, k.y));
+                        }
+                    }
+                    float alpha = 1.f;
+                    bool rescale = false;
+                    if (mx > m + 8.f) {  // lazy: the running reference moves only when the maximum passes it by 2^8
+                        if (m != -INFINITY) alpha = fast_exp2(m - mx), rescale = true;
+                        m = mx;
+                    }
+                    const float mr = m == -INFINITY ? 0.f : m;
+                    uint64_t acc[2] = {0ull, 0ull};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t u[1][32];
+                        tmem_ld32_issue(s_tm + 32 * c, u[0]);
+                        tmem_ld_wait(u);
+                        if (masked) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (!((vis[c] >> j) & 1u)) u[0][j] = 0xff800000u;
+                        }
+                        uint32_t hl[32];  // hi pairs, then lo pairs
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            const float4 k = cst[2 * c + q];
+                            const uint64_t kc = dup2(k.x), kd = dup2(k.y - mr), ki = dup2(k.z);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                const int e = 16 * q + 2 * j;
+                                float x0, x1;
+                                upk2(fma2(pk2(__uint_as_float(u[0][e]), __uint_as_float(u[0][e + 1])), kc, kd), x0, x1);
+                                x0 = fast_exp2(x0), x1 = fast_exp2(x1);
+                                acc[j & 1] = fma2(pk2(x0, x1), ki, acc[j & 1]);
+                                split_bf16(x0, x1, hl[8 * q + j], hl[16 + 8 * q + j]);
+                            }
+                        }
+                        tmem_st32u(s_tm + 32 * c, hl);  // over the 32 scores they come from
+                    }
+                    float a0, a1;
+                    upk2(add2(acc[0], acc[1]), a0, a1);
+                    l = fmaf(l, alpha, a0 + a1);
+                    if (__any_sync(MFD_FULL_MASK, rescale)) {  // O must hold this group's last product
+                        if (done >= 1) {
+                            ok = __all_sync(MFD_FULL_MASK,
+                                            ok & mbar_wait(&bars[L::kPV + grp], (n_s[grp] + done - 1) & 1, kTries));
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int oc = 0; oc < kD; oc += 32) {
+                                float o[32];
+                                tmem_ld32(o_tm + oc, o);
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) o[j] *= alpha;
+                                tmem_st32(o_tm + oc, o);
+                            }
+                        }
+                    }
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars[L::kPFull + grp]);
+                if (!ok) break;
+            }
+            // ------------------------------------------------------------ epilogue
+            if (done > 0 && ok) {
+                ok = __all_sync(MFD_FULL_MASK, mbar_wait(&bars[L::kPV + grp], (n_s[grp] + done - 1) & 1, kTries));
+                tc_fence_after();
+            }
+            // alternate: the two groups' (m, l) of a row meet in the raw ring (every code is converted by now), and each
+            // group finishes 64 columns
+            float m_fin = m, l_fin = l, f_own = 1.f, f_oth = 0.f;
+            if (alternate) {
+                float* x = reinterpret_cast<float*>(smem + L::kOffRaw);
+                bar_sync<256>(1);  // (a group without a step has waited for nothing: the other's last product has)
+                x[grp * 128 + rt] = m;
+                x[256 + grp * 128 + rt] = l;
+                tc_fence_before();
+                bar_sync<256>(1);  // (both groups' products are complete: each waited for its own)
+                tc_fence_after();
+                const float mo = x[(1 - grp) * 128 + rt], lo = x[256 + (1 - grp) * 128 + rt];
+                m_fin = fmaxf(m, mo);
+                f_own = m == -INFINITY ? 0.f : fast_exp2(m - m_fin);
+                f_oth = mo == -INFINITY ? 0.f : fast_exp2(mo - m_fin);
+                l_fin = l * f_own + lo * f_oth;
+                fence_proxy_async_smem();  // (the next piece's copies land here)
+            }
+            const bool own_used = done > 0, oth_used = alternate && (grp == 0 ? nsteps > 1 : nsteps > 0);
+            const bool odd = *s_odd != 0;
+            const int own0 = max(pc.t0 - tp, 0) * kKt, own1 = min(p.nn, (t1 - tp) * kKt);  // own keys of this piece
+            if (quarter_live && ok) {
+                const float inv = l_fin > 0.f ? 1.f / l_fin : (l_fin == 0.f ? 0.f : l_fin);
+                const int c_lo = alternate ? 64 * grp : 0, c_hi = alternate ? c_lo + 64 : kD;
+                float* slot = p.part + (int64_t)pc.slot * kSlotFloats(PAIR);
+                const int srow = (alternate ? 0 : 128 * grp) + rt;
+                if (c_lo == 0) {
+                    if (pc.pieces > 1) {
+                        slot[srow] = m_fin;
+                        slot[kSlotRows(PAIR) + srow] = l_fin;
+                    } else if (live && p.lse) {
+                        p.lse[((int64_t)pc.b * p.n + node) * p.H + pc.hk * p.G + row % p.G] =
+                            l_fin == 0.f ? -INFINITY : 0.6931471805599453f * (m_fin + log2f(l_fin));
+                    }
+                }
+#pragma unroll 1
+                for (int oc = c_lo; oc < c_hi; oc += 32) {
+                    float o[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) o[j] = 0.f;
+                    if (own_used) {
+                        tmem_ld32(o_tm + oc, o);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] *= f_own;
+                    }
+                    if (oth_used) {
+                        float o2[32];
+                        tmem_ld32(tmem + lane_off + 128 * (1 - grp) + oc, o2);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] = fmaf(o2[j], f_oth, o[j]);
+                    }
+                    if (odd && live) {  // rare: infinities and NaNs of the own values the row sees
+                        for (int key = own0; key < own1; ++key) {
+                            if (!((visible_word(p, pc.b, node, key >> 6) >> (key & 63)) & 1ull)) continue;
+                            const __nv_bfloat16* vr = p.vn + (int64_t)pc.b * p.sn_b + (int64_t)key * p.sn_n +
+                                                      (int64_t)pc.hk * p.sn_h + oc;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                const float y = __bfloat162float(vr[j]);
+                                if (!(fabsf(y) < INFINITY)) o[j] += y;
+                            }
+                        }
+                    }
+                    if (pc.pieces > 1) {
+                        float4* dst = reinterpret_cast<float4*>(slot + 2 * kSlotRows(PAIR));
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4)
+                            dst[((oc + j) >> 2) * kSlotRows(PAIR) + srow] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                    } else if (live) {
+                        uint4* dst = reinterpret_cast<uint4*>(p.out + (int64_t)pc.b * p.so_b + (int64_t)node * p.so_n +
+                                                              (int64_t)(pc.hk * p.G + row % p.G) * p.so_h + oc);
+#pragma unroll
+                        for (int j = 0; j < 32; j += 8)
+                            dst[j >> 3] = make_uint4(pack_bf16(o[j] * inv, o[j + 1] * inv), pack_bf16(o[j + 2] * inv, o[j + 3] * inv),
+                                                     pack_bf16(o[j + 4] * inv, o[j + 5] * inv),
+                                                     pack_bf16(o[j + 6] * inv, o[j + 7] * inv));
+                    }
+                }
+            }
+            tc_fence_before();
+        } else if (warp < 12) {
+            // ------------------------------------------------------------ converters
+            const int cw = warp - 8;
+            for (int i = 0; i < ntiles && ok; ++i) {
+                const int tile = pc.t0 + i;
+                const uint32_t nr = n_raw + i, st = nr % kStages;
+                ok &= mbar_wait(&bars[L::kRawFull + st], (nr / kStages) & 1, kTries);
+#pragma unroll 1
+                for (int which = 0; which < 2 && ok; ++which) {
+                    unsigned char* dst;
+                    if (which == 0) {
+                        const uint32_t n = n_k + i;
+                        if (n >= 1) ok &= mbar_wait(&bars[L::kKEmpty], (n - 1) & 1, kTries);
+                        dst = smem + L::kOffK;
+                    } else {
+                        const uint32_t n = n_v + i;
+                        if (n >= 2) ok &= mbar_wait(&bars[L::kVEmpty + (n & 1)], ((n >> 1) - 1) & 1, kTries);
+                        dst = smem + L::kOffV + (n & 1) * kTileBytes;
+                    }
+                    ok = __all_sync(MFD_FULL_MASK, ok);
+                    if (!ok) break;
+                    if (tile < tp) {
+                        const int valid = min(kKt, len - tile * kKt);
+                        const unsigned char* src = smem + L::kOffRaw + st * kRawBytes + which * (kRawBytes / 2);
+                        const int c = lane & 7, h = c >> 2, q = 2 * (c & 3);
+#pragma unroll 4
+                        for (int j = 0; j < 8; ++j) {  // 4 rows of 8 16-byte chunks an instruction
+                            const int r = (cw + 4 * j) * 4 + (lane >> 3);
+                            uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                            if (r < valid) x = *reinterpret_cast<const uint4*>(src + r * kD + c * 16);
+                            uint4 y0, y1;
+                            bfloats<FP8>(x.x, y0.x, y0.y);
+                            bfloats<FP8>(x.y, y0.z, y0.w);
+                            bfloats<FP8>(x.z, y1.x, y1.y);
+                            bfloats<FP8>(x.w, y1.z, y1.w);
+                            unsigned char* base = dst + h * (kTileBytes / 2) + r * 128;
+                            // chunks q and q + 1; the upper half's lanes store them in the other order, so the eight
+                            // lanes of a row hit eight different bank groups
+                            const int first = h ? q + 1 : q, second = h ? q : q + 1;
+                            *reinterpret_cast<uint4*>(base + ((first ^ (r & 7)) << 4)) = h ? y1 : y0;
+                            *reinterpret_cast<uint4*>(base + ((second ^ (r & 7)) << 4)) = h ? y0 : y1;
+                        }
+                    } else {  // the nodes' own rows; a non-finite value leaves the product (0 times it is not 0)
+                        const __nv_bfloat16* src = (which ? p.vn : p.kn) + (int64_t)pc.b * p.sn_b + (int64_t)pc.hk * p.sn_h;
+                        const int key0 = (tile - tp) * kKt;
+                        bool odd = false;
+#pragma unroll 4
+                        for (int j = 0; j < 16; ++j) {
+                            const int r = (cw + 4 * j) * 2 + (lane >> 4), c = lane & 15;
+                            uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                            if (key0 + r < p.nn)
+                                x = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)(key0 + r) * p.sn_n + c * 8));
+                            if (which) {
+                                uint32_t v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                                for (int u = 0; u < 4; ++u) {
+                                    if ((v[u] & 0x7f80u) == 0x7f80u) v[u] &= 0xffff0000u, odd = true;
+                                    if ((v[u] & 0x7f800000u) == 0x7f800000u) v[u] &= 0xffffu, odd = true;
+                                }
+                                x = make_uint4(v[0], v[1], v[2], v[3]);
+                            }
+                            *reinterpret_cast<uint4*>(dst + sw128_offset(r, c * 8, 128)) = x;
+                        }
+                        if (odd) *s_odd = 1;
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(which == 0 ? &bars[L::kKFull] : &bars[L::kVFull + ((n_v + i) & 1)]);
+                        if (which == 1) mbar_arrive(&bars[L::kRawEmpty + st]);
+                    }
+                }
+            }
+        } else if (warp == 12) {
+            // ------------------------------------------------------------ producer
+            const int ppt = kKt >> p.c.page_shift;  // pages per tile; lane j < ppt takes page j
+            const int gpp = p.c.page >> 4;
+            auto id_of = [&](int tile) {
+                const int pg = tile * ppt + lane;
+                return (lane < ppt && tile < tp && (pg << p.c.page_shift) < len) ? page_id(p.c, pc.b, pg) : -1;
+            };
+            int id = id_of(pc.t0);
+            for (int i = 0; i < ntiles && ok; ++i) {
+                const int tile = pc.t0 + i;
+                const uint32_t nr = n_raw + i, st = nr % kStages;
+                const int id_next = i + 1 < ntiles ? id_of(tile + 1) : -1;
+                if (nr >= (uint32_t)kStages) {
+                    ok &= mbar_wait(&bars[L::kRawEmpty + st], (nr / kStages - 1) & 1, kTries);
+                    ok = __all_sync(MFD_FULL_MASK, ok);
+                    if (!ok) break;
+                }
+                float4* cst = consts + (size_t)(nr & (kRing - 1)) * 8;
+                uint64_t* bar = &bars[L::kRawFull + st];
+                if (id >= 0) {
+                    const uint32_t half = (uint32_t)(p.c.page * kD);
+                    const uint32_t dst = sbase + L::kOffRaw + st * kRawBytes + lane * half;
+                    mbar_expect_tx(bar, 2 * half);
+                    tma_page(dst, &tmk, bar, pc.hk, id);
+                    tma_page(dst + kRawBytes / 2, &tmv, bar, pc.hk, id);
+                    const float sk = __ldg(p.c.k_scale + (int64_t)id * p.c.Hkv + pc.hk);
+                    const float sv = fmaxf(__ldg(p.c.v_scale + (int64_t)id * p.c.Hkv + pc.hk), kScaleFloor);
+                    const float4 k = make_float4(sk * p.scale_log2, __log2f(sv), __frcp_rn(sv), 0.f);
+                    for (int g = 0; g < gpp; ++g) cst[lane * gpp + g] = k;
+                } else if (lane < ppt) {
+                    const float4 k = make_float4(p.scale_log2, 0.f, 1.f, 0.f);  // own keys, or behind the request's end
+                    for (int g = 0; g < gpp; ++g) cst[lane * gpp + g] = k;
+                }
+                // the lanes without a page arrive last (lanes 8 .. 31 never have one), after every constant is stored
+                __syncwarp();
+                if (id < 0) mbar_arrive(bar);
+                id = id_next;
+                issued = nr + 1;
+            }
+        } else if (lane == 0) {
+            // ------------------------------------------------------------ MMA issuer
+            constexpr uint32_t kIdescS = idesc_bf16(128, kKt, 0);
+            constexpr uint32_t kIdescO = idesc_bf16(128, kD, 1);
+            auto scores = [&](int s) {
+                const int i = alternate ? s : s >> 1, grp = s & 1;
+                if (alternate || grp == 0) {
+                    ok &= mbar_wait(&bars[L::kKFull], (n_k + i) & 1, kTries);
+                    tc_fence_after();
+                }
+                const uint32_t q = sbase + L::kOffQ + (alternate ? 0 : grp * kTileBytes), k = sbase + L::kOffK;
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks)
+                    umma(tmem + 256 + 128 * grp, sw128_desc(q, ks, 128), sw128_desc(k, ks, 128), kIdescS, ks > 0);
+                umma_commit(&bars[L::kSFull + grp]);
+                if (alternate || grp == 1) umma_commit(&bars[L::kKEmpty]);
+            };
+            if (nsteps > 0) ok &= mbar_wait(&bars[L::kQFull], n_piece & 1, kTries);
+            tc_fence_after();
+            if (nsteps > 0 && ok) scores(0);
+            if (nsteps > 1 && ok) scores(1);
+            for (int s = 0; s < nsteps && ok; ++s) {
+                const int i = alternate ? s : s >> 1, grp = s & 1;
+                const uint32_t nv = n_v + i;
+                ok &= mbar_wait(&bars[L::kPFull + grp], (n_s[grp] + (s >> 1)) & 1, kTries);
+                if (alternate || grp == 0) ok &= mbar_wait(&bars[L::kVFull + (nv & 1)], (nv >> 1) & 1, kTries);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t v = sbase + L::kOffV + (nv & 1) * kTileBytes, pt = tmem + 256 + 128 * grp;
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks) {  // 16 keys: hi, then lo
+                    const uint64_t vd = sdesc(v + ks * 2048, kTileBytes / 2, 1024);
+                    const uint32_t pa = pt + 32 * (ks >> 1) + 8 * (ks & 1);
+                    umma_ts(tmem + 128 * grp, pa, vd, kIdescO, (s >= 2 || ks > 0) ? 1u : 0u);
+                    umma_ts(tmem + 128 * grp, pa + 16, vd, kIdescO, 1u);
+                }
+                umma_commit(&bars[L::kPV + grp]);
+                if (alternate || grp == 1) umma_commit(&bars[L::kVEmpty + (nv & 1)]);
+                if (s + 2 < nsteps) scores(s + 2);
+            }
+        }
+        if (!ok) *s_failed = 1;
+        tc_fence_before();
+        __syncthreads();  // the piece is over for every role
+        tc_fence_after();
+        if (*s_failed) break;
+        n_piece += 1;
+        n_raw += ntiles, n_k += ntiles, n_v += ntiles;
+        n_s[0] += (nsteps + 1) >> 1, n_s[1] += nsteps >> 1;
+        if (tid == 0) *s_odd = 0;
+        __syncthreads();
+    }
+    if (*s_failed) {
+        if (tid == 0) atomicExch(p.status, 1);
+        // copies in flight end before the CTA does (bounded)
+        if (warp == 12)
+            for (uint32_t f = issued > kStages ? issued - kStages : 0u; f < issued; ++f)
+                mbar_wait(&bars[L::kRawFull + f % kStages], (f / kStages) & 1, 1u << 14);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 13) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+}
+
+// Adds up the pieces of every unit that was cut, in their order.  One warp per row of 128 columns at a time.
+template <bool PAIR>
+__global__ void __launch_bounds__(256) kv8_combine_kernel(const AttnParams p, int ctas) {
+    constexpr int kRowsU = kSlotRows(PAIR);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Work w = make_work(p, kRowsU, ctas);
+    const int64_t rows = (int64_t)p.bs * w.per_req * kRowsU;
+    for (int64_t x = (int64_t)blockIdx.x * 8 + warp; x < rows; x += (int64_t)gridDim.x * 8) {
+        const int64_t unit = x / kRowsU;
+        const int r = (int)(x % kRowsU);
+        const int b = (int)(unit / w.per_req), u = (int)(unit % w.per_req);
+        const int hk = u / w.RB, rb = u % w.RB;
+        const int row = p.row0 + rb * kRowsU + r;
+        if (row >= p.rows) continue;
+        const int tiles = tiles_of(p, b);
+        // where the unit's pieces are
+        int64_t before = 0;
+        for (int b0 = 0; b0 < b; b0 += 32) {
+            const int o = b0 + lane;
+            unsigned v = 0u;
+            if (o < b) v = w.split ? (unsigned)((tiles_of(p, o) + w.per - 1) / w.per) : (unsigned)tiles_of(p, o);
+            before += __reduce_add_sync(MFD_FULL_MASK, v);
+        }
+        before *= w.per_req;
+        int first, pieces;
+        bool second = false;  // the first piece is its CTA's second slot
+        if (w.split) {
+            pieces = (int)((tiles + w.per - 1) / w.per);
+            first = (int)(before + (int64_t)u * pieces);
+        } else {
+            const int64_t lo = before + (int64_t)u * tiles;
+            first = (int)(lo / w.per);
+            pieces = (int)((lo + tiles - 1) / w.per) - first + 1;
+            second = (int64_t)first * w.per < lo;
+        }
+        if (pieces == 1) continue;  // written by its CTA
+        auto slot_of = [&](int i) { return p.part + (int64_t)(2 * (first + i) + (second && i == 0 ? 1 : 0)) * kSlotFloats(PAIR); };
+        float mm = -INFINITY, ll = 0.f;
+        for (int i = lane; i < pieces; i += 32) mm = fmaxf(mm, __ldg(slot_of(i) + r));
+        mm = warp_max_f32(mm);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int i = 0; i < pieces; ++i) {
+            const float* s = slot_of(i);
+            const float mi = __ldg(s + r), li = __ldg(s + kRowsU + r);
+            const float4 o = __ldg(reinterpret_cast<const float4*>(s + 2 * kRowsU) + (int64_t)lane * kRowsU + r);
+            const float a = mi == -INFINITY ? 0.f : fast_exp2(mi - mm);
+            ll = fmaf(a, li, ll);
+            v.x = fmaf(a, o.x, v.x), v.y = fmaf(a, o.y, v.y), v.z = fmaf(a, o.z, v.z), v.w = fmaf(a, o.w, v.w);
+        }
+        const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
+        const int node = row / p.G, head = hk * p.G + row % p.G;
+        *reinterpret_cast<uint2*>(p.out + (int64_t)b * p.so_b + (int64_t)node * p.so_n + (int64_t)head * p.so_h + 4 * lane) =
+            make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+        if (p.lse && lane == 0)
+            p.lse[((int64_t)b * p.n + node) * p.H + head] = ll == 0.f ? -INFINITY : 0.6931471805599453f * (mm + log2f(ll));
+    }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    if (!fn) {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = (PFN_cuTensorMapEncodeTiled_v12000)ptr;
+    }
+    return fn;
+}
+
+// codes as (128, page, KV heads, pages); one page of one head a box, unswizzled (the converters read plain rows)
+bool make_map(CUtensorMap* m, const uint8_t* base, const Cache& c) {
+    auto fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)kD, (cuuint64_t)c.page, (cuuint64_t)c.Hkv, (cuuint64_t)c.num_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)c.sc_t, (cuuint64_t)c.sc_h, (cuuint64_t)c.sc_p};
+    const cuuint32_t box[4] = {(cuuint32_t)kD, (cuuint32_t)c.page, 1, 1};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool FP8, bool PAIR>
+int launch_tc_one(const AttnParams& p, int sms, cudaStream_t stream) {
+    CUtensorMap tk, tv;
+    if (!make_map(&tk, p.c.k, p.c) || !make_map(&tv, p.c.v, p.c)) {
+        set_error("mfd_kv8_attention: could not encode the TMA tensor maps");
+        return MFD_ERR_CUDA;
+    }
+    static bool opted[64];
+    cudaError_t e = opt_in_smem((const void*)kv8_tc_kernel<FP8, PAIR>, Layout<PAIR>::kBytes, opted);
+    if (e != cudaSuccess) {
+        set_error("mfd_kv8_attention: %s", cudaGetErrorString(e));
+        return MFD_ERR_CUDA;
+    }
+    kv8_tc_kernel<FP8, PAIR><<<sms, kTcThreads, Layout<PAIR>::kBytes, stream>>>(tk, tv, p);
+    MFD_CHECK_LAUNCH("mfd_kv8_attention");
+    kv8_combine_kernel<PAIR><<<2 * sms, 256, 0, stream>>>(p, sms);
+    MFD_CHECK_LAUNCH("mfd_kv8_attention (combination)");
+    return MFD_OK;
+}
+
+}  // namespace
+
+size_t tc_workspace(int sms) { return (size_t)sms * 2 * kSlotFloats(true) * sizeof(float); }
+
+int launch_tc(const AttnParams& p, bool pair, int sms, cudaStream_t stream) {
+    if (p.fp8) return pair ? launch_tc_one<true, true>(p, sms, stream) : launch_tc_one<true, false>(p, sms, stream);
+    return pair ? launch_tc_one<false, true>(p, sms, stream) : launch_tc_one<false, false>(p, sms, stream);
+}
+
+}  // namespace kv8
+}  // namespace mfd
