@@ -82,12 +82,13 @@ __device__ __forceinline__ void bfloats(uint32_t w, uint32_t& lo, uint32_t& hi) 
     }
 }
 
-// a pair of weights as bf16 hi + lo (16 bits of each): hi is the rounded weight, lo what it left
-__device__ __forceinline__ void split_bf16(float a, float b, uint32_t& hi, uint32_t& lo) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    const __nv_bfloat162 r = __floats2bfloat162_rn(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
-    lo = *reinterpret_cast<const uint32_t*>(&r);
+// A pair of weights as bf16 hi + lo, both cut off instead of rounded (byte moves and one packed subtraction; the rounding
+// conversions run at half rate): hi keeps the top 8 bits, lo the next 8, so a weight loses at most 2^-15 of itself.
+__device__ __forceinline__ void split_bf16(uint64_t w, uint32_t& hi, uint32_t& lo) {
+    const uint64_t top = w & 0xffff0000ffff0000ull;
+    const uint64_t left = sub2(w, top);
+    hi = __byte_perm((uint32_t)w, (uint32_t)(w >> 32), 0x7632);
+    lo = __byte_perm((uint32_t)left, (uint32_t)(left >> 32), 0x7632);
 }
 
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
@@ -152,40 +153,140 @@ __device__ __forceinline__ int listed_rows(const int64_t* path, int64_t path_str
     return c;
 }
 
-// Work laid end to end over the requests, f(b) of it for request b; every warp computes where it is by itself.
-// warp-wide sum over requests of f(b)
-template <class F>
-__device__ __forceinline__ int64_t over_requests(int bs, F f) {
-    int64_t sum = 0;
-    for (int b0 = 0; b0 < bs; b0 += 32) {
-        const int b = b0 + (threadIdx.x & 31);
-        const unsigned v = b < bs ? (unsigned)f(b) : 0u;
-        sum += __reduce_add_sync(MFD_FULL_MASK, v);
-    }
-    return sum;
+// a / b for a >= 0, b > 0: the 32-bit quotient where it suffices (the 64-bit one takes several times as long)
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    if (((uint64_t)(a | b) >> 32) == 0) return (int64_t)((uint32_t)a / (uint32_t)b);
+    return a / b;
 }
-// the request whose range [before, before + f(b)) contains x, and before
-template <class F>
-__device__ __forceinline__ int find_request(int bs, int64_t x, F f, int64_t& before) {
-    before = 0;
-    for (int b0 = 0; b0 < bs; b0 += 32) {
-        const int lane = threadIdx.x & 31, b = b0 + lane;
-        const int64_t v = b < bs ? f(b) : 0;
-        int64_t inc = v;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int64_t o = __shfl_up_sync(MFD_FULL_MASK, inc, d);
-            if (lane >= d) inc += o;
-        }
-        const uint32_t hit = __ballot_sync(MFD_FULL_MASK, before + inc > x);
-        if (hit) {
-            const int l = __ffs(hit) - 1;
-            before += __shfl_sync(MFD_FULL_MASK, inc - v, l);
-            return b0 + l;
-        }
-        before += __shfl_sync(MFD_FULL_MASK, inc, 31);
+
+// Work laid end to end over the requests, f(length) * mul of it for each; every warp finds its place by itself.  The
+// lengths of the first 32 requests stay in the lanes' registers.
+struct Lengths {
+    const Cache& c;
+    int bs, mine;
+    __device__ __forceinline__ Lengths(const Cache& cache, int requests) : c(cache), bs(requests) {
+        const int lane = threadIdx.x & 31;
+        mine = lane < bs ? seq_len(c, lane) : 0;
     }
-    return -1;
+    template <class F>
+    __device__ __forceinline__ uint32_t part(int b0, F f, int& len) const {
+        const int b = b0 + (threadIdx.x & 31);
+        len = b0 == 0 ? mine : (b < bs ? seq_len(c, b) : 0);
+        return b < bs ? (uint32_t)f(len) : 0u;
+    }
+    // the sum over all requests, or over those before `upto`
+    template <class F>
+    __device__ __forceinline__ int64_t sum(F f, int upto) const {
+        int64_t total = 0;
+        for (int b0 = 0; b0 < upto; b0 += 32) {
+            int len;
+            const uint32_t v = part(b0, f, len);
+            total += __reduce_add_sync(MFD_FULL_MASK, b0 + (int)(threadIdx.x & 31) < upto ? v : 0u);
+        }
+        return total;
+    }
+    // the request whose range [before, before + f * mul) contains x, its length and before; -1 behind the last
+    template <class F>
+    __device__ __forceinline__ int find(int64_t x, int64_t mul, F f, int64_t& before, int& len) const {
+        const int lane = threadIdx.x & 31;
+        int64_t base = 0;
+        for (int b0 = 0; b0 < bs; b0 += 32) {
+            const uint32_t v = part(b0, f, len);
+            uint32_t inc = v;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint32_t o = __shfl_up_sync(MFD_FULL_MASK, inc, d);
+                if (lane >= d) inc += o;
+            }
+            const uint32_t hit = __ballot_sync(MFD_FULL_MASK, (base + inc) * mul > x);
+            if (hit) {
+                const int l = __ffs(hit) - 1;
+                before = (base + __shfl_sync(MFD_FULL_MASK, inc - v, l)) * mul;
+                len = __shfl_sync(MFD_FULL_MASK, len, l);
+                return b0 + l;
+            }
+            base += __shfl_sync(MFD_FULL_MASK, inc, 31);
+        }
+        return -1;
+    }
+};
+
+// How the units' work is cut over `ctas` CTAs: few units (split) into pieces of `per`, at most one piece a CTA;
+// otherwise equal ranges of `per` end to end, which may begin and end inside a unit.
+struct Cut {
+    int64_t total, per;
+    int per_req;  // units per request
+    bool split;
+};
+template <class F>
+__device__ __forceinline__ Cut make_cut(const Lengths& lens, F f, int per_req, int ctas, int least) {
+    Cut w;
+    w.per_req = per_req;
+    const int64_t units = (int64_t)lens.bs * per_req;
+    w.total = lens.sum(f, lens.bs) * per_req;
+    w.split = units * 2 <= (int64_t)ctas;
+    const int64_t n = w.split ? ctas - units : ctas;  // (pieces <= total / per + units)
+    w.per = quotient(w.total + n - 1, n);
+    w.per = w.split ? quotient(w.per + least - 1, least) * least : (w.per < least ? least : w.per);
+    if (w.per < least) w.per = least;
+    return w;
+}
+// [begin, end) of CTA `cta`: a range of the work, or (split) a piece's number
+__device__ __forceinline__ void cut_range(const Cut& w, int cta, int64_t& begin, int64_t& end) {
+    begin = w.split ? cta : (int64_t)cta * w.per;
+    end = w.split ? begin + 1 : min(w.total, begin + w.per);
+}
+
+struct Piece {
+    int b, len;      // request and its length
+    int u;           // unit of the request
+    int g0, g1, of;  // the piece's part [g0, g1) of the unit's `of`
+    int first;       // the CTA of the unit's first piece
+    int pieces;
+    int slot;        // this piece's partial record (two a CTA: a range can end one unit and begin another)
+    bool second;     // the unit's first piece is its CTA's second record
+};
+// the next piece of CTA `cta` at `pos` (moved on); false at the end
+template <class F>
+__device__ __forceinline__ bool next_piece(const Lengths& lens, F f, const Cut& w, int cta, int64_t& pos, int64_t end,
+                                           Piece& pc) {
+    if (pos >= end) return false;
+    int64_t before;
+    if (w.split) {
+        auto pieces_of = [&](int len) { return quotient(f(len) + w.per - 1, w.per); };
+        pc.b = lens.find(pos, w.per_req, pieces_of, before, pc.len);
+        if (pc.b < 0) return false;
+        pc.of = f(pc.len);
+        pc.pieces = (int)pieces_of(pc.len);
+        const int64_t off = pos - before;
+        pc.u = (int)quotient(off, pc.pieces);
+        const int i = (int)(off - (int64_t)pc.u * pc.pieces);
+        pc.g0 = (int)(i * w.per);
+        pc.g1 = (int)min((int64_t)pc.of, (i + 1) * w.per);
+        pc.first = (int)pos - i;
+        pc.slot = 2 * cta;
+        pc.second = false;
+        pos = end;
+    } else {
+        pc.b = lens.find(pos, w.per_req, f, before, pc.len);
+        if (pc.b < 0) return false;
+        pc.of = f(pc.len);
+        const int64_t off = pos - before;
+        pc.u = (int)quotient(off, pc.of);
+        pc.g0 = (int)(off - (int64_t)pc.u * pc.of);
+        pc.g1 = (int)min((int64_t)pc.of, pc.g0 + (end - pos));
+        const int64_t lo = pos - pc.g0;  // where the unit begins
+        pc.first = (int)quotient(lo, w.per);
+        pc.pieces = (int)quotient(lo + pc.of - 1, w.per) - pc.first + 1;
+        pc.second = (int64_t)pc.first * w.per < lo;
+        pc.slot = 2 * cta + (pos == (int64_t)cta * w.per ? 0 : 1);
+        pos += pc.g1 - pc.g0;
+    }
+    return true;
+}
+// the partial record of piece i of a unit
+__device__ __forceinline__ int64_t slot_of(const Piece& pc, int i) {
+    return 2 * (int64_t)(pc.first + i) + (pc.second && i == 0 ? 1 : 0);
 }
 
 __device__ __forceinline__ float quad_max(float v) {

@@ -37,19 +37,6 @@ constexpr int kTBlock = 36, kRowStride = 4 * kTBlock;  // floats: a lane quad's 
 constexpr int kSlot = 16 * (kD + 2);                   // floats of a partial: m[16], l[16], O[16][128]
 constexpr int kCtasPerSm = 2;
 
-struct Piece {
-    int b, hk, rb;       // unit: request, KV head, block of 16 rows
-    int g0, g1, groups;  // the piece's groups of the unit's
-    int slot;            // its partial record
-    int first_cta, pieces;
-    int64_t unit;
-};
-
-// Where the work is: groups of 16 keys per unit of request b (cached tokens, then own keys).
-__device__ __forceinline__ int unit_groups(const AttnParams& p, int b) {
-    return max(1, (seq_len(p.c, b) + 15) / 16 + (p.nn + 15) / 16);  // (a unit without keys still writes its rows)
-}
-
 __device__ __forceinline__ bool not_finite_pair(uint32_t w) {  // a bf16 pair holds an infinity or a NaN
     return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
@@ -67,59 +54,19 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
     const int g = lane >> 2, t = lane & 3;
     const int nrows = p.rows - p.row0;
     const int RB = (nrows + 15) / 16;
-    const int per_req = p.c.Hkv * RB;  // units per request
 
-    // ---- this CTA's share of the work
-    const int64_t units = (int64_t)p.bs * per_req;
-    auto groups_of = [&](int b) { return unit_groups(p, b); };
-    const int64_t total = over_requests(p.bs, groups_of) * per_req;
-    const bool split = units * 2 <= (int64_t)gridDim.x;
-    // split: pieces of `per` groups (a multiple of the warps), at most gridDim.x in all; otherwise equal ranges
-    int64_t per = split ? (total + gridDim.x - units - 1) / (gridDim.x - units) : (total + gridDim.x - 1) / gridDim.x;
-    if (split) per = (per + kWarps - 1) / kWarps * kWarps;
-    if (per < kWarps) per = kWarps;
-    int64_t pos = (int64_t)blockIdx.x * per, end = pos + per < total ? pos + per : total;
-    if (split) pos = blockIdx.x, end = pos + 1;  // one piece
+    // ---- this CTA's share of the work, in groups of 16 keys (cached tokens, then own keys)
+    auto groups_of = [&](int len) { return max(1, (len + 15) / 16 + (p.nn + 15) / 16); };  // (one, to write zeros)
+    const Lengths lens(p.c, p.bs);
+    const Cut cut = make_cut(lens, groups_of, p.c.Hkv * RB, gridDim.x, kWarps);
+    int64_t pos, end;
+    cut_range(cut, blockIdx.x, pos, end);
 
-    while (pos < end) {
-        // ---- the next piece
-        Piece pc;
-        if (split) {
-            auto pieces_of = [&](int b) { return (int64_t)per_req * ((unit_groups(p, b) + per - 1) / per); };
-            int64_t before;
-            pc.b = find_request(p.bs, pos, pieces_of, before);
-            if (pc.b < 0) return;  // (uniform: more CTAs than pieces)
-            pc.groups = unit_groups(p, pc.b);
-            pc.pieces = (int)((pc.groups + per - 1) / per);
-            const int64_t off = pos - before;
-            const int u = (int)(off / pc.pieces), i = (int)(off % pc.pieces);
-            pc.unit = (int64_t)pc.b * per_req + u;
-            pc.hk = u / RB, pc.rb = u % RB;
-            pc.g0 = (int)(i * per), pc.g1 = min(pc.groups, (int)((i + 1) * per));
-            pc.first_cta = (int)pos - i;
-            pc.slot = 2 * (int)blockIdx.x;
-            pos = end;
-        } else {
-            auto span_of = [&](int b) { return (int64_t)per_req * unit_groups(p, b); };
-            int64_t before;
-            pc.b = find_request(p.bs, pos, span_of, before);
-            if (pc.b < 0) return;
-            pc.groups = unit_groups(p, pc.b);
-            const int64_t off = pos - before;
-            const int u = (int)(off / pc.groups);
-            pc.unit = (int64_t)pc.b * per_req + u;
-            pc.hk = u / RB, pc.rb = u % RB;
-            pc.g0 = (int)(off % pc.groups);
-            pc.g1 = (int)min((int64_t)pc.groups, pc.g0 + (end - pos));
-            const int64_t lo = pos - pc.g0;  // the unit's first group
-            pc.first_cta = (int)(lo / per);
-            pc.pieces = (int)((lo + pc.groups - 1) / per) - pc.first_cta + 1;
-            pc.slot = 2 * (int)blockIdx.x + (pos == (int64_t)blockIdx.x * per ? 0 : 1);
-            pos += pc.g1 - pc.g0;
-        }
-        const int len = seq_len(p.c, pc.b);
+    Piece pc;
+    while (next_piece(lens, groups_of, cut, blockIdx.x, pos, end, pc)) {
+        const int hk = pc.u / RB, rb = pc.u % RB, len = pc.len;
         const int gp = (len + 15) / 16;  // groups of cached tokens; own keys follow
-        const int base = p.row0 + pc.rb * 16;
+        const int base = p.row0 + rb * 16;
 
         // ---- the query rows as float16 operands, divided by a power of two
         float rf[kHalves];            // score factor of the row: the power of two, the scale and log2(e)
@@ -131,7 +78,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
             const bool live = r < p.rows;
             node[h] = live ? r / p.G : -1;
             qrow[h] = p.q + (int64_t)pc.b * p.sq_b + (int64_t)(live ? r / p.G : 0) * p.sq_n +
-                      (int64_t)(pc.hk * p.G + (live ? r % p.G : 0)) * p.sq_h;
+                      (int64_t)(hk * p.G + (live ? r % p.G : 0)) * p.sq_h;
             uint4 x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {  // columns 16 t + 8 (i & 1) + 64 (i >> 1) ..
@@ -222,8 +169,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
         };
 
         // ---- cached tokens
-        const uint8_t* kbase = p.c.k + (int64_t)pc.hk * p.c.sc_h + (int64_t)g * p.c.sc_t + 16 * t;
-        const uint8_t* vbase = p.c.v + (int64_t)pc.hk * p.c.sc_h + (int64_t)(2 * t) * p.c.sc_t + 16 * g;
+        const uint8_t* kbase = p.c.k + (int64_t)hk * p.c.sc_h + (int64_t)g * p.c.sc_t + 16 * t;
+        const uint8_t* vbase = p.c.v + (int64_t)hk * p.c.sc_h + (int64_t)(2 * t) * p.c.sc_t + 16 * g;
         const int slot_mask = p.c.page - 1;
         int gi = pc.g0 + warp;
         int id_next = gi < min(pc.g1, gp) ? page_id(p.c, pc.b, (gi * 16) >> p.c.page_shift) : 0;
@@ -240,8 +187,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
 #pragma unroll
             for (int i = 0; i < 4; ++i)  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
                 vw[i] = ldg_stream_u4(vbase + off + (int64_t)((i & 1) + 8 * (i >> 1)) * p.c.sc_t);
-            const float sk = __ldg(p.c.k_scale + (int64_t)id * p.c.Hkv + pc.hk);
-            const float sv = fmaxf(__ldg(p.c.v_scale + (int64_t)id * p.c.Hkv + pc.hk), kScaleFloor);
+            const float sk = __ldg(p.c.k_scale + (int64_t)id * p.c.Hkv + hk);
+            const float sv = fmaxf(__ldg(p.c.v_scale + (int64_t)id * p.c.Hkv + hk), kScaleFloor);
             if (gi + kWarps < min(pc.g1, gp)) id_next = page_id(p.c, pc.b, ((gi + kWarps) * 16) >> p.c.page_shift);
 
             float acc[2][4];
@@ -290,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                for (int h = 0; h < kHalves; ++h) split_bf16(w[kt][2 * h], w[kt][2 * h + 1], hi[kt][h], lo[kt][h]);
+                for (int h = 0; h < kHalves; ++h) split_bf16(pk2(w[kt][2 * h], w[kt][2 * h + 1]), hi[kt][h], lo[kt][h]);
             const uint32_t v0[4] = {vw[0].x, vw[0].y, vw[0].z, vw[0].w}, v1[4] = {vw[1].x, vw[1].y, vw[1].z, vw[1].w};
             const uint32_t v2[4] = {vw[2].x, vw[2].y, vw[2].z, vw[2].w}, v3[4] = {vw[3].x, vw[3].y, vw[3].z, vw[3].w};
 #pragma unroll
@@ -309,8 +256,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
         const int g_own = min(pc.g1, gp + (p.nn + 15) / 16);
         for (; gi < g_own; gi += kWarps) {
             const int j0 = (gi - gp) * 16;
-            const __nv_bfloat16* kn = p.kn + (int64_t)pc.b * p.sn_b + (int64_t)pc.hk * p.sn_h;
-            const __nv_bfloat16* vn = p.vn + (int64_t)pc.b * p.sn_b + (int64_t)pc.hk * p.sn_h;
+            const __nv_bfloat16* kn = p.kn + (int64_t)pc.b * p.sn_b + (int64_t)hk * p.sn_h;
+            const __nv_bfloat16* vn = p.vn + (int64_t)pc.b * p.sn_b + (int64_t)hk * p.sn_h;
             float acc[2][4];
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
@@ -345,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-                for (int h = 0; h < kHalves; ++h) split_bf16(w[kt][2 * h], w[kt][2 * h + 1], hi[kt][h], lo[kt][h]);
+                for (int h = 0; h < kHalves; ++h) split_bf16(pk2(w[kt][2 * h], w[kt][2 * h + 1]), hi[kt][h], lo[kt][h]);
             bool odd = false;  // a non-finite value among this group's
 #pragma unroll
             for (int half = 0; half < 2; ++half) {  // columns 16 g + 8 half .. + 7
@@ -419,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
         float* slot = p.part + (int64_t)pc.slot * kSlot;
         auto store = [&](int r, int col, float4 v, float mm, float ll) {  // columns col .. col + 3 of row r, and lse
             const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
-            const int row = base + r, nd = row / p.G, hd = pc.hk * p.G + row % p.G;
+            const int row = base + r, nd = row / p.G, hd = hk * p.G + row % p.G;
             *reinterpret_cast<uint2*>(p.out + (int64_t)pc.b * p.so_b + (int64_t)nd * p.so_n + (int64_t)hd * p.so_h + col) =
                 make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
             if (p.lse && col == 0)
@@ -450,28 +397,26 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
             // ---- the unit's last CTA merges its pieces, in their order
             __threadfence();
             __syncthreads();
-            if (tid == 0) s_last = atomicAdd(p.tickets + pc.unit, 1u) == (unsigned)(pc.pieces - 1);
+            unsigned int* ticket = p.tickets + (int64_t)pc.b * cut.per_req + pc.u;
+            if (tid == 0) s_last = atomicAdd(ticket, 1u) == (unsigned)(pc.pieces - 1);
             __syncthreads();
             if (s_last) {
                 __threadfence();
-                auto slot_of = [&](int i) {  // piece i: the CTA's first piece, except a unit that starts inside a CTA
-                    const int second = (!split && i == 0 && (int64_t)pc.first_cta * per < (pos - (pc.g1 - pc.g0)) - pc.g0) ? 1 : 0;
-                    return p.part + (int64_t)(2 * (pc.first_cta + i) + second) * kSlot;
-                };
+                auto record = [&](int i) { return p.part + slot_of(pc, i) * kSlot; };
                 float* wgt = smem;  // [pieces][16] weights in turn, the rows' (m, l) in s_m[0], s_l[0]
                 constexpr int kBatch = 512;
                 float4 v[2];
                 v[0] = v[1] = make_float4(0.f, 0.f, 0.f, 0.f);
                 for (int r = warp; r < live_rows; r += kWarps) {
                     float mm = -INFINITY;
-                    for (int i = lane; i < pc.pieces; i += 32) mm = fmaxf(mm, __ldcg(slot_of(i) + r));
+                    for (int i = lane; i < pc.pieces; i += 32) mm = fmaxf(mm, __ldcg(record(i) + r));
                     mm = warp_max_f32(mm);
                     float ll = 0.f;
                     for (int i = lane; i < pc.pieces; i += 32) {
-                        const float mi = __ldcg(slot_of(i) + r);
+                        const float mi = __ldcg(record(i) + r);
                         const float a = mi == -INFINITY ? 0.f : fast_exp2(mi - mm);
                         if (i < kBatch) wgt[i * 16 + r] = a;
-                        ll += a * __ldcg(slot_of(i) + 16 + r);
+                        ll += a * __ldcg(record(i) + 16 + r);
                     }
 #pragma unroll
                     for (int d = 16; d; d >>= 1) ll += __shfl_xor_sync(MFD_FULL_MASK, ll, d);
@@ -485,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
                     if (r < live_rows) {
 #pragma unroll 4
                         for (int i = 0; i < pc.pieces; ++i) {
-                            const float* sl = slot_of(i);
+                            const float* sl = record(i);
                             float a;
                             if (i < kBatch) {
                                 a = wgt[i * 16 + r];
@@ -500,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
                         store(r, 4 * c4, v[u], s_m[0][r], s_l[0][r]);
                     }
                 }
-                if (tid == 0) p.tickets[pc.unit] = 0u;
+                if (tid == 0) *ticket = 0u;
             }
         }
         __syncthreads();  // smem, s_m and s_l are free for the next piece

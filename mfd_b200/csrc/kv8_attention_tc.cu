@@ -13,12 +13,13 @@
 //   single a CTA takes one row tile; group t takes every other key tile and the two (m, l, O) merge at the end
 // In both, step s is group s & 1; the products run PV(s), S(s + 2) in order.
 //
-// Warp roles (448 threads, one CTA an SM):
-//   warps 0-7    softmax, thread = row; 128 scores read from TMEM twice (maximum, then weights) instead of held
-//   warps 8-11   converters: raw codes -> bf16 tiles in the 128-byte-swizzled operand layout; the nodes' own keys are
+// Warp roles (512 threads, one CTA an SM; the softmax warps take registers from the others, so that a thread holds its
+// 128 scores: 256 x 184 + 256 x 72 = 512 x 128 registers, what the CTA was launched with):
+//   warps 0-7    softmax, thread = row
+//   warps 8-13   converters: raw codes -> bf16 tiles in the 128-byte-swizzled operand layout; the nodes' own keys are
 //                copied there (past the end of a request: zeros, whatever the page holds)
-//   warp 12      producer: page ids and scales, one TMA load per page and tensor into the raw ring (no multicast)
-//   warp 13      MMA issuer
+//   warp 14      producer: page ids and scales, one TMA load per page and tensor into the raw ring (no multicast)
+//   warp 15      MMA issuer
 // Shared memory: Q (32 KB a row tile), K tile 32 KB, V tiles 2 x 32 KB, raw ring 32 KB a stage.  K needs one buffer: it
 // is free from the last S of its tile to the end of the next PV, and the PV of hi + lo is the longer product.
 //
@@ -42,7 +43,9 @@ namespace kv8 {
 
 namespace {
 
-constexpr int kTcThreads = 448;
+constexpr int kTcThreads = 512;
+constexpr int kConv = 6;                 // converter warps
+constexpr int kSoftmaxRegs = 184, kOtherRegs = 72;
 constexpr int kKt = 128;                 // keys per tile
 constexpr int kTileBytes = kKt * kD * 2;  // 32 KB: a bf16 tile, [2 d-halves][128 rows][128 B]
 constexpr int kRawBytes = 2 * kKt * kD;   // 32 KB: the codes of K and V
@@ -89,63 +92,16 @@ __device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, u
         : "memory");
 }
 
-// The pieces of the work, shared by the attention and the combination.
-struct Work {
-    int64_t total, per;
-    bool split;
-    int RB, per_req;
+// What a piece's tiles are (of 128 keys: cached tokens first, then the nodes' own).
+struct Tiles {
+    int hk, rb;       // KV head, block of rows
+    int tp, t1;       // tiles of cached tokens of the request; end of the piece's
+    int ntiles;       // the piece's
+    int row_base, ntl;  // first row, row tiles in use
+    bool alternate;   // key tiles alternate between the groups, which share the rows
+    int nsteps;
+    uint32_t n_piece, n_tile, n_s0, n_s1;  // pieces, tiles and the groups' steps before
 };
-__device__ __forceinline__ int tiles_of(const AttnParams& p, int b) {
-    return max(1, (seq_len(p.c, b) + kKt - 1) / kKt + (p.nn + kKt - 1) / kKt);
-}
-__device__ __forceinline__ Work make_work(const AttnParams& p, int rows_per_unit, int ctas) {
-    Work w;
-    w.RB = (p.rows - p.row0 + rows_per_unit - 1) / rows_per_unit;
-    w.per_req = p.c.Hkv * w.RB;
-    const int64_t units = (int64_t)p.bs * w.per_req;
-    w.total = over_requests(p.bs, [&](int b) { return tiles_of(p, b); }) * w.per_req;
-    w.split = units * 2 <= (int64_t)ctas;
-    w.per = w.split ? (w.total + ctas - units - 1) / (ctas - units) : (w.total + ctas - 1) / ctas;
-    if (w.per < 1) w.per = 1;
-    return w;
-}
-
-struct Piece {
-    int b, hk, rb, t0, t1, tiles, slot, pieces;
-};
-// the piece of CTA `cta` that starts at `pos` (range mode: a tile index; split mode: the piece index); moves pos on
-__device__ __forceinline__ bool next_piece(const AttnParams& p, const Work& w, int cta, int64_t& pos, int64_t end,
-                                           Piece& pc) {
-    if (pos >= end) return false;
-    int64_t before;
-    if (w.split) {
-        pc.b = find_request(p.bs, pos, [&](int b) { return (int64_t)w.per_req * ((tiles_of(p, b) + w.per - 1) / w.per); },
-                            before);
-        if (pc.b < 0) return false;
-        pc.tiles = tiles_of(p, pc.b);
-        pc.pieces = (int)((pc.tiles + w.per - 1) / w.per);
-        const int64_t off = pos - before;
-        const int u = (int)(off / pc.pieces), i = (int)(off % pc.pieces);
-        pc.hk = u / w.RB, pc.rb = u % w.RB;
-        pc.t0 = (int)(i * w.per), pc.t1 = (int)min((int64_t)pc.tiles, (i + 1) * w.per);
-        pc.slot = 2 * cta;
-        pos = end;
-    } else {
-        pc.b = find_request(p.bs, pos, [&](int b) { return (int64_t)w.per_req * tiles_of(p, b); }, before);
-        if (pc.b < 0) return false;
-        pc.tiles = tiles_of(p, pc.b);
-        const int64_t off = pos - before;
-        const int u = (int)(off / pc.tiles);
-        pc.hk = u / w.RB, pc.rb = u % w.RB;
-        pc.t0 = (int)(off % pc.tiles);
-        pc.t1 = (int)min((int64_t)pc.tiles, pc.t0 + (end - pos));
-        const int64_t lo = pos - pc.t0;
-        pc.pieces = (int)((lo + pc.tiles - 1) / w.per - lo / w.per) + 1;
-        pc.slot = 2 * cta + (pos == (int64_t)cta * w.per ? 0 : 1);
-        pos += pc.t1 - pc.t0;
-    }
-    return true;
-}
 
 template <int N>
 __device__ __forceinline__ void bar_sync(int id) {
@@ -172,12 +128,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         mbar_init(&bars[L::kQFull], 8);
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&bars[L::kRawFull + i], 32);
-            mbar_init(&bars[L::kRawEmpty + i], 4);
+            mbar_init(&bars[L::kRawEmpty + i], kConv);
         }
-        mbar_init(&bars[L::kKFull], 4);
+        mbar_init(&bars[L::kKFull], kConv);
         mbar_init(&bars[L::kKEmpty], 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&bars[L::kVFull + i], 4);
+            mbar_init(&bars[L::kVFull + i], kConv);
             mbar_init(&bars[L::kVEmpty + i], 1);
             mbar_init(&bars[L::kSFull + i], 1);
             mbar_init(&bars[L::kPFull + i], 4);
@@ -187,7 +143,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         *s_odd = 0;
         mbar_fence_init();
     }
-    if (warp == 13) {
+    if (warp == 15) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -196,36 +152,62 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     // TMEM columns: O of group t at 128 t, S of group t at 256 + 128 t
-    const Work w = make_work(p, 128 * L::kRowTiles, gridDim.x);
-    int64_t pos = w.split ? blockIdx.x : (int64_t)blockIdx.x * w.per;
-    const int64_t end = w.split ? pos + 1 : min(w.total, pos + w.per);
+    const int RB = (p.rows - p.row0 + 128 * L::kRowTiles - 1) / (128 * L::kRowTiles);
+    auto tiles_of = [&](int len) { return max(1, (len + kKt - 1) / kKt + (p.nn + kKt - 1) / kKt); };
+    const Lengths lens(p.c, p.bs);
+    const Cut cut = make_cut(lens, tiles_of, p.c.Hkv * RB, gridDim.x, 1);
+    int64_t pos, end;
+    cut_range(cut, blockIdx.x, pos, end);
 
-    // counters that run on over the CTA's pieces (barrier phases)
-    uint32_t n_piece = 0, n_raw = 0, n_k = 0, n_v = 0, n_s[2] = {0u, 0u};
-    uint32_t issued = 0;  // producer: raw stages filled
+    // Every role walks the CTA's pieces in its own loop (below), all meeting at the end of each.
     bool ok = true;
-    Piece pc;
-    while (next_piece(p, w, blockIdx.x, pos, end, pc)) {
-        const int len = seq_len(p.c, pc.b);
-        const int tp = (len + kKt - 1) / kKt;  // tiles of cached tokens, then own keys
-        const int tn = (p.nn + kKt - 1) / kKt;
-        const int t1 = min(pc.t1, tp + tn);      // (a unit without keys has one empty tile: nothing runs)
-        const int ntiles = max(0, t1 - pc.t0);
-        const int row_base = p.row0 + pc.rb * 128 * L::kRowTiles;
-        const int ntl = PAIR ? (p.rows - row_base > 128 ? 2 : 1) : 1;  // row tiles in use
-        const bool alternate = !PAIR || ntl == 1;  // key tiles alternate between the groups, which share the rows
-        const int nsteps = alternate ? ntiles : 2 * ntiles;
+    uint32_t issued = 0;  // producer: raw stages filled
+    auto pieces = [&](auto body) {
+        uint32_t n_piece = 0, n_tile = 0, n_s[2] = {0u, 0u};  // running counts: the barriers' phases
+        Piece pc;
+        while (next_piece(lens, tiles_of, cut, blockIdx.x, pos, end, pc)) {
+            Tiles x;
+            x.hk = pc.u / RB, x.rb = pc.u % RB;
+            x.tp = (pc.len + kKt - 1) / kKt;
+            x.t1 = min(pc.g1, x.tp + (p.nn + kKt - 1) / kKt);  // (a unit without keys has one empty tile)
+            x.ntiles = max(0, x.t1 - pc.g0);
+            x.row_base = p.row0 + x.rb * 128 * L::kRowTiles;
+            x.ntl = PAIR ? (p.rows - x.row_base > 128 ? 2 : 1) : 1;
+            x.alternate = !PAIR || x.ntl == 1;
+            x.nsteps = x.alternate ? x.ntiles : 2 * x.ntiles;
+            x.n_piece = n_piece, x.n_tile = n_tile, x.n_s0 = n_s[0], x.n_s1 = n_s[1];
+            body(pc, x);
+            __syncwarp();  // (the MMA warp's one lane has been apart)
+            if (!ok) *s_failed = 1;
+            tc_fence_before();
+            bar_sync<kTcThreads>(0);  // the piece is over for every role
+            tc_fence_after();
+            if (*s_failed) break;
+            n_piece += 1, n_tile += x.ntiles;
+            n_s[0] += (x.nsteps + 1) >> 1, n_s[1] += x.nsteps >> 1;
+            if (tid == 0) *s_odd = 0;
+            bar_sync<kTcThreads>(0);
+        }
+    };
 
-        if (warp < 8) {
+    if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        pieces([&](const Piece& pc, const Tiles& x) {
             // ------------------------------------------------------------ queries into their operand layout
-            for (int e = tid; e < ntl * 128 * 16; e += 256) {
-                const int r = e >> 4, c = e & 15, row = row_base + r;
-                uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                if (row < p.rows)
-                    x = __ldg(reinterpret_cast<const uint4*>(p.q + (int64_t)pc.b * p.sq_b + (int64_t)(row / p.G) * p.sq_n +
-                                                             (int64_t)(pc.hk * p.G + row % p.G) * p.sq_h + c * 8));
-                *reinterpret_cast<uint4*>(smem + L::kOffQ + (r >> 7) * kTileBytes +
-                                          sw128_offset(r & 127, c * 8, 128)) = x;
+            for (int rtile = 0; rtile < x.ntl; ++rtile) {
+                uint4 qv[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int r = (tid >> 4) + 16 * j, c = tid & 15, row = x.row_base + 128 * rtile + r;
+                    qv[j] = make_uint4(0u, 0u, 0u, 0u);
+                    if (row < p.rows)
+                        qv[j] = __ldg(reinterpret_cast<const uint4*>(p.q + (int64_t)pc.b * p.sq_b + (int64_t)(row / p.G) * p.sq_n +
+                                                                    (int64_t)(x.hk * p.G + row % p.G) * p.sq_h + c * 8));
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    *reinterpret_cast<uint4*>(smem + L::kOffQ + rtile * kTileBytes +
+                                              sw128_offset((tid >> 4) + 16 * j, (tid & 15) * 8, 128)) = qv[j];
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -234,7 +216,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // ------------------------------------------------------------ softmax
             const int grp = warp >> 2, quarter = warp & 3;
             const int rt = quarter * 32 + lane;
-            const int row = row_base + (alternate ? 0 : 128 * grp) + rt;
+            const int row = x.row_base + (x.alternate ? 0 : 128 * grp) + rt;
             const bool live = row < p.rows;
             const bool quarter_live = row - lane < p.rows;
             const int node = live ? row / p.G : 0;
@@ -242,17 +224,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const uint32_t s_tm = tmem + lane_off + 256 + 128 * grp, o_tm = tmem + lane_off + 128 * grp;
             float m = -INFINITY, l = 0.f;
             int done = 0;  // steps of this group
-            for (int s = grp; s < nsteps; s += 2, ++done) {
-                const int tile = pc.t0 + (alternate ? s : s >> 1);
-                ok = __all_sync(MFD_FULL_MASK, ok & mbar_wait(&bars[L::kSFull + grp], (n_s[grp] + done) & 1, kTries));
+            for (int s = grp; s < x.nsteps; s += 2, ++done) {
+                const int tile = pc.g0 + (x.alternate ? s : s >> 1);
+                ok = __all_sync(MFD_FULL_MASK, ok & mbar_wait(&bars[L::kSFull + grp], ((grp ? x.n_s1 : x.n_s0) + done) & 1, kTries));
                 tc_fence_after();
                 if (quarter_live && ok) {
-                    const float4* cst = consts + (size_t)((n_raw + tile - pc.t0) & (kRing - 1)) * 8;
+                    const float4* cst = consts + (size_t)((x.n_tile + tile - pc.g0) & (kRing - 1)) * 8;
                     // visibility of the tile's keys, 32 a word
                     uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
                     bool masked = false;
-                    if (tile < tp) {
-                        const int valid = len - tile * kKt;
+                    if (tile < x.tp) {
+                        const int valid = pc.len - tile * kKt;
                         if (valid < kKt) {
                             masked = true;
 #pragma unroll
@@ -263,34 +245,34 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         masked = true;
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            const uint64_t v = live ? visible_word(p, pc.b, node, 2 * (tile - tp) + c) : 0ull;
+                            const uint64_t v = live ? visible_word(p, pc.b, node, 2 * (tile - x.tp) + c) : 0ull;
                             vis[2 * c] = (uint32_t)v;
                             vis[2 * c + 1] = (uint32_t)(v >> 32);
                         }
                     }
-                    float mx = -INFINITY;
+                    uint32_t u[4][32];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t u[1][32];
-                        tmem_ld32_issue(s_tm + 32 * c, u[0]);
-                        tmem_ld_wait(u);
-                        if (masked) {
+                    for (int c = 0; c < 4; ++c) tmem_ld32_issue(s_tm + 32 * c, u[c]);
+                    tmem_ld_wait(u);
+                    if (masked) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
 #pragma unroll
                             for (int j = 0; j < 32; ++j)
-                                if (!((vis[c] >> j) & 1u)) u[0][j] = 0xff800000u;
-                        }
+                                if (!((vis[c] >> j) & 1u)) u[c][j] = 0xff800000u;
+                    }
+                    float mx = -INFINITY;
 #pragma unroll
-                        for (int q = 0; q < 2; ++q) {  // 16 keys: one page
-                            float a[6];
+                    for (int g = 0; g < 8; ++g) {  // 16 keys: one page
+                        const uint32_t* su = &u[g >> 1][16 * (g & 1)];
+                        float a[6];
 #pragma unroll
-                            for (int j = 0; j < 5; ++j)
-                                a[j] = fmax3(__uint_as_float(u[0][16 * q + 3 * j]), __uint_as_float(u[0][16 * q + 3 * j + 1]),
-                                             __uint_as_float(u[0][16 * q + 3 * j + 2]));
-                            a[5] = __uint_as_float(u[0][16 * q + 15]);
-                            const float g = fmax3(fmax3(a[0], a[1], a[2]), fmax3(a[3], a[4], a[5]), -INFINITY);
-                            const float4 k = cst[2 * c + q];
-                            mx = fmaxf(mx, g == -INFINITY ? g : fmaf(g, k.x, k.y));
-                        }
+                        for (int j = 0; j < 5; ++j)
+                            a[j] = fmax3(__uint_as_float(su[3 * j]), __uint_as_float(su[3 * j + 1]), __uint_as_float(su[3 * j + 2]));
+                        a[5] = __uint_as_float(su[15]);
+                        const float top = fmaxf(fmax3(a[0], a[1], a[2]), fmax3(a[3], a[4], a[5]));
+                        const float2 k = *reinterpret_cast<const float2*>(cst + g);
+                        mx = fmaxf(mx, top == -INFINITY ? top : fmaf(top, k.x, k.y));
                     }
                     float alpha = 1.f;
                     bool rescale = false;
@@ -302,14 +284,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     uint64_t acc[2] = {0ull, 0ull};
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        uint32_t u[1][32];
-                        tmem_ld32_issue(s_tm + 32 * c, u[0]);
-                        tmem_ld_wait(u);
-                        if (masked) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (!((vis[c] >> j) & 1u)) u[0][j] = 0xff800000u;
-                        }
                         uint32_t hl[32];  // hi pairs, then lo pairs
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
@@ -319,10 +293,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             for (int j = 0; j < 8; ++j) {
                                 const int e = 16 * q + 2 * j;
                                 float x0, x1;
-                                upk2(fma2(pk2(__uint_as_float(u[0][e]), __uint_as_float(u[0][e + 1])), kc, kd), x0, x1);
-                                x0 = fast_exp2(x0), x1 = fast_exp2(x1);
-                                acc[j & 1] = fma2(pk2(x0, x1), ki, acc[j & 1]);
-                                split_bf16(x0, x1, hl[8 * q + j], hl[16 + 8 * q + j]);
+                                upk2(fma2(pk2(__uint_as_float(u[c][e]), __uint_as_float(u[c][e + 1])), kc, kd), x0, x1);
+                                const uint64_t w = pk2(fast_exp2(x0), fast_exp2(x1));
+                                acc[j & 1] = fma2(w, ki, acc[j & 1]);
+                                split_bf16(w, hl[8 * q + j], hl[16 + 8 * q + j]);
                             }
                         }
                         tmem_st32u(s_tm + 32 * c, hl);  // over the 32 scores they come from
@@ -333,7 +307,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (__any_sync(MFD_FULL_MASK, rescale)) {  // O must hold this group's last product
                         if (done >= 1) {
                             ok = __all_sync(MFD_FULL_MASK,
-                                            ok & mbar_wait(&bars[L::kPV + grp], (n_s[grp] + done - 1) & 1, kTries));
+                                            ok & mbar_wait(&bars[L::kPV + grp], ((grp ? x.n_s1 : x.n_s0) + done - 1) & 1, kTries));
                             tc_fence_after();
 #pragma unroll 1
                             for (int oc = 0; oc < kD; oc += 32) {
@@ -354,41 +328,41 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             // ------------------------------------------------------------ epilogue
             if (done > 0 && ok) {
-                ok = __all_sync(MFD_FULL_MASK, mbar_wait(&bars[L::kPV + grp], (n_s[grp] + done - 1) & 1, kTries));
+                ok = __all_sync(MFD_FULL_MASK, mbar_wait(&bars[L::kPV + grp], ((grp ? x.n_s1 : x.n_s0) + done - 1) & 1, kTries));
                 tc_fence_after();
             }
-            // alternate: the two groups' (m, l) of a row meet in the raw ring (every code is converted by now), and each
+            // x.alternate: the two groups' (m, l) of a row meet in the raw ring (every code is converted by now), and each
             // group finishes 64 columns
             float m_fin = m, l_fin = l, f_own = 1.f, f_oth = 0.f;
-            if (alternate) {
-                float* x = reinterpret_cast<float*>(smem + L::kOffRaw);
+            if (x.alternate) {
+                float* xch = reinterpret_cast<float*>(smem + L::kOffRaw);
                 bar_sync<256>(1);  // (a group without a step has waited for nothing: the other's last product has)
-                x[grp * 128 + rt] = m;
-                x[256 + grp * 128 + rt] = l;
+                xch[grp * 128 + rt] = m;
+                xch[256 + grp * 128 + rt] = l;
                 tc_fence_before();
                 bar_sync<256>(1);  // (both groups' products are complete: each waited for its own)
                 tc_fence_after();
-                const float mo = x[(1 - grp) * 128 + rt], lo = x[256 + (1 - grp) * 128 + rt];
+                const float mo = xch[(1 - grp) * 128 + rt], lo = xch[256 + (1 - grp) * 128 + rt];
                 m_fin = fmaxf(m, mo);
                 f_own = m == -INFINITY ? 0.f : fast_exp2(m - m_fin);
                 f_oth = mo == -INFINITY ? 0.f : fast_exp2(mo - m_fin);
                 l_fin = l * f_own + lo * f_oth;
                 fence_proxy_async_smem();  // (the next piece's copies land here)
             }
-            const bool own_used = done > 0, oth_used = alternate && (grp == 0 ? nsteps > 1 : nsteps > 0);
+            const bool own_used = done > 0, oth_used = x.alternate && (grp == 0 ? x.nsteps > 1 : x.nsteps > 0);
             const bool odd = *s_odd != 0;
-            const int own0 = max(pc.t0 - tp, 0) * kKt, own1 = min(p.nn, (t1 - tp) * kKt);  // own keys of this piece
+            const int own0 = max(pc.g0 - x.tp, 0) * kKt, own1 = min(p.nn, (x.t1 - x.tp) * kKt);  // own keys of this piece
             if (quarter_live && ok) {
                 const float inv = l_fin > 0.f ? 1.f / l_fin : (l_fin == 0.f ? 0.f : l_fin);
-                const int c_lo = alternate ? 64 * grp : 0, c_hi = alternate ? c_lo + 64 : kD;
+                const int c_lo = x.alternate ? 64 * grp : 0, c_hi = x.alternate ? c_lo + 64 : kD;
                 float* slot = p.part + (int64_t)pc.slot * kSlotFloats(PAIR);
-                const int srow = (alternate ? 0 : 128 * grp) + rt;
+                const int srow = (x.alternate ? 0 : 128 * grp) + rt;
                 if (c_lo == 0) {
                     if (pc.pieces > 1) {
                         slot[srow] = m_fin;
                         slot[kSlotRows(PAIR) + srow] = l_fin;
                     } else if (live && p.lse) {
-                        p.lse[((int64_t)pc.b * p.n + node) * p.H + pc.hk * p.G + row % p.G] =
+                        p.lse[((int64_t)pc.b * p.n + node) * p.H + x.hk * p.G + row % p.G] =
                             l_fin == 0.f ? -INFINITY : 0.6931471805599453f * (m_fin + log2f(l_fin));
                     }
                 }
@@ -412,7 +386,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         for (int key = own0; key < own1; ++key) {
                             if (!((visible_word(p, pc.b, node, key >> 6) >> (key & 63)) & 1ull)) continue;
                             const __nv_bfloat16* vr = p.vn + (int64_t)pc.b * p.sn_b + (int64_t)key * p.sn_n +
-                                                      (int64_t)pc.hk * p.sn_h + oc;
+                                                      (int64_t)x.hk * p.sn_h + oc;
 #pragma unroll
                             for (int j = 0; j < 32; ++j) {
                                 const float y = __bfloat162float(vr[j]);
@@ -427,7 +401,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             dst[((oc + j) >> 2) * kSlotRows(PAIR) + srow] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
                     } else if (live) {
                         uint4* dst = reinterpret_cast<uint4*>(p.out + (int64_t)pc.b * p.so_b + (int64_t)node * p.so_n +
-                                                              (int64_t)(pc.hk * p.G + row % p.G) * p.so_h + oc);
+                                                              (int64_t)(x.hk * p.G + row % p.G) * p.so_h + oc);
 #pragma unroll
                         for (int j = 0; j < 32; j += 8)
                             dst[j >> 3] = make_uint4(pack_bf16(o[j] * inv, o[j + 1] * inv), pack_bf16(o[j + 2] * inv, o[j + 3] * inv),
@@ -437,41 +411,45 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
             }
             tc_fence_before();
-        } else if (warp < 12) {
+        });
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp < 8 + kConv) {
+            pieces([&](const Piece& pc, const Tiles& x) {
             // ------------------------------------------------------------ converters
             const int cw = warp - 8;
-            for (int i = 0; i < ntiles && ok; ++i) {
-                const int tile = pc.t0 + i;
-                const uint32_t nr = n_raw + i, st = nr % kStages;
+            for (int i = 0; i < x.ntiles && ok; ++i) {
+                const int tile = pc.g0 + i;
+                const uint32_t nr = x.n_tile + i, st = nr % kStages;
                 ok &= mbar_wait(&bars[L::kRawFull + st], (nr / kStages) & 1, kTries);
 #pragma unroll 1
                 for (int which = 0; which < 2 && ok; ++which) {
                     unsigned char* dst;
                     if (which == 0) {
-                        const uint32_t n = n_k + i;
+                        const uint32_t n = x.n_tile + i;
                         if (n >= 1) ok &= mbar_wait(&bars[L::kKEmpty], (n - 1) & 1, kTries);
                         dst = smem + L::kOffK;
                     } else {
-                        const uint32_t n = n_v + i;
+                        const uint32_t n = x.n_tile + i;
                         if (n >= 2) ok &= mbar_wait(&bars[L::kVEmpty + (n & 1)], ((n >> 1) - 1) & 1, kTries);
                         dst = smem + L::kOffV + (n & 1) * kTileBytes;
                     }
                     ok = __all_sync(MFD_FULL_MASK, ok);
                     if (!ok) break;
-                    if (tile < tp) {
-                        const int valid = min(kKt, len - tile * kKt);
+                    if (tile < x.tp) {
+                        const int valid = min(kKt, pc.len - tile * kKt);
                         const unsigned char* src = smem + L::kOffRaw + st * kRawBytes + which * (kRawBytes / 2);
                         const int c = lane & 7, h = c >> 2, q = 2 * (c & 3);
-#pragma unroll 4
-                        for (int j = 0; j < 8; ++j) {  // 4 rows of 8 16-byte chunks an instruction
-                            const int r = (cw + 4 * j) * 4 + (lane >> 3);
-                            uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                            if (r < valid) x = *reinterpret_cast<const uint4*>(src + r * kD + c * 16);
+#pragma unroll 3
+                        for (int j = cw; j < 32; j += kConv) {  // 4 rows of 8 16-byte chunks an instruction
+                            const int r = j * 4 + (lane >> 3);
+                            uint4 cw4 = make_uint4(0u, 0u, 0u, 0u);
+                            if (r < valid) cw4 = *reinterpret_cast<const uint4*>(src + r * kD + c * 16);
                             uint4 y0, y1;
-                            bfloats<FP8>(x.x, y0.x, y0.y);
-                            bfloats<FP8>(x.y, y0.z, y0.w);
-                            bfloats<FP8>(x.z, y1.x, y1.y);
-                            bfloats<FP8>(x.w, y1.z, y1.w);
+                            bfloats<FP8>(cw4.x, y0.x, y0.y);
+                            bfloats<FP8>(cw4.y, y0.z, y0.w);
+                            bfloats<FP8>(cw4.z, y1.x, y1.y);
+                            bfloats<FP8>(cw4.w, y1.z, y1.w);
                             unsigned char* base = dst + h * (kTileBytes / 2) + r * 128;
                             // chunks q and q + 1; the upper half's lanes store them in the other order, so the eight
                             // lanes of a row hit eight different bank groups
@@ -480,49 +458,51 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             *reinterpret_cast<uint4*>(base + ((second ^ (r & 7)) << 4)) = h ? y0 : y1;
                         }
                     } else {  // the nodes' own rows; a non-finite value leaves the product (0 times it is not 0)
-                        const __nv_bfloat16* src = (which ? p.vn : p.kn) + (int64_t)pc.b * p.sn_b + (int64_t)pc.hk * p.sn_h;
-                        const int key0 = (tile - tp) * kKt;
+                        const __nv_bfloat16* src = (which ? p.vn : p.kn) + (int64_t)pc.b * p.sn_b + (int64_t)x.hk * p.sn_h;
+                        const int key0 = (tile - x.tp) * kKt;
                         bool odd = false;
 #pragma unroll 4
-                        for (int j = 0; j < 16; ++j) {
-                            const int r = (cw + 4 * j) * 2 + (lane >> 4), c = lane & 15;
-                            uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                        for (int j = cw; j < 64; j += kConv) {
+                            const int r = 2 * j + (lane >> 4), c = lane & 15;
+                            uint4 cw4 = make_uint4(0u, 0u, 0u, 0u);
                             if (key0 + r < p.nn)
-                                x = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)(key0 + r) * p.sn_n + c * 8));
+                                cw4 = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)(key0 + r) * p.sn_n + c * 8));
                             if (which) {
-                                uint32_t v[4] = {x.x, x.y, x.z, x.w};
+                                uint32_t v[4] = {cw4.x, cw4.y, cw4.z, cw4.w};
 #pragma unroll
                                 for (int u = 0; u < 4; ++u) {
                                     if ((v[u] & 0x7f80u) == 0x7f80u) v[u] &= 0xffff0000u, odd = true;
                                     if ((v[u] & 0x7f800000u) == 0x7f800000u) v[u] &= 0xffffu, odd = true;
                                 }
-                                x = make_uint4(v[0], v[1], v[2], v[3]);
+                                cw4 = make_uint4(v[0], v[1], v[2], v[3]);
                             }
-                            *reinterpret_cast<uint4*>(dst + sw128_offset(r, c * 8, 128)) = x;
+                            *reinterpret_cast<uint4*>(dst + sw128_offset(r, c * 8, 128)) = cw4;
                         }
                         if (odd) *s_odd = 1;
                     }
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
-                        mbar_arrive(which == 0 ? &bars[L::kKFull] : &bars[L::kVFull + ((n_v + i) & 1)]);
+                        mbar_arrive(which == 0 ? &bars[L::kKFull] : &bars[L::kVFull + ((x.n_tile + i) & 1)]);
                         if (which == 1) mbar_arrive(&bars[L::kRawEmpty + st]);
                     }
                 }
             }
-        } else if (warp == 12) {
+            });
+        } else if (warp == 14) {
+            pieces([&](const Piece& pc, const Tiles& x) {
             // ------------------------------------------------------------ producer
             const int ppt = kKt >> p.c.page_shift;  // pages per tile; lane j < ppt takes page j
             const int gpp = p.c.page >> 4;
             auto id_of = [&](int tile) {
                 const int pg = tile * ppt + lane;
-                return (lane < ppt && tile < tp && (pg << p.c.page_shift) < len) ? page_id(p.c, pc.b, pg) : -1;
+                return (lane < ppt && tile < x.tp && (pg << p.c.page_shift) < pc.len) ? page_id(p.c, pc.b, pg) : -1;
             };
-            int id = id_of(pc.t0);
-            for (int i = 0; i < ntiles && ok; ++i) {
-                const int tile = pc.t0 + i;
-                const uint32_t nr = n_raw + i, st = nr % kStages;
-                const int id_next = i + 1 < ntiles ? id_of(tile + 1) : -1;
+            int id = id_of(pc.g0);
+            for (int i = 0; i < x.ntiles && ok; ++i) {
+                const int tile = pc.g0 + i;
+                const uint32_t nr = x.n_tile + i, st = nr % kStages;
+                const int id_next = i + 1 < x.ntiles ? id_of(tile + 1) : -1;
                 if (nr >= (uint32_t)kStages) {
                     ok &= mbar_wait(&bars[L::kRawEmpty + st], (nr / kStages - 1) & 1, kTries);
                     ok = __all_sync(MFD_FULL_MASK, ok);
@@ -534,10 +514,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     const uint32_t half = (uint32_t)(p.c.page * kD);
                     const uint32_t dst = sbase + L::kOffRaw + st * kRawBytes + lane * half;
                     mbar_expect_tx(bar, 2 * half);
-                    tma_page(dst, &tmk, bar, pc.hk, id);
-                    tma_page(dst + kRawBytes / 2, &tmv, bar, pc.hk, id);
-                    const float sk = __ldg(p.c.k_scale + (int64_t)id * p.c.Hkv + pc.hk);
-                    const float sv = fmaxf(__ldg(p.c.v_scale + (int64_t)id * p.c.Hkv + pc.hk), kScaleFloor);
+                    tma_page(dst, &tmk, bar, x.hk, id);
+                    tma_page(dst + kRawBytes / 2, &tmv, bar, x.hk, id);
+                    const float sk = __ldg(p.c.k_scale + (int64_t)id * p.c.Hkv + x.hk);
+                    const float sv = fmaxf(__ldg(p.c.v_scale + (int64_t)id * p.c.Hkv + x.hk), kScaleFloor);
                     const float4 k = make_float4(sk * p.scale_log2, __log2f(sv), __frcp_rn(sv), 0.f);
                     for (int g = 0; g < gpp; ++g) cst[lane * gpp + g] = k;
                 } else if (lane < ppt) {
@@ -550,32 +530,38 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 id = id_next;
                 issued = nr + 1;
             }
-        } else if (lane == 0) {
+            });
+            if (*s_failed)  // copies in flight end before the CTA does (bounded)
+                for (uint32_t f = issued > kStages ? issued - kStages : 0u; f < issued; ++f)
+                    mbar_wait(&bars[L::kRawFull + f % kStages], (f / kStages) & 1, 1u << 14);
+        } else {
+            pieces([&](const Piece& pc, const Tiles& x) {
+                if (lane != 0) return;
             // ------------------------------------------------------------ MMA issuer
             constexpr uint32_t kIdescS = idesc_bf16(128, kKt, 0);
             constexpr uint32_t kIdescO = idesc_bf16(128, kD, 1);
             auto scores = [&](int s) {
-                const int i = alternate ? s : s >> 1, grp = s & 1;
-                if (alternate || grp == 0) {
-                    ok &= mbar_wait(&bars[L::kKFull], (n_k + i) & 1, kTries);
+                const int i = x.alternate ? s : s >> 1, grp = s & 1;
+                if (x.alternate || grp == 0) {
+                    ok &= mbar_wait(&bars[L::kKFull], (x.n_tile + i) & 1, kTries);
                     tc_fence_after();
                 }
-                const uint32_t q = sbase + L::kOffQ + (alternate ? 0 : grp * kTileBytes), k = sbase + L::kOffK;
+                const uint32_t q = sbase + L::kOffQ + (x.alternate ? 0 : grp * kTileBytes), k = sbase + L::kOffK;
 #pragma unroll
                 for (int ks = 0; ks < 8; ++ks)
                     umma(tmem + 256 + 128 * grp, sw128_desc(q, ks, 128), sw128_desc(k, ks, 128), kIdescS, ks > 0);
                 umma_commit(&bars[L::kSFull + grp]);
-                if (alternate || grp == 1) umma_commit(&bars[L::kKEmpty]);
+                if (x.alternate || grp == 1) umma_commit(&bars[L::kKEmpty]);
             };
-            if (nsteps > 0) ok &= mbar_wait(&bars[L::kQFull], n_piece & 1, kTries);
+            if (x.nsteps > 0) ok &= mbar_wait(&bars[L::kQFull], x.n_piece & 1, kTries);
             tc_fence_after();
-            if (nsteps > 0 && ok) scores(0);
-            if (nsteps > 1 && ok) scores(1);
-            for (int s = 0; s < nsteps && ok; ++s) {
-                const int i = alternate ? s : s >> 1, grp = s & 1;
-                const uint32_t nv = n_v + i;
-                ok &= mbar_wait(&bars[L::kPFull + grp], (n_s[grp] + (s >> 1)) & 1, kTries);
-                if (alternate || grp == 0) ok &= mbar_wait(&bars[L::kVFull + (nv & 1)], (nv >> 1) & 1, kTries);
+            if (x.nsteps > 0 && ok) scores(0);
+            if (x.nsteps > 1 && ok) scores(1);
+            for (int s = 0; s < x.nsteps && ok; ++s) {
+                const int i = x.alternate ? s : s >> 1, grp = s & 1;
+                const uint32_t nv = x.n_tile + i;
+                ok &= mbar_wait(&bars[L::kPFull + grp], ((grp ? x.n_s1 : x.n_s0) + (s >> 1)) & 1, kTries);
+                if (x.alternate || grp == 0) ok &= mbar_wait(&bars[L::kVFull + (nv & 1)], (nv >> 1) & 1, kTries);
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t v = sbase + L::kOffV + (nv & 1) * kTileBytes, pt = tmem + 256 + 128 * grp;
@@ -587,93 +573,71 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     umma_ts(tmem + 128 * grp, pa + 16, vd, kIdescO, 1u);
                 }
                 umma_commit(&bars[L::kPV + grp]);
-                if (alternate || grp == 1) umma_commit(&bars[L::kVEmpty + (nv & 1)]);
-                if (s + 2 < nsteps) scores(s + 2);
+                if (x.alternate || grp == 1) umma_commit(&bars[L::kVEmpty + (nv & 1)]);
+                if (s + 2 < x.nsteps) scores(s + 2);
             }
+            });
         }
-        if (!ok) *s_failed = 1;
-        tc_fence_before();
-        __syncthreads();  // the piece is over for every role
-        tc_fence_after();
-        if (*s_failed) break;
-        n_piece += 1;
-        n_raw += ntiles, n_k += ntiles, n_v += ntiles;
-        n_s[0] += (nsteps + 1) >> 1, n_s[1] += nsteps >> 1;
-        if (tid == 0) *s_odd = 0;
-        __syncthreads();
     }
-    if (*s_failed) {
-        if (tid == 0) atomicExch(p.status, 1);
-        // copies in flight end before the CTA does (bounded)
-        if (warp == 12)
-            for (uint32_t f = issued > kStages ? issued - kStages : 0u; f < issued; ++f)
-                mbar_wait(&bars[L::kRawFull + f % kStages], (f / kStages) & 1, 1u << 14);
-    }
+    if (*s_failed && tid == 0) atomicExch(p.status, 1);
     tc_fence_before();
     __syncthreads();
-    if (warp == 13) {
+    if (warp == 15) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
 }
 
-// Adds up the pieces of every unit that was cut, in their order.  One warp per row of 128 columns at a time.
+// Adds up the pieces of every unit that was cut, in their order.  Block x is the CTA boundary (range cut: the first one
+// inside its unit; split: the unit's first piece) that answers for a unit, block y 32 of its rows; a warp takes 16
+// columns of them, lane = row, so every load of a piece is 512 contiguous bytes.
 template <bool PAIR>
 __global__ void __launch_bounds__(256) kv8_combine_kernel(const AttnParams p, int ctas) {
     constexpr int kRowsU = kSlotRows(PAIR);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Work w = make_work(p, kRowsU, ctas);
-    const int64_t rows = (int64_t)p.bs * w.per_req * kRowsU;
-    for (int64_t x = (int64_t)blockIdx.x * 8 + warp; x < rows; x += (int64_t)gridDim.x * 8) {
-        const int64_t unit = x / kRowsU;
-        const int r = (int)(x % kRowsU);
-        const int b = (int)(unit / w.per_req), u = (int)(unit % w.per_req);
-        const int hk = u / w.RB, rb = u % w.RB;
-        const int row = p.row0 + rb * kRowsU + r;
-        if (row >= p.rows) continue;
-        const int tiles = tiles_of(p, b);
-        // where the unit's pieces are
-        int64_t before = 0;
-        for (int b0 = 0; b0 < b; b0 += 32) {
-            const int o = b0 + lane;
-            unsigned v = 0u;
-            if (o < b) v = w.split ? (unsigned)((tiles_of(p, o) + w.per - 1) / w.per) : (unsigned)tiles_of(p, o);
-            before += __reduce_add_sync(MFD_FULL_MASK, v);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
+    const int RB = (p.rows - p.row0 + kRowsU - 1) / kRowsU;
+    auto tiles_of = [&](int len) { return max(1, (len + kKt - 1) / kKt + (p.nn + kKt - 1) / kKt); };
+    const Lengths lens(p.c, p.bs);
+    const Cut cut = make_cut(lens, tiles_of, p.c.Hkv * RB, ctas, 1);
+    int64_t pos, end;
+    cut_range(cut, cta, pos, end);
+    Piece pc;
+    if (!next_piece(lens, tiles_of, cut, cta, pos, end, pc)) return;
+    if (cut.split ? (pc.first != cta || pc.pieces == 1) : (pc.g0 == 0 || pc.first != cta - 1)) return;
+    const int hk = pc.u / RB, rb = pc.u % RB;
+    const int r = blockIdx.y * 32 + lane, row = p.row0 + rb * kRowsU + r;
+    if (row - lane >= p.rows) return;
+    float mm = -INFINITY;
+    for (int i = 0; i < pc.pieces; ++i) mm = fmaxf(mm, __ldg(p.part + slot_of(pc, i) * kSlotFloats(PAIR) + r));
+    float ll = 0.f;
+    float4 v[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+    for (int i = 0; i < pc.pieces; ++i) {
+        const float* s = p.part + slot_of(pc, i) * kSlotFloats(PAIR);
+        const float mi = __ldg(s + r), li = __ldg(s + kRowsU + r);
+        const float a = mi == -INFINITY ? 0.f : fast_exp2(mi - mm);
+        ll = fmaf(a, li, ll);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const float4 o = __ldg(reinterpret_cast<const float4*>(s + 2 * kRowsU) + (int64_t)(4 * warp + c) * kRowsU + r);
+            v[c].x = fmaf(a, o.x, v[c].x), v[c].y = fmaf(a, o.y, v[c].y);
+            v[c].z = fmaf(a, o.z, v[c].z), v[c].w = fmaf(a, o.w, v[c].w);
         }
-        before *= w.per_req;
-        int first, pieces;
-        bool second = false;  // the first piece is its CTA's second slot
-        if (w.split) {
-            pieces = (int)((tiles + w.per - 1) / w.per);
-            first = (int)(before + (int64_t)u * pieces);
-        } else {
-            const int64_t lo = before + (int64_t)u * tiles;
-            first = (int)(lo / w.per);
-            pieces = (int)((lo + tiles - 1) / w.per) - first + 1;
-            second = (int64_t)first * w.per < lo;
-        }
-        if (pieces == 1) continue;  // written by its CTA
-        auto slot_of = [&](int i) { return p.part + (int64_t)(2 * (first + i) + (second && i == 0 ? 1 : 0)) * kSlotFloats(PAIR); };
-        float mm = -INFINITY, ll = 0.f;
-        for (int i = lane; i < pieces; i += 32) mm = fmaxf(mm, __ldg(slot_of(i) + r));
-        mm = warp_max_f32(mm);
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int i = 0; i < pieces; ++i) {
-            const float* s = slot_of(i);
-            const float mi = __ldg(s + r), li = __ldg(s + kRowsU + r);
-            const float4 o = __ldg(reinterpret_cast<const float4*>(s + 2 * kRowsU) + (int64_t)lane * kRowsU + r);
-            const float a = mi == -INFINITY ? 0.f : fast_exp2(mi - mm);
-            ll = fmaf(a, li, ll);
-            v.x = fmaf(a, o.x, v.x), v.y = fmaf(a, o.y, v.y), v.z = fmaf(a, o.z, v.z), v.w = fmaf(a, o.w, v.w);
-        }
-        const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
-        const int node = row / p.G, head = hk * p.G + row % p.G;
-        *reinterpret_cast<uint2*>(p.out + (int64_t)b * p.so_b + (int64_t)node * p.so_n + (int64_t)head * p.so_h + 4 * lane) =
-            make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
-        if (p.lse && lane == 0)
-            p.lse[((int64_t)b * p.n + node) * p.H + head] = ll == 0.f ? -INFINITY : 0.6931471805599453f * (mm + log2f(ll));
     }
+    if (row >= p.rows) return;
+    const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
+    const int node = row / p.G, head = hk * p.G + row % p.G;
+    uint4* dst = reinterpret_cast<uint4*>(p.out + (int64_t)pc.b * p.so_b + (int64_t)node * p.so_n + (int64_t)head * p.so_h +
+                                          16 * warp);
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+        dst[c] = make_uint4(pack_bf16(v[2 * c].x * inv, v[2 * c].y * inv), pack_bf16(v[2 * c].z * inv, v[2 * c].w * inv),
+                            pack_bf16(v[2 * c + 1].x * inv, v[2 * c + 1].y * inv),
+                            pack_bf16(v[2 * c + 1].z * inv, v[2 * c + 1].w * inv));
+    if (p.lse && warp == 0)
+        p.lse[((int64_t)pc.b * p.n + node) * p.H + head] = ll == 0.f ? -INFINITY : 0.6931471805599453f * (mm + log2f(ll));
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -716,7 +680,8 @@ int launch_tc_one(const AttnParams& p, int sms, cudaStream_t stream) {
     }
     kv8_tc_kernel<FP8, PAIR><<<sms, kTcThreads, Layout<PAIR>::kBytes, stream>>>(tk, tv, p);
     MFD_CHECK_LAUNCH("mfd_kv8_attention");
-    kv8_combine_kernel<PAIR><<<2 * sms, 256, 0, stream>>>(p, sms);
+    const int rows = p.rows - p.row0 < kSlotRows(PAIR) ? p.rows - p.row0 : kSlotRows(PAIR);
+    kv8_combine_kernel<PAIR><<<dim3((unsigned)sms, (unsigned)((rows + 31) / 32)), 256, 0, stream>>>(p, sms);
     MFD_CHECK_LAUNCH("mfd_kv8_attention (combination)");
     return MFD_OK;
 }

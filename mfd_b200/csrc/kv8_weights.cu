@@ -51,21 +51,22 @@ __global__ void __launch_bounds__(kWThreads, kWCtasPerSm) kv8_weights_kernel(con
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
     const int Hkv = p.c.Hkv;
-    auto tasks_of = [&](int b) { return max(1, (seq_len(p.c, b) + 31) / 32); };
-    const int64_t total = over_requests(p.bs, tasks_of) * Hkv;
-    int64_t per = (total + gridDim.x - 1) / gridDim.x;
+    auto tasks_of = [&](int len) { return max(1, (len + 31) / 32); };
+    const Lengths lens(p.c, p.bs);
+    const int64_t total = lens.sum(tasks_of, p.bs) * Hkv;
+    int64_t per = quotient(total + gridDim.x - 1, gridDim.x);
     if (per < kWWarps) per = kWWarps;
     int64_t pos = (int64_t)blockIdx.x * per;
     const int64_t end = pos + per < total ? pos + per : total;
-    auto span_of = [&](int b) { return (int64_t)Hkv * tasks_of(b); };
 
     while (pos < end) {
         int64_t before;
-        const int b = find_request(p.bs, pos, span_of, before);
+        int len;
+        const int b = lens.find(pos, Hkv, tasks_of, before, len);
         if (b < 0) return;
-        const int tasks = tasks_of(b), len = seq_len(p.c, b);
+        const int tasks = tasks_of(len);
         const int64_t off = pos - before;
-        const int hk = (int)(off / tasks), t0 = (int)(off % tasks);
+        const int hk = (int)quotient(off, tasks), t0 = (int)(off - (int64_t)hk * tasks);
         const int t1 = (int)min((int64_t)tasks, t0 + (end - pos));
         const int listed = listed_rows(p.path, p.path_stride, p.rows, p.counts, p.n, b);
         const int nrows = listed * p.G;
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(kWThreads, kWCtasPerSm) kv8_weights_kernel(con
         // ---- the request's last CTA adds up its pages
         if (pos >= end || pos >= before + (int64_t)tasks * Hkv) {
             const int64_t last = before + (int64_t)tasks * Hkv - 1;
-            const int pieces = (int)(last / per - before / per) + 1;
+            const int pieces = (int)(quotient(last, per) - quotient(before, per)) + 1;
             __threadfence();
             __syncthreads();
             if (tid == 0) s_last = pieces == 1 || atomicAdd(p.tickets + b, 1u) == (unsigned)(pieces - 1);
