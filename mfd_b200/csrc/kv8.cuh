@@ -225,10 +225,14 @@ __device__ __forceinline__ Cut make_cut(const Lengths& lens, F f, int per_req, i
     const int64_t units = (int64_t)lens.bs * per_req;
     w.total = lens.sum(f, lens.bs) * per_req;
     w.split = units * 2 <= (int64_t)ctas;
-    const int64_t n = w.split ? ctas - units : ctas;  // (pieces <= total / per + units)
-    w.per = quotient(w.total + n - 1, n);
-    w.per = w.split ? quotient(w.per + least - 1, least) * least : (w.per < least ? least : w.per);
+    w.per = quotient(w.total + ctas - 1, ctas);
     if (w.per < least) w.per = least;
+    if (w.split) {
+        // the smallest piece (nearly: 1/16 steps) of which there are at most ctas; total / (ctas - units) always is one
+        w.per = quotient(w.per + least - 1, least) * least;
+        const int64_t step = max((int64_t)least, quotient(w.per, 16 * least) * least);
+        while (lens.sum([&](int len) { return quotient(f(len) + w.per - 1, w.per); }, lens.bs) * per_req > ctas) w.per += step;
+    }
     return w;
 }
 // [begin, end) of CTA `cta`: a range of the work, or (split) a piece's number

@@ -231,48 +231,38 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (quarter_live && ok) {
                     const float4* cst = consts + (size_t)((x.n_tile + tile - pc.g0) & (kRing - 1)) * 8;
                     // visibility of the tile's keys, 32 a word
-                    uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
-                    bool masked = false;
-                    if (tile < x.tp) {
-                        const int valid = pc.len - tile * kKt;
-                        if (valid < kKt) {
-                            masked = true;
-#pragma unroll
-                            for (int c = 0; c < 4; ++c)
-                                vis[c] = valid >= 32 * c + 32 ? ~0u : (valid <= 32 * c ? 0u : (1u << (valid - 32 * c)) - 1u);
-                        }
-                    } else {
-                        masked = true;
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            const uint64_t v = live ? visible_word(p, pc.b, node, 2 * (tile - x.tp) + c) : 0ull;
-                            vis[2 * c] = (uint32_t)v;
-                            vis[2 * c + 1] = (uint32_t)(v >> 32);
-                        }
-                    }
-                    uint32_t u[4][32];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_ld32_issue(s_tm + 32 * c, u[c]);
-                    tmem_ld_wait(u);
-                    if (masked) {
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
+                    const int valid = pc.len - tile * kKt;
+                    const bool masked = tile >= x.tp || valid < kKt;
+                    auto visible = [&](int c) -> uint32_t {
+                        if (tile < x.tp)
+                            return valid >= 32 * c + 32 ? ~0u : (valid <= 32 * c ? 0u : (1u << (valid - 32 * c)) - 1u);
+                        const uint64_t v = live ? visible_word(p, pc.b, node, 2 * (tile - x.tp) + (c >> 1)) : 0ull;
+                        return (uint32_t)(v >> (32 * (c & 1)));
+                    };
+                    float mx = -INFINITY;
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {  // (rolled: the unrolled step misses the instruction cache)
+                        uint32_t u[1][32];
+                        tmem_ld32_issue(s_tm + 32 * c, u[0]);
+                        tmem_ld_wait(u);
+                        if (masked) {
+                            const uint32_t vis = visible(c);
 #pragma unroll
                             for (int j = 0; j < 32; ++j)
-                                if (!((vis[c] >> j) & 1u)) u[c][j] = 0xff800000u;
-                    }
-                    float mx = -INFINITY;
+                                if (!((vis >> j) & 1u)) u[0][j] = 0xff800000u;
+                        }
 #pragma unroll
-                    for (int g = 0; g < 8; ++g) {  // 16 keys: one page
-                        const uint32_t* su = &u[g >> 1][16 * (g & 1)];
-                        float a[6];
+                        for (int q = 0; q < 2; ++q) {  // 16 keys: one page
+                            float a[6];
 #pragma unroll
-                        for (int j = 0; j < 5; ++j)
-                            a[j] = fmax3(__uint_as_float(su[3 * j]), __uint_as_float(su[3 * j + 1]), __uint_as_float(su[3 * j + 2]));
-                        a[5] = __uint_as_float(su[15]);
-                        const float top = fmaxf(fmax3(a[0], a[1], a[2]), fmax3(a[3], a[4], a[5]));
-                        const float2 k = *reinterpret_cast<const float2*>(cst + g);
-                        mx = fmaxf(mx, top == -INFINITY ? top : fmaf(top, k.x, k.y));
+                            for (int j = 0; j < 5; ++j)
+                                a[j] = fmax3(__uint_as_float(u[0][16 * q + 3 * j]), __uint_as_float(u[0][16 * q + 3 * j + 1]),
+                                             __uint_as_float(u[0][16 * q + 3 * j + 2]));
+                            a[5] = __uint_as_float(u[0][16 * q + 15]);
+                            const float top = fmaxf(fmax3(a[0], a[1], a[2]), fmax3(a[3], a[4], a[5]));
+                            const float2 k = *reinterpret_cast<const float2*>(cst + 2 * c + q);
+                            mx = fmaxf(mx, top == -INFINITY ? top : fmaf(top, k.x, k.y));
+                        }
                     }
                     float alpha = 1.f;
                     bool rescale = false;
@@ -282,8 +272,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                     const float mr = m == -INFINITY ? 0.f : m;
                     uint64_t acc[2] = {0ull, 0ull};
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
+                        uint32_t u[1][32];
+                        tmem_ld32_issue(s_tm + 32 * c, u[0]);
+                        tmem_ld_wait(u);
+                        if (masked) {
+                            const uint32_t vis = visible(c);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (!((vis >> j) & 1u)) u[0][j] = 0xff800000u;
+                        }
                         uint32_t hl[32];  // hi pairs, then lo pairs
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
@@ -293,7 +292,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             for (int j = 0; j < 8; ++j) {
                                 const int e = 16 * q + 2 * j;
                                 float x0, x1;
-                                upk2(fma2(pk2(__uint_as_float(u[c][e]), __uint_as_float(u[c][e + 1])), kc, kd), x0, x1);
+                                upk2(fma2(pk2(__uint_as_float(u[0][e]), __uint_as_float(u[0][e + 1])), kc, kd), x0, x1);
                                 const uint64_t w = pk2(fast_exp2(x0), fast_exp2(x1));
                                 acc[j & 1] = fma2(w, ki, acc[j & 1]);
                                 split_bf16(w, hl[8 * q + j], hl[16 + 8 * q + j]);
