@@ -91,6 +91,22 @@ __device__ __forceinline__ void split_bf16(uint64_t w, uint32_t& hi, uint32_t& l
     lo = __byte_perm((uint32_t)left, (uint32_t)(left >> 32), 0x7632);
 }
 
+// The same as float16 hi + lo, rounded: 22 bits of each down to 2^-24 (the caller lifts the weights well above it).
+__device__ __forceinline__ void split_half(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    const __half2 r = __floats2half2_rn(a - f.x, b - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// the 8 x 8 transpose of 16-bit values held two a lane (row lane / 4, columns 2 (lane % 4) and the next)
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -153,9 +169,16 @@ __device__ __forceinline__ int listed_rows(const int64_t* path, int64_t path_str
     return c;
 }
 
-// a / b for a >= 0, b > 0: the 32-bit quotient where it suffices (the 64-bit one takes several times as long)
+// a / b for a >= 0, b > 0.  Small ones (all but extreme cases) by a reciprocal estimate, within one of the quotient, and
+// its correction: a few instructions where the 64-bit division takes hundreds of cycles at every CTA's start.
 __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
-    if (((uint64_t)(a | b) >> 32) == 0) return (int64_t)((uint32_t)a / (uint32_t)b);
+    if (((uint64_t)(a | b) >> 22) == 0) {
+        const int x = (int)a, y = (int)b;
+        int q = __float2int_rz(__fdividef((float)x, (float)y));
+        const int r = x - q * y;
+        q += r >= y ? 1 : (r < 0 ? -1 : 0);
+        return q;
+    }
     return a / b;
 }
 
@@ -293,13 +316,20 @@ __device__ __forceinline__ int64_t slot_of(const Piece& pc, int i) {
     return 2 * (int64_t)(pc.first + i) + (pc.second && i == 0 ? 1 : 0);
 }
 
+// over the lanes with the same lane % 4
+__device__ __forceinline__ float column_max(float v) {
+    v = fmaxf(v, __shfl_xor_sync(MFD_FULL_MASK, v, 4));
+    v = fmaxf(v, __shfl_xor_sync(MFD_FULL_MASK, v, 8));
+    return fmaxf(v, __shfl_xor_sync(MFD_FULL_MASK, v, 16));
+}
+__device__ __forceinline__ float column_sum(float v) {
+    v += __shfl_xor_sync(MFD_FULL_MASK, v, 4);
+    v += __shfl_xor_sync(MFD_FULL_MASK, v, 8);
+    return v + __shfl_xor_sync(MFD_FULL_MASK, v, 16);
+}
 __device__ __forceinline__ float quad_max(float v) {
     v = fmaxf(v, __shfl_xor_sync(MFD_FULL_MASK, v, 1));
     return fmaxf(v, __shfl_xor_sync(MFD_FULL_MASK, v, 2));
-}
-__device__ __forceinline__ float quad_sum(float v) {
-    v += __shfl_xor_sync(MFD_FULL_MASK, v, 1);
-    return v + __shfl_xor_sync(MFD_FULL_MASK, v, 2);
 }
 // SMs of the current device, and the opt-in to a kernel's dynamic shared memory, asked of the driver once per device
 int sm_count();

@@ -1,25 +1,26 @@
 // kv8_attention_rows.cu -- attention of a few query rows over the 8-bit paged cache: the decode step and short drafts.
 //
 // The mathematics, for a row with query q over keys j (page P(j), codes a_j and c_j, scales sk and sv):
-//   score  s_j = sk (q . a_j) scale log2(e),      w_j = s_j + log2(sv),      m = max_j w_j
+//   score  s_j = sk (q . a_j) scale log2(e),      w_j = s_j + log2(sv),      m = max_j w_j - 12
 //   O = sum_j 2^(w_j - m) c_j,   l = sum_j 2^(w_j - m) / sv,                 out = O / l,  lse = ln2 (m + log2 l)
-// so the value scale rides in the exponent and no code is multiplied by its scale.  The scores are products of float16
-// operands (codes and the query row divided by a power of two are exact there), for the nodes' own keys of bf16
-// operands.  The weights meet the values in bf16 as hi + lo, two tensor instructions: one bf16 weight (8 bits) would
-// err by as much as the output's own rounding, and float16 (11 bits) loses a small weight beside a large one in a
-// column where the large one's code is 0; hi + lo keeps 16 bits over the whole float32 range.  All sums and statistics
-// are float32.
+// so the value scale rides in the exponent and no code is multiplied by its scale.  The products have float16 operands
+// and float32 sums: codes are exact there, and so is the query row divided by a power of two.  The weights go in as
+// float16 hi + lo, two tensor instructions, lifted to at most 2^15: 22 bits of a weight, down to 2^-37 of the row's
+// largest.  (One float16 or bf16 weight would err by a good part of the output's own rounding.)  The nodes' own bf16
+// keys and values take bf16 operands, the weights hi + lo as well.  All sums and statistics are float32.
 //
-// Bound: bytes (256 codes a token and KV head for 4 G n multiply-adds each).  So the codes go from memory straight to
-// registers, 16 bytes a lane, in a layout in which they are the operands: the d index of the first product is permuted
-// (lane quad t holds d = 16 t .. 16 t + 15 of either half row, the query alike), and the value rows of two keys are
-// interleaved byte by byte before they become float16 pairs.  No shared memory is touched in the loop.
-//   scores   m16n8k16: A = query rows (16), B = 8 keys; lane (g, t) loads 32 bytes of key g's row
-//   values   m16n8k16: A = weights (16 rows x 16 keys, the score registers), B = 16 keys x 8 columns; lane (g, t) loads
-//            columns 16 g .. 16 g + 15 of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9, so column tile j is d = 16 g + j
-// A warp takes 16 keys at a time (one page has all 16: one scale), its 8 loads in flight together; 16 warps an SM
-// hold 64 KB in flight.  The 8 warps of a CTA take every eighth group of 16 keys with their own (m, l, O) and merge in
-// shared memory at the end of the piece.
+// Bound: bytes (256 codes a token and KV head for 4 G n multiply-adds each); next, instructions: turning the codes into
+// operands.  So the codes go from memory straight to registers, 16 bytes a lane, in a layout in which they are the
+// wide operand of the tensor instruction and the query rows, which are few, the narrow one:
+//   scores   m16n8k16: A = 16 keys, B = 8 query rows; the d index is permuted (lane (g, t) holds d = 16 t .. 16 t + 15 of
+//            either half row of keys g and g + 8, the query alike), so a lane's operand registers are its bytes in order
+//   values   m16n8k16: A = 16 columns of the values x 16 keys, B = the weights (the scores' registers transposed by
+//            movmatrix); lane (g, t) loads d = 16 g .. 16 g + 15 of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 and interleaves
+//            the bytes of two keys before they become float16 pairs; column tile j is d = 16 g + 2 j and the next
+// A warp takes 16 keys at a time (one page has all 16: one scale).  The next group's K loads are issued when the scores
+// have consumed this one's registers, its V loads when the products have, so a load has most of a group's time to
+// arrive without a second set of registers.  The 8 warps of a CTA take every eighth group with their own (m, l, O) and
+// merge in shared memory at the end of the piece.
 //
 // Split: the groups of all (request, KV head, 16 rows) units are laid end to end and cut into equal pieces, one per
 // CTA (two CTAs an SM), so ragged lengths balance and one long request fills the GPU; the lengths are read on the
@@ -33,28 +34,29 @@ namespace kv8 {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kTBlock = 36, kRowStride = 4 * kTBlock;  // floats: a lane quad's 32 columns, padded against bank conflicts
-constexpr int kSlot = 16 * (kD + 2);                   // floats of a partial: m[16], l[16], O[16][128]
+// floats: a lane's 16 columns, padded so that the 8 lanes of a store hit different banks
+constexpr int kDBlock = 20, kRowStride = 8 * kDBlock + 4;
+constexpr int kSlot = 16 * (kD + 2);  // floats of a partial: m[16], l[16], O[16][128]
 constexpr int kCtasPerSm = 2;
+constexpr float kLift = 12.f;  // the largest weights are 2^12, and up to 2^15 before the reference moves
+constexpr float kLazy = 3.f;
 
 __device__ __forceinline__ bool not_finite_pair(uint32_t w) {  // a bf16 pair holds an infinity or a NaN
     return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
 
-// TALL: 16 rows a unit, else at most 8 (rows 8 .. 15 of every product are zero and cost no registers)
-template <bool FP8, bool TALL>
+// NT: 8-row tiles a unit
+template <bool FP8, int NT>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const AttnParams p) {
-    constexpr int kHalves = TALL ? 2 : 1;  // row halves (g and g + 8) a lane holds
-    constexpr int kRows = 8 * kHalves;
+    constexpr int kRows = 8 * NT;
     extern __shared__ __align__(16) float smem[];  // [kWarps][kRows][kRowStride]; merge weights
     __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
-    __shared__ uint32_t s_q[8][32][2 * kHalves];  // query operands of the 8 16-column steps, the same for every warp
+    __shared__ uint2 s_q[NT == 1 ? 1 : NT][8][32];  // query operands, where two tiles of them would not fit the registers
     __shared__ int s_last;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
     const int nrows = p.rows - p.row0;
     const int RB = (nrows + 15) / 16;
-
     // ---- this CTA's share of the work, in groups of 16 keys (cached tokens, then own keys)
     auto groups_of = [&](int len) { return max(1, (len + 15) / 16 + (p.nn + 15) / 16); };  // (one, to write zeros)
     const Lengths lens(p.c, p.bs);
@@ -67,23 +69,53 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
         const int hk = pc.u / RB, rb = pc.u % RB, len = pc.len;
         const int gp = (len + 15) / 16;  // groups of cached tokens; own keys follow
         const int base = p.row0 + rb * 16;
+        const int g_cached = min(pc.g1, gp);
 
-        // ---- the query rows as float16 operands, divided by a power of two
-        float rf[kHalves];            // score factor of the row: the power of two, the scale and log2(e)
-        int node[kHalves];
-        const __nv_bfloat16* qrow[kHalves];
+        // ---- the first group's codes, before anything waits
+        const uint8_t* kbase = p.c.k + (int64_t)hk * p.c.sc_h + (int64_t)g * p.c.sc_t + 16 * t;
+        const uint8_t* vbase = p.c.v + (int64_t)hk * p.c.sc_h + (int64_t)(2 * t) * p.c.sc_t + 16 * g;
+        const int slot_mask = p.c.page - 1;
+        uint4 kw[2][2], vw[4];  // K: key g, g + 8; d half.  V: keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+        float sk = 0.f, sv = 1.f;
+        auto offset = [&](int gi, int id) {
+            return (int64_t)id * p.c.sc_p + (int64_t)((gi * 16) & slot_mask) * p.c.sc_t;
+        };
+        auto load_k = [&](int gi, int id) {
+            const uint8_t* src = kbase + offset(gi, id);
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-            const int r = base + g + 8 * h;
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) kw[h][i] = ldg_stream_u4(src + (int64_t)(8 * h) * p.c.sc_t + 64 * i);
+        };
+        auto load_v = [&](int gi, int id) {
+            const uint8_t* src = vbase + offset(gi, id);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) vw[i] = ldg_stream_u4(src + (int64_t)((i & 1) + 8 * (i >> 1)) * p.c.sc_t);
+        };
+        auto id_of = [&](int gi) { return gi < g_cached ? page_id(p.c, pc.b, (gi * 16) >> p.c.page_shift) : 0; };
+        int gi = pc.g0 + warp;
+        int id = id_of(gi), id_next = id_of(gi + kWarps);
+        if (gi < g_cached) {
+            load_k(gi, id);
+            load_v(gi, id);
+            sk = __ldg(p.c.k_scale + (int64_t)id * p.c.Hkv + hk);
+            sv = __ldg(p.c.v_scale + (int64_t)id * p.c.Hkv + hk);
+        }
+
+        // ---- query row g (+ 8 nt) as float16 operands, divided by a power of two; the lane's softmax rows are 2 t, 2 t + 1
+        uint32_t qb[8][2];
+        float rf[NT][2];  // score factor of rows 2 t and 2 t + 1: the power of two, the scale and log2(e)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int r = base + 8 * n + g;
             const bool live = r < p.rows;
-            node[h] = live ? r / p.G : -1;
-            qrow[h] = p.q + (int64_t)pc.b * p.sq_b + (int64_t)(live ? r / p.G : 0) * p.sq_n +
-                      (int64_t)(hk * p.G + (live ? r % p.G : 0)) * p.sq_h;
+            const int nd = live ? r / p.G : 0, hd = hk * p.G + (live ? r - nd * p.G : 0);
+            const __nv_bfloat16* qrow = p.q + (int64_t)pc.b * p.sq_b + (int64_t)nd * p.sq_n + (int64_t)hd * p.sq_h;
             uint4 x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {  // columns 16 t + 8 (i & 1) + 64 (i >> 1) ..
                 x[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (live) x[i] = __ldg(reinterpret_cast<const uint4*>(qrow[h] + 16 * t + 8 * (i & 1) + 64 * (i >> 1)));
+                if (live) x[i] = __ldg(reinterpret_cast<const uint4*>(qrow + 16 * t + 8 * (i & 1) + 64 * (i >> 1)));
             }
             float mx = 0.f;
 #pragma unroll
@@ -98,204 +130,206 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
             mx = quad_max(mx);
             float down, up;
             row_power(mx, down, up);
-            rf[h] = up * p.scale_log2;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {  // 8 columns: words 2 (i & 1), 2 (i & 1) + 1 of half i >> 1
+            for (int e = 0; e < 2; ++e) rf[n][e] = __shfl_sync(MFD_FULL_MASK, up, 4 * (2 * t + e)) * p.scale_log2;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
                 const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const float2 f0 = bf2(w[2 * j]), f1 = bf2(w[2 * j + 1]);
                     const int ks = 4 * (i >> 1) + 2 * (i & 1) + j;
-                    if (warp == 0) {  // rows g, g + 8 at columns k, then both at k + 8
-                        s_q[ks][lane][h] = pack_half2(f0.x * down, f0.y * down);
-                        s_q[ks][lane][kHalves + h] = pack_half2(f1.x * down, f1.y * down);
-                    }
+                    const uint32_t b0 = pack_half2(f0.x * down, f0.y * down), b1 = pack_half2(f1.x * down, f1.y * down);
+                    if (NT == 1) qb[ks][0] = b0, qb[ks][1] = b1;
+                    else if (warp == 0) s_q[n][ks][lane] = make_uint2(b0, b1);
                 }
             }
         }
-        __syncthreads();
 
-        float o[16][2 * kHalves];
-        float m[kHalves], l[kHalves];
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-#pragma unroll
-            for (int e = 0; e < 2 * kHalves; ++e) o[j][e] = 0.f;
-#pragma unroll
-        for (int h = 0; h < kHalves; ++h) m[h] = -INFINITY, l[h] = 0.f;
+        if (NT > 1) __syncthreads();
 
-        // the softmax step of a group: raw scores sc[key tile][row half x 2] already scaled into w (log2), -inf where
-        // masked; returns the weights, rescales O
-        auto step = [&](float (&w)[2][2 * kHalves], float inv_sv) {
-            float mx[kHalves];
+        // O of rows 2 t, 2 t + 1 (+ 8 n): o[n][j] = d 16 g + 2 j (both rows), then the next d (both rows)
+        float o[NT][8][4];
+        float m[NT][2], l[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[n][j][e] = 0.f;
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+        }
+
+        // the softmax step of a group: w (log2; -inf where masked) of key g (row 2 t, 2 t + 1), then key g + 8, becomes
+        // the weights; O is rescaled when a row's reference moves
+        auto step = [&](float (&w)[NT][4], float inv_sv) {
             bool grow = false;
+            float mx[NT][2];
 #pragma unroll
-            for (int h = 0; h < kHalves; ++h) {
-                mx[h] = quad_max(fmaxf(fmaxf(w[0][2 * h], w[0][2 * h + 1]), fmaxf(w[1][2 * h], w[1][2 * h + 1])));
-                // a maximum that grows by less than 2^8 is left: a rescale of O costs more than the range
-                grow |= mx[h] > m[h] + 8.f || (m[h] == -INFINITY && mx[h] > -INFINITY);
-            }
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    mx[n][e] = column_max(fmaxf(w[n][e], w[n][2 + e])) - kLift;
+                    grow |= mx[n][e] > m[n][e] + kLazy || (m[n][e] == -INFINITY && mx[n][e] > -INFINITY);
+                }
             if (__any_sync(MFD_FULL_MASK, grow)) {
 #pragma unroll
-                for (int h = 0; h < kHalves; ++h) {
-                    const float mn = fmaxf(m[h], mx[h]);
-                    const float a = m[h] == -INFINITY ? 0.f : fast_exp2(m[h] - mn);
-                    m[h] = mn;
-                    l[h] *= a;
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) o[j][2 * h] *= a, o[j][2 * h + 1] *= a;
+                    for (int e = 0; e < 2; ++e) {
+                        const float mn = fmaxf(m[n][e], mx[n][e]);
+                        const float a = m[n][e] == -INFINITY ? 0.f : fast_exp2(m[n][e] - mn);
+                        m[n][e] = mn;
+                        l[n][e] *= a;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) o[n][j][e] *= a, o[n][j][2 + e] *= a;
+                    }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float mr = m[n][e] == -INFINITY ? 0.f : m[n][e];
+                    w[n][e] = fast_exp2(w[n][e] - mr);
+                    w[n][2 + e] = fast_exp2(w[n][2 + e] - mr);
+                    l[n][e] = fmaf(w[n][e] + w[n][2 + e], inv_sv, l[n][e]);
                 }
-            }
-#pragma unroll
-            for (int h = 0; h < kHalves; ++h) {
-                const float mr = m[h] == -INFINITY ? 0.f : m[h];
-                float sum = 0.f;
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) sum += w[kt][2 * h + e] = fast_exp2(w[kt][2 * h + e] - mr);
-                l[h] = fmaf(sum, inv_sv, l[h]);
-            }
-        };
-
-        // O's column tile += weights (hi + lo) x 16 keys of it
-        auto values = [&](float (&oj)[2 * kHalves], const uint32_t (&hi)[2][kHalves], const uint32_t (&lo)[2][kHalves],
-                          uint32_t b0, uint32_t b1) {
-            float d[4] = {oj[0], oj[1], TALL ? oj[2 * kHalves - 2] : 0.f, TALL ? oj[2 * kHalves - 1] : 0.f};
-            mma_bf16(d, hi[0][0], TALL ? hi[0][kHalves - 1] : 0u, hi[1][0], TALL ? hi[1][kHalves - 1] : 0u, b0, b1);
-            mma_bf16(d, lo[0][0], TALL ? lo[0][kHalves - 1] : 0u, lo[1][0], TALL ? lo[1][kHalves - 1] : 0u, b0, b1);
-            oj[0] = d[0], oj[1] = d[1];
-            if (TALL) oj[2 * kHalves - 2] = d[2], oj[2 * kHalves - 1] = d[3];
         };
 
         // ---- cached tokens
-        const uint8_t* kbase = p.c.k + (int64_t)hk * p.c.sc_h + (int64_t)g * p.c.sc_t + 16 * t;
-        const uint8_t* vbase = p.c.v + (int64_t)hk * p.c.sc_h + (int64_t)(2 * t) * p.c.sc_t + 16 * g;
-        const int slot_mask = p.c.page - 1;
-        int gi = pc.g0 + warp;
-        int id_next = gi < min(pc.g1, gp) ? page_id(p.c, pc.b, (gi * 16) >> p.c.page_shift) : 0;
-        for (; gi < min(pc.g1, gp); gi += kWarps) {
+        for (; gi < g_cached; gi += kWarps) {
             const int key0 = gi * 16;
-            const int id = id_next;
-            const int64_t off = (int64_t)id * p.c.sc_p + (int64_t)(key0 & slot_mask) * p.c.sc_t;
-            uint4 kw[2][2], vw[4];
+            const bool tail = key0 + 16 > len, more = gi + kWarps < g_cached;
+            float acc[NT][4];
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    kw[kt][i] = ldg_stream_u4(kbase + off + (int64_t)(8 * kt) * p.c.sc_t + 64 * i);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-                vw[i] = ldg_stream_u4(vbase + off + (int64_t)((i & 1) + 8 * (i >> 1)) * p.c.sc_t);
-            const float sk = __ldg(p.c.k_scale + (int64_t)id * p.c.Hkv + hk);
-            const float sv = fmaxf(__ldg(p.c.v_scale + (int64_t)id * p.c.Hkv + hk), kScaleFloor);
-            if (gi + kWarps < min(pc.g1, gp)) id_next = page_id(p.c, pc.b, ((gi + kWarps) * 16) >> p.c.page_shift);
-
-            float acc[2][4];
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[kt][e] = 0.f;
+                for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks) {
-                uint32_t a[4] = {0u, 0u, 0u, 0u};
-                if (TALL) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(s_q[ks][lane]);
-                    a[0] = x.x, a[1] = x.y, a[2] = x.z, a[3] = x.w;
-                } else {
-                    const uint2 x = *reinterpret_cast<const uint2*>(s_q[ks][lane]);
-                    a[0] = x.x, a[2] = x.y;
-                }
+                const uint4 x = kw[0][ks >> 2], y = kw[1][ks >> 2];
+                const uint32_t wx = (ks & 3) == 0 ? x.x : (ks & 3) == 1 ? x.y : (ks & 3) == 2 ? x.z : x.w;
+                const uint32_t wy = (ks & 3) == 0 ? y.x : (ks & 3) == 1 ? y.y : (ks & 3) == 2 ? y.z : y.w;
+                uint32_t a0, a1, a2, a3;
+                halves<FP8>(wx, a0, a2);
+                halves<FP8>(wy, a1, a3);
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt) {
-                    const uint4 r = kw[kt][ks >> 2];
-                    const uint32_t w = (ks & 3) == 0 ? r.x : (ks & 3) == 1 ? r.y : (ks & 3) == 2 ? r.z : r.w;
-                    uint32_t b0, b1;
-                    halves<FP8>(w, b0, b1);
-                    mma_f16(acc[kt], a[0], a[1], a[2], a[3], b0, b1);
+                for (int n = 0; n < NT; ++n) {
+                    const uint2 q = NT == 1 ? make_uint2(qb[ks][0], qb[ks][1]) : s_q[n][ks][lane];
+                    mma_f16(acc[n], a0, a1, a2, a3, q.x, q.y);
                 }
             }
-            const float lsv = __log2f(sv);
-            float w[2][2 * kHalves];
-            const bool tail = key0 + 16 > len;
+            const float skc = sk, svc = fmaxf(sv, kScaleFloor);
+            id = id_next;
+            if (more) {
+                load_k(gi + kWarps, id);
+                sk = __ldg(p.c.k_scale + (int64_t)id * p.c.Hkv + hk);
+                sv = __ldg(p.c.v_scale + (int64_t)id * p.c.Hkv + hk);
+                id_next = id_of(gi + 2 * kWarps);
+            }
+            const float lsv = __log2f(svc);
+            float w[NT][4];
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int h = 0; h < kHalves; ++h)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        w[kt][2 * h + e] = fmaf(acc[kt][2 * h + e], sk * rf[h], lsv);
-                        if (tail && key0 + 8 * kt + 2 * t + e >= len) w[kt][2 * h + e] = -INFINITY;
-                    }
+                for (int e = 0; e < 4; ++e) w[n][e] = fmaf(acc[n][e], skc * rf[n][e & 1], lsv);
             if (tail) {  // slots past the length hold any bits (an e4m3 NaN too): their weight is 0, their codes too
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (key0 + g + 8 * (e >> 1) >= len) w[n][e] = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (key0 + 2 * t + (i & 1) + 8 * (i >> 1) >= len) vw[i] = make_uint4(0u, 0u, 0u, 0u);
             }
-            step(w, __frcp_rn(sv));
-            uint32_t hi[2][kHalves], lo[2][kHalves];
+            step(w, __frcp_rn(svc));
+            uint32_t hi[NT][2], lo[NT][2];  // keys 0 .. 7 and 8 .. 15: B operands
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int h = 0; h < kHalves; ++h) split_bf16(pk2(w[kt][2 * h], w[kt][2 * h + 1]), hi[kt][h], lo[kt][h]);
+                for (int h = 0; h < 2; ++h) {
+                    split_half(w[n][2 * h], w[n][2 * h + 1], hi[n][h], lo[n][h]);
+                    hi[n][h] = transpose8(hi[n][h]);
+                    lo[n][h] = transpose8(lo[n][h]);
+                }
             const uint32_t v0[4] = {vw[0].x, vw[0].y, vw[0].z, vw[0].w}, v1[4] = {vw[1].x, vw[1].y, vw[1].z, vw[1].w};
             const uint32_t v2[4] = {vw[2].x, vw[2].y, vw[2].z, vw[2].w}, v3[4] = {vw[3].x, vw[3].y, vw[3].z, vw[3].w};
 #pragma unroll
-            for (int j4 = 0; j4 < 4; ++j4) {  // columns 16 g + 4 j4 .. + 3
-                uint32_t b0[4], b1[4];
-                bfloats<FP8>(__byte_perm(v0[j4], v1[j4], 0x5140), b0[0], b0[1]);
-                bfloats<FP8>(__byte_perm(v0[j4], v1[j4], 0x7362), b0[2], b0[3]);
-                bfloats<FP8>(__byte_perm(v2[j4], v3[j4], 0x5140), b1[0], b1[1]);
-                bfloats<FP8>(__byte_perm(v2[j4], v3[j4], 0x7362), b1[2], b1[3]);
+            for (int j2 = 0; j2 < 4; ++j2) {  // d = 16 g + 4 j2 .. + 3: two column tiles
+                uint32_t a[4], c[4];           // keys 2 t, 2 t + 1, then 2 t + 8, 2 t + 9, of the four d
+                halves<FP8>(__byte_perm(v0[j2], v1[j2], 0x5140), a[0], a[1]);
+                halves<FP8>(__byte_perm(v2[j2], v3[j2], 0x5140), c[0], c[1]);
+                halves<FP8>(__byte_perm(v0[j2], v1[j2], 0x7362), a[2], a[3]);
+                halves<FP8>(__byte_perm(v2[j2], v3[j2], 0x7362), c[2], c[3]);
 #pragma unroll
-                for (int u = 0; u < 4; ++u) values(o[4 * j4 + u], hi, lo, b0[u], b1[u]);
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        float(&d)[4] = o[n][2 * j2 + u];
+                        mma_f16(d, a[2 * u], a[2 * u + 1], c[2 * u], c[2 * u + 1], hi[n][0], hi[n][1]);
+                        mma_f16(d, a[2 * u], a[2 * u + 1], c[2 * u], c[2 * u + 1], lo[n][0], lo[n][1]);
+                    }
             }
+            if (more) load_v(gi + kWarps, id);
         }
 
         // ---- the nodes' own keys, in bf16
         const int g_own = min(pc.g1, gp + (p.nn + 15) / 16);
+#pragma unroll 1
         for (; gi < g_own; gi += kWarps) {
             const int j0 = (gi - gp) * 16;
             const __nv_bfloat16* kn = p.kn + (int64_t)pc.b * p.sn_b + (int64_t)hk * p.sn_h;
             const __nv_bfloat16* vn = p.vn + (int64_t)pc.b * p.sn_b + (int64_t)hk * p.sn_h;
-            float acc[2][4];
+            float acc[NT][4];
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[kt][e] = 0.f;
-                const int key = min(j0 + 8 * kt + g, p.nn - 1);  // past the end: the last key again, masked below
+                for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+            const __nv_bfloat16* k0 = kn + (int64_t)min(j0 + g, p.nn - 1) * p.sn_n;  // past the end: the last key
+            const __nv_bfloat16* k1 = kn + (int64_t)min(j0 + g + 8, p.nn - 1) * p.sn_n;  // again, masked below
+            const __nv_bfloat16* qr[NT];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int col = 16 * t + 8 * (i & 1) + 64 * (i >> 1);
-                    const uint4 kx = __ldg(reinterpret_cast<const uint4*>(kn + (int64_t)key * p.sn_n + col));
-                    const uint4 q0 = __ldg(reinterpret_cast<const uint4*>(qrow[0] + col));
-                    uint4 q1 = make_uint4(0u, 0u, 0u, 0u);
-                    if (TALL) q1 = __ldg(reinterpret_cast<const uint4*>(qrow[kHalves - 1] + col));
-                    mma_bf16(acc[kt], q0.x, q1.x, q0.y, q1.y, kx.x, kx.y);
-                    mma_bf16(acc[kt], q0.z, q1.z, q0.w, q1.w, kx.z, kx.w);
+            for (int n = 0; n < NT; ++n) {
+                const int r = min(base + 8 * n + g, p.rows - 1), nd = r / p.G;
+                qr[n] = p.q + (int64_t)pc.b * p.sq_b + (int64_t)nd * p.sq_n + (int64_t)(hk * p.G + r - nd * p.G) * p.sq_h;
+            }
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {
+                const int col = 16 * t + 8 * (i & 1) + 64 * (i >> 1);
+                const uint4 x = __ldg(reinterpret_cast<const uint4*>(k0 + col)), y = __ldg(reinterpret_cast<const uint4*>(k1 + col));
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const uint4 q = __ldg(reinterpret_cast<const uint4*>(qr[n] + col));
+                    mma_bf16(acc[n], x.x, y.x, x.y, y.y, q.x, q.y);
+                    mma_bf16(acc[n], x.z, y.z, x.w, y.w, q.z, q.w);
                 }
             }
-            uint32_t see[kHalves];  // bit i: this lane's row sees own key j0 + i
-            float w[2][2 * kHalves];
+            uint32_t see[NT][2];  // bit i: the lane's row sees own key j0 + i
+            float w[NT][4];
 #pragma unroll
-            for (int h = 0; h < kHalves; ++h) {
-                see[h] = node[h] >= 0 ? (uint32_t)(visible_word(p, pc.b, node[h], j0 >> 6) >> (j0 & 63)) & 0xffffu : 0u;
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        w[kt][2 * h + e] = (see[h] >> (8 * kt + 2 * t + e)) & 1u ? acc[kt][2 * h + e] * p.scale_log2
-                                                                                : -INFINITY;
-            }
+                for (int e = 0; e < 2; ++e) {
+                    const int r = base + 8 * n + 2 * t + e;
+                    see[n][e] = r < p.rows ? (uint32_t)(visible_word(p, pc.b, r / p.G, j0 >> 6) >> (j0 & 63)) & 0xffffu : 0u;
+                    w[n][e] = (see[n][e] >> g) & 1u ? acc[n][e] * p.scale_log2 : -INFINITY;
+                    w[n][2 + e] = (see[n][e] >> (g + 8)) & 1u ? acc[n][2 + e] * p.scale_log2 : -INFINITY;
+                }
             step(w, 1.f);
-            uint32_t hi[2][kHalves], lo[2][kHalves];
+            uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int h = 0; h < kHalves; ++h) split_bf16(pk2(w[kt][2 * h], w[kt][2 * h + 1]), hi[kt][h], lo[kt][h]);
+                for (int h = 0; h < 2; ++h) {
+                    split_bf16(pk2(w[n][2 * h], w[n][2 * h + 1]), hi[n][h], lo[n][h]);
+                    hi[n][h] = transpose8(hi[n][h]);
+                    lo[n][h] = transpose8(lo[n][h]);
+                }
             bool odd = false;  // a non-finite value among this group's
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {  // columns 16 g + 8 half .. + 7
+            for (int half = 0; half < 2; ++half) {  // d = 16 g + 8 half .. + 7
                 uint32_t x[4][4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -311,28 +345,31 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
                     }
                 }
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                for (int c = 0; c < 4; ++c) {
+                    const uint32_t a0 = __byte_perm(x[0][c], x[1][c], 0x5410), a1 = __byte_perm(x[0][c], x[1][c], 0x7632);
+                    const uint32_t a2 = __byte_perm(x[2][c], x[3][c], 0x5410), a3 = __byte_perm(x[2][c], x[3][c], 0x7632);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int j = 8 * half + 2 * c + e;
-                        const uint32_t sel = e ? 0x7632 : 0x5410;
-                        values(o[j], hi, lo, __byte_perm(x[0][c], x[1][c], sel), __byte_perm(x[2][c], x[3][c], sel));
+                    for (int n = 0; n < NT; ++n) {
+                        mma_bf16(o[n][4 * half + c], a0, a1, a2, a3, hi[n][0], hi[n][1]);
+                        mma_bf16(o[n][4 * half + c], a0, a1, a2, a3, lo[n][0], lo[n][1]);
                     }
+                }
             }
             if (__any_sync(MFD_FULL_MASK, odd)) {
                 // rare: add the infinities and NaNs to the rows that see their key (a weight is above 0, so their
-                // size does not matter): O[row][d] of this lane are d = 32 t + j and 32 t + 16 + j
+                // size does not matter)
+#pragma unroll 1
                 for (int i = 0; i < min(16, p.nn - j0); ++i) {
-                    const __nv_bfloat16* vrow = vn + (int64_t)(j0 + i) * p.sn_n + 32 * t;
+                    const __nv_bfloat16* vrow = vn + (int64_t)(j0 + i) * p.sn_n + 16 * g;
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                        const float y0 = __bfloat162float(vrow[j]), y1 = __bfloat162float(vrow[16 + j]);
+                        const float y = __bfloat162float(vrow[j]);
+                        if (fabsf(y) < INFINITY) continue;
 #pragma unroll
-                        for (int h = 0; h < kHalves; ++h) {
-                            if (!((see[h] >> i) & 1u)) continue;
-                            if (!(fabsf(y0) < INFINITY)) o[j][2 * h] += y0;
-                            if (!(fabsf(y1) < INFINITY)) o[j][2 * h + 1] += y1;
-                        }
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                if ((see[n][e] >> i) & 1u) o[n][j >> 1][2 * (j & 1) + e] += y;
                     }
                 }
             }
@@ -340,26 +377,28 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
 
         // ---- the warps of the piece merge
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-            l[h] = quad_sum(l[h]);
-            if (t == 0) s_m[warp][g + 8 * h] = m[h], s_l[warp][g + 8 * h] = l[h];
-        }
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                l[n][e] = column_sum(l[n][e]);
+                if (g == 0) s_m[warp][8 * n + 2 * t + e] = m[n][e], s_l[warp][8 * n + 2 * t + e] = l[n][e];
+            }
         __syncthreads();
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-            float mm = -INFINITY;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w][g + 8 * h]);
-            const float a = m[h] == -INFINITY ? 0.f : fast_exp2(m[h] - mm);
-            float* row = smem + (warp * kRows + g + 8 * h) * kRowStride + t * kTBlock;
+            for (int e = 0; e < 2; ++e) {
+                const int r = 8 * n + 2 * t + e;
+                float mm = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+                for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w][r]);
+                const float a = m[n][e] == -INFINITY ? 0.f : fast_exp2(m[n][e] - mm);
+                float* row = smem + (warp * kRows + r) * kRowStride + g * kDBlock;
 #pragma unroll
-                for (int j = 0; j < 16; j += 4)
-                    *reinterpret_cast<float4*>(row + 16 * e + j) =
-                        make_float4(o[j][2 * h + e] * a, o[j + 1][2 * h + e] * a, o[j + 2][2 * h + e] * a,
-                                    o[j + 3][2 * h + e] * a);
-        }
+                for (int j = 0; j < 8; j += 2)
+                    *reinterpret_cast<float4*>(row + 2 * j) = make_float4(o[n][j][e] * a, o[n][j][2 + e] * a,
+                                                                          o[n][j + 1][e] * a, o[n][j + 1][2 + e] * a);
+            }
         __syncthreads();
         const int live_rows = min(16, p.rows - base);
         const bool whole = pc.pieces == 1;
@@ -382,8 +421,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
             for (int w = 0; w < kWarps; ++w) {
                 const float mw = s_m[w][r];
                 ll += s_l[w][r] * (mw == -INFINITY ? 0.f : fast_exp2(mw - mm));  // (a NaN sum stays one)
-                const float4 x = *reinterpret_cast<const float4*>(smem + (w * kRows + r) * kRowStride + (c4 >> 3) * kTBlock +
-                                                                  (c4 & 7) * 4);
+                const float4 x = *reinterpret_cast<const float4*>(smem + (w * kRows + r) * kRowStride + (c4 >> 2) * kDBlock +
+                                                                  (c4 & 3) * 4);
                 v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
             }
             if (whole) {
@@ -455,25 +494,25 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
 int64_t rows_tickets(int64_t bs, int64_t hkv, int64_t rows) { return bs * hkv * ((rows + 15) / 16); }
 size_t rows_workspace(int sms) { return (size_t)sms * kCtasPerSm * 2 * kSlot * sizeof(float); }
 
-template <bool FP8, bool TALL>
+template <bool FP8, int NT>
 static int launch_one(const AttnParams& p, int sms, cudaStream_t stream) {
-    constexpr int kSmem = kWarps * (TALL ? 16 : 8) * kRowStride * 4;
+    constexpr int kSmem = kWarps * 8 * NT * kRowStride * 4;
     static_assert(kSmem >= 512 * 16 * 4, "the merge weights fit");
     static bool opted[64];
-    cudaError_t e = opt_in_smem((const void*)kv8_rows_kernel<FP8, TALL>, kSmem, opted);
+    cudaError_t e = opt_in_smem((const void*)kv8_rows_kernel<FP8, NT>, kSmem, opted);
     if (e != cudaSuccess) {
         set_error("mfd_kv8_attention: %s", cudaGetErrorString(e));
         return MFD_ERR_CUDA;
     }
-    kv8_rows_kernel<FP8, TALL><<<sms * kCtasPerSm, kThreads, kSmem, stream>>>(p);
+    kv8_rows_kernel<FP8, NT><<<sms * kCtasPerSm, kThreads, kSmem, stream>>>(p);
     MFD_CHECK_LAUNCH("mfd_kv8_attention");
     return MFD_OK;
 }
 
 int launch_rows(const AttnParams& p, int sms, cudaStream_t stream) {
     const bool tall = p.rows - p.row0 > 8;
-    if (p.fp8) return tall ? launch_one<true, true>(p, sms, stream) : launch_one<true, false>(p, sms, stream);
-    return tall ? launch_one<false, true>(p, sms, stream) : launch_one<false, false>(p, sms, stream);
+    if (p.fp8) return tall ? launch_one<true, 2>(p, sms, stream) : launch_one<true, 1>(p, sms, stream);
+    return tall ? launch_one<false, 2>(p, sms, stream) : launch_one<false, 1>(p, sms, stream);
 }
 
 }  // namespace kv8
