@@ -1,6 +1,38 @@
 // kv8_attention.cu -- C entry point of the attention over the 8-bit paged cache: checks, and which kernel takes the
 // rows.
+#include <cudaTypedefs.h>
+
 #include "kv8_attention.cuh"
+
+namespace mfd {
+namespace kv8 {
+
+static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    if (!fn) {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = (PFN_cuTensorMapEncodeTiled_v12000)ptr;
+    }
+    return fn;
+}
+
+bool make_page_map(CUtensorMap* m, const uint8_t* base, const Cache& c, bool swizzle) {
+    auto fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)kD, (cuuint64_t)c.page, (cuuint64_t)c.Hkv, (cuuint64_t)c.num_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)c.sc_t, (cuuint64_t)c.sc_h, (cuuint64_t)c.sc_p};
+    const cuuint32_t box[4] = {(cuuint32_t)kD, (cuuint32_t)c.page, 1, 1};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace kv8
+}  // namespace mfd
 
 using namespace mfd;
 

@@ -1,6 +1,8 @@
 // kv8_attention.cuh -- parameters shared by the attention kernels over the 8-bit paged cache and their C entry point.
 #pragma once
 
+#include <cuda.h>
+
 #include "kv8.cuh"
 
 namespace mfd {
@@ -27,6 +29,20 @@ struct AttnParams {
     unsigned int* tickets;
     int* status;
 };
+
+// TMA map of a cache tensor's codes: (128, page, KV heads, pages), one page of one head a box (swizzle: 128-byte)
+bool make_page_map(CUtensorMap* m, const uint8_t* base, const Cache& c, bool swizzle);
+__device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int head, int page) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
+        "%5}], [%6];" ::"r"(dst),
+        "l"(map), "r"(0), "r"(0), "r"(head), "r"(page), "r"(smem_addr(bar))
+        : "memory");
+}
+template <int N>
+__device__ __forceinline__ void bar_sync(int id) {
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
+}
 
 // rows [p.row0, p.rows) with the register kernel (16 rows a unit)
 int launch_rows(const AttnParams& p, int sms, cudaStream_t stream);

@@ -10,22 +10,25 @@
 // keys and values take bf16 operands, the weights hi + lo as well.  All sums and statistics are float32.
 //
 // Bound: bytes (256 codes a token and KV head for 4 G n multiply-adds each); next, instructions: turning the codes into
-// operands.  So the codes go from memory straight to registers, 16 bytes a lane, in a layout in which they are the
-// wide operand of the tensor instruction and the query rows, which are few, the narrow one:
-//   scores   m16n8k16: A = 16 keys, B = 8 query rows; the d index is permuted (lane (g, t) holds d = 16 t .. 16 t + 15 of
-//            either half row of keys g and g + 8, the query alike), so a lane's operand registers are its bytes in order
+// operands.  The codes are the wide operand of the tensor instruction and the query rows, which are few, the narrow one,
+// in a layout in which a lane's operand registers are its bytes in order:
+//   scores   m16n8k16: A = 16 keys, B = 8 query rows; the d index is permuted (lane (g, t) holds d = 32 t .. 32 t + 31 of
+//            keys g and g + 8, the query alike)
 //   values   m16n8k16: A = 16 columns of the values x 16 keys, B = the weights (the scores' registers transposed by
-//            movmatrix); lane (g, t) loads d = 16 g .. 16 g + 15 of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 and interleaves
+//            movmatrix); lane (g, t) holds d = 16 g .. 16 g + 15 of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 and interleaves
 //            the bytes of two keys before they become float16 pairs; column tile j is d = 16 g + 2 j and the next
-// A warp takes 16 keys at a time (one page has all 16: one scale).  The next group's K loads are issued when the scores
-// have consumed this one's registers, its V loads when the products have, so a load has most of a group's time to
-// arrive without a second set of registers.  The 8 warps of a CTA take every eighth group with their own (m, l, O) and
-// merge in shared memory at the end of the piece.
+// Tiles of 128 keys come by TMA, a page a copy, into a ring of three 32 KB stages (two CTAs an SM: 192 KB in flight; loads
+// straight to registers kept too few bytes in flight and reached half the bandwidth).  The 128-byte swizzle of the copies
+// makes both register layouts' 16-byte shared-memory loads free of bank conflicts.  Warp 0 issues the copies of the tile two
+// ahead (a ninth warp would cost every thread a quarter of its registers).  The 8 warps take 16 keys of every tile each
+// (one page has all 16: one scale), with their own (m, l, O), and merge in shared memory at the end of the piece.
 //
-// Split: the groups of all (request, KV head, 16 rows) units are laid end to end and cut into equal pieces, one per
-// CTA (two CTAs an SM), so ragged lengths balance and one long request fills the GPU; the lengths are read on the
-// device.  A unit cut into pieces is merged by the CTA that finishes last (its partial (m, l, O) in the workspace, a
-// ticket per unit; the pieces are added in their order, so the result does not depend on who merges).
+// Split: the tiles of all (request, KV head, 16 rows) units are laid end to end and cut into equal pieces, one per CTA, so
+// ragged lengths balance and one long request fills the GPU; the lengths are read on the device.  The nodes' own keys
+// belong to a unit's last piece.  A unit cut into pieces is merged by the CTA that finishes last (its partial (m, l, O) in
+// the workspace, a ticket per unit; the pieces are added in their order, so the result does not depend on who merges).
+//
+// Every mbarrier wait is bounded; a CTA whose wait gave up records status 1 and stops.
 #include "kv8_attention.cuh"
 #include "tcgen05.cuh"
 
@@ -34,6 +37,10 @@ namespace kv8 {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
+constexpr int kTile = 128;             // keys a stage
+constexpr int kStages = 3;
+constexpr int kStageBytes = 2 * kTile * kD;  // K, then V
+constexpr uint32_t kTries = 1u << 20;
 // floats: a lane's 16 columns, padded so that the 8 lanes of a store hit different banks
 constexpr int kDBlock = 20, kRowStride = 8 * kDBlock + 4;
 constexpr int kSlot = 16 * (kD + 2);  // floats of a partial: m[16], l[16], O[16][128]
@@ -47,63 +54,88 @@ __device__ __forceinline__ bool not_finite_pair(uint32_t w) {  // a bf16 pair ho
 
 // NT: 8-row tiles a unit
 template <bool FP8, int NT>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+    kv8_rows_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const AttnParams p) {
     constexpr int kRows = 8 * NT;
-    extern __shared__ __align__(16) float smem[];  // [kWarps][kRows][kRowStride]; merge weights
+    // the ring; at a piece's end [kWarps][kRows][kRowStride] floats, then the merge weights
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    unsigned char* ring = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+    float* smem = reinterpret_cast<float*>(ring);
+    __shared__ float4 s_const[kStages][kWarps];  // of 16 keys: K scale, log2 and reciprocal of the V scale
     __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
-    __shared__ uint2 s_q[NT == 1 ? 1 : NT][8][32];  // query operands, where two tiles of them would not fit the registers
-    __shared__ int s_last;
+    __shared__ uint2 s_q[NT][8][32];  // query operands, the same for every warp (in registers they would spill)
+    __shared__ uint64_t s_full[kStages], s_empty[kStages];
+    __shared__ int s_last, s_failed;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
+    if (tid == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&s_full[i], 32);
+            mbar_init(&s_empty[i], kWarps);
+        }
+        s_failed = 0;
+        mbar_fence_init();
+    }
     const int nrows = p.rows - p.row0;
     const int RB = (nrows + 15) / 16;
-    // ---- this CTA's share of the work, in groups of 16 keys (cached tokens, then own keys)
-    auto groups_of = [&](int len) { return max(1, (len + 15) / 16 + (p.nn + 15) / 16); };  // (one, to write zeros)
+    // ---- this CTA's share of the work, in tiles
+    auto tiles_of = [](int len) { return max(1, (len + kTile - 1) / kTile); };  // (one, for the own keys or to write zeros)
     const Lengths lens(p.c, p.bs);
-    const Cut cut = make_cut(lens, groups_of, p.c.Hkv * RB, gridDim.x, kWarps);
+    const Cut cut = make_cut(lens, tiles_of, p.c.Hkv * RB, gridDim.x, 1);
     int64_t pos, end;
     cut_range(cut, blockIdx.x, pos, end);
+    __syncthreads();
 
     Piece pc;
-    while (next_piece(lens, groups_of, cut, blockIdx.x, pos, end, pc)) {
+    uint32_t n_tile = 0;  // tiles of the CTA's earlier pieces: the barriers' phases
+    bool ok = true;
+    while (next_piece(lens, tiles_of, cut, blockIdx.x, pos, end, pc)) {
         const int hk = pc.u / RB, rb = pc.u % RB, len = pc.len;
-        const int gp = (len + 15) / 16;  // groups of cached tokens; own keys follow
         const int base = p.row0 + rb * 16;
-        const int g_cached = min(pc.g1, gp);
 
-        // ---- the first group's codes, before anything waits
-        const uint8_t* kbase = p.c.k + (int64_t)hk * p.c.sc_h + (int64_t)g * p.c.sc_t + 16 * t;
-        const uint8_t* vbase = p.c.v + (int64_t)hk * p.c.sc_h + (int64_t)(2 * t) * p.c.sc_t + 16 * g;
-        const int slot_mask = p.c.page - 1;
-        uint4 kw[2][2], vw[4];  // K: key g, g + 8; d half.  V: keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+        // ---- the producer, warp 0: tile `next`'s copies and constants.  Page ids are read two tiles ahead and scales
+        // one, so it waits for neither; a stage is free once every warp has read its codes, two tiles before.
+        const int ppt = kTile >> p.c.page_shift, gpp = p.c.page >> 4;
+        int next = pc.g0, id0, id1;
         float sk = 0.f, sv = 1.f;
-        auto offset = [&](int gi, int id) {
-            return (int64_t)id * p.c.sc_p + (int64_t)((gi * 16) & slot_mask) * p.c.sc_t;
+        auto id_of = [&](int tile) {  // lane j < ppt takes page j of a tile
+            const int pg = tile * ppt + lane;
+            return lane < ppt && tile < pc.g1 && (pg << p.c.page_shift) < len ? page_id(p.c, pc.b, pg) : -1;
         };
-        auto load_k = [&](int gi, int id) {
-            const uint8_t* src = kbase + offset(gi, id);
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) kw[h][i] = ldg_stream_u4(src + (int64_t)(8 * h) * p.c.sc_t + 64 * i);
-        };
-        auto load_v = [&](int gi, int id) {
-            const uint8_t* src = vbase + offset(gi, id);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) vw[i] = ldg_stream_u4(src + (int64_t)((i & 1) + 8 * (i >> 1)) * p.c.sc_t);
-        };
-        auto id_of = [&](int gi) { return gi < g_cached ? page_id(p.c, pc.b, (gi * 16) >> p.c.page_shift) : 0; };
-        int gi = pc.g0 + warp;
-        int id = id_of(gi), id_next = id_of(gi + kWarps);
-        if (gi < g_cached) {
-            load_k(gi, id);
-            load_v(gi, id);
+        auto scales = [&](int id) {
+            if (id < 0) return;
             sk = __ldg(p.c.k_scale + (int64_t)id * p.c.Hkv + hk);
             sv = __ldg(p.c.v_scale + (int64_t)id * p.c.Hkv + hk);
+        };
+        auto produce = [&]() {
+            const uint32_t nt = n_tile + next - pc.g0, st = nt % kStages;
+            if (nt >= (uint32_t)kStages)
+                ok = __all_sync(MFD_FULL_MASK, ok & mbar_wait(&s_empty[st], (nt / kStages - 1) & 1, kTries));
+            if (!ok) return;
+            if (id0 >= 0) {
+                const uint32_t half = (uint32_t)(p.c.page * kD), dst = smem_addr(ring) + st * kStageBytes + lane * half;
+                mbar_expect_tx(&s_full[st], 2 * half);
+                tma_page(dst, &tmk, &s_full[st], hk, id0);
+                tma_page(dst + kStageBytes / 2, &tmv, &s_full[st], hk, id0);
+                const float s = fmaxf(sv, kScaleFloor);
+                const float4 k = make_float4(sk, __log2f(s), __frcp_rn(s), 0.f);
+                for (int i = 0; i < gpp; ++i) s_const[st][lane * gpp + i] = k;
+            }
+            __syncwarp();  // lanes without a page (8 .. 31 never have one) arrive last, after every constant is stored
+            if (id0 < 0) mbar_arrive(&s_full[st]);
+            ++next;
+            id0 = id1;
+            scales(id0);
+            id1 = id_of(next + 1);
+        };
+        if (warp == 0) {
+            id0 = id_of(next);
+            id1 = id_of(next + 1);
+            scales(id0);
+            for (int i = 0; i < kStages - 1 && next < pc.g1; ++i) produce();
         }
 
         // ---- query row g (+ 8 nt) as float16 operands, divided by a power of two; the lane's softmax rows are 2 t, 2 t + 1
-        uint32_t qb[8][2];
         float rf[NT][2];  // score factor of rows 2 t and 2 t + 1: the power of two, the scale and log2(e)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -113,9 +145,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
             const __nv_bfloat16* qrow = p.q + (int64_t)pc.b * p.sq_b + (int64_t)nd * p.sq_n + (int64_t)hd * p.sq_h;
             uint4 x[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {  // columns 16 t + 8 (i & 1) + 64 (i >> 1) ..
+            for (int i = 0; i < 4; ++i) {  // columns 32 t + 8 i ..
                 x[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (live) x[i] = __ldg(reinterpret_cast<const uint4*>(qrow + 16 * t + 8 * (i & 1) + 64 * (i >> 1)));
+                if (live) x[i] = __ldg(reinterpret_cast<const uint4*>(qrow + 32 * t + 8 * i));
             }
             float mx = 0.f;
 #pragma unroll
@@ -138,15 +170,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const float2 f0 = bf2(w[2 * j]), f1 = bf2(w[2 * j + 1]);
-                    const int ks = 4 * (i >> 1) + 2 * (i & 1) + j;
-                    const uint32_t b0 = pack_half2(f0.x * down, f0.y * down), b1 = pack_half2(f1.x * down, f1.y * down);
-                    if (NT == 1) qb[ks][0] = b0, qb[ks][1] = b1;
-                    else if (warp == 0) s_q[n][ks][lane] = make_uint2(b0, b1);
+                    const int ks = 2 * i + j;
+                    if (warp == 0)
+                        s_q[n][ks][lane] = make_uint2(pack_half2(f0.x * down, f0.y * down), pack_half2(f1.x * down, f1.y * down));
                 }
             }
         }
 
-        if (NT > 1) __syncthreads();
+        __syncthreads();
 
         // O of rows 2 t, 2 t + 1 (+ 8 n): o[n][j] = d 16 g + 2 j (both rows), then the next d (both rows)
         float o[NT][8][4];
@@ -198,14 +229,33 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
         };
 
         // ---- cached tokens
-        for (; gi < g_cached; gi += kWarps) {
-            const int key0 = gi * 16;
-            const bool tail = key0 + 16 > len, more = gi + kWarps < g_cached;
-            float acc[NT][4];
+        const uint32_t swk = (uint32_t)(g & 7) << 4;
+#pragma unroll 1
+        for (int tile = pc.g0; tile < pc.g1; ++tile) {
+            if (warp == 0 && next < pc.g1) produce();
+            const uint32_t nt = n_tile + tile - pc.g0, st = nt % kStages;
+            ok = __all_sync(MFD_FULL_MASK, ok & mbar_wait(&s_full[st], (nt / kStages) & 1, kTries));
+            if (!ok) break;
+            const int key0 = tile * kTile + 16 * warp;
+            if (key0 >= len) {  // (a tile's last warps, behind the request's end)
+                if (lane == 0) mbar_arrive(&s_empty[st]);
+                continue;
+            }
+            const bool tail = key0 + 16 > len;
+            const unsigned char* kt = ring + st * kStageBytes + (16 * warp + g) * kD;  // key g's row; g + 8: 1 KB on
+            const unsigned char* vt = ring + st * kStageBytes + kStageBytes / 2 + (16 * warp + 2 * t) * kD;
+            uint4 kw[2][2], vw[4];  // K: key g, g + 8; chunk 2 t, 2 t + 1.  V: keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    kw[h][i] = *reinterpret_cast<const uint4*>(kt + h * 8 * kD + (((uint32_t)(2 * t + i) << 4) ^ swk));
+            const float4 cst = s_const[st][warp];
+            float acc[NT][4], acc2[NT][4];  // two chains: the instruction's latency is several times its issue
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+                for (int e = 0; e < 4; ++e) acc[n][e] = acc2[n][e] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks) {
                 const uint4 x = kw[0][ks >> 2], y = kw[1][ks >> 2];
@@ -216,24 +266,20 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
                 halves<FP8>(wy, a1, a3);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const uint2 q = NT == 1 ? make_uint2(qb[ks][0], qb[ks][1]) : s_q[n][ks][lane];
-                    mma_f16(acc[n], a0, a1, a2, a3, q.x, q.y);
+                    const uint2 q = s_q[n][ks][lane];
+                    mma_f16((ks & 1) ? acc2[n] : acc[n], a0, a1, a2, a3, q.x, q.y);
                 }
             }
-            const float skc = sk, svc = fmaxf(sv, kScaleFloor);
-            id = id_next;
-            if (more) {
-                load_k(gi + kWarps, id);
-                sk = __ldg(p.c.k_scale + (int64_t)id * p.c.Hkv + hk);
-                sv = __ldg(p.c.v_scale + (int64_t)id * p.c.Hkv + hk);
-                id_next = id_of(gi + 2 * kWarps);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = 2 * t + (i & 1);
+                vw[i] = *reinterpret_cast<const uint4*>(vt + ((i & 1) + 8 * (i >> 1)) * kD + ((uint32_t)(g ^ r) << 4));
             }
-            const float lsv = __log2f(svc);
             float w[NT][4];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[n][e] = fmaf(acc[n][e], skc * rf[n][e & 1], lsv);
+                for (int e = 0; e < 4; ++e) w[n][e] = fmaf(acc[n][e] + acc2[n][e], cst.x * rf[n][e & 1], cst.y);
             if (tail) {  // slots past the length hold any bits (an e4m3 NaN too): their weight is 0, their codes too
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
@@ -244,7 +290,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
                 for (int i = 0; i < 4; ++i)
                     if (key0 + 2 * t + (i & 1) + 8 * (i >> 1) >= len) vw[i] = make_uint4(0u, 0u, 0u, 0u);
             }
-            step(w, __frcp_rn(svc));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_empty[st]);  // every lane has its codes
+            step(w, cst.z);
             uint32_t hi[NT][2], lo[NT][2];  // keys 0 .. 7 and 8 .. 15: B operands
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -264,22 +312,21 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
                 halves<FP8>(__byte_perm(v0[j2], v1[j2], 0x7362), a[2], a[3]);
                 halves<FP8>(__byte_perm(v2[j2], v3[j2], 0x7362), c[2], c[3]);
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int part = 0; part < 2; ++part)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        float(&d)[4] = o[n][2 * j2 + u];
-                        mma_f16(d, a[2 * u], a[2 * u + 1], c[2 * u], c[2 * u + 1], hi[n][0], hi[n][1]);
-                        mma_f16(d, a[2 * u], a[2 * u + 1], c[2 * u], c[2 * u + 1], lo[n][0], lo[n][1]);
-                    }
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            mma_f16(o[n][2 * j2 + u], a[2 * u], a[2 * u + 1], c[2 * u], c[2 * u + 1],
+                                    part ? lo[n][0] : hi[n][0], part ? lo[n][1] : hi[n][1]);
             }
-            if (more) load_v(gi + kWarps, id);
         }
 
         // ---- the nodes' own keys, in bf16
-        const int g_own = min(pc.g1, gp + (p.nn + 15) / 16);
+        const int g_own = pc.g1 == pc.of ? (p.nn + 15) / 16 : 0;  // of a unit's last piece
 #pragma unroll 1
-        for (; gi < g_own; gi += kWarps) {
-            const int j0 = (gi - gp) * 16;
+        for (int gi = warp; gi < g_own; gi += kWarps) {
+            const int j0 = gi * 16;
             const __nv_bfloat16* kn = p.kn + (int64_t)pc.b * p.sn_b + (int64_t)hk * p.sn_h;
             const __nv_bfloat16* vn = p.vn + (int64_t)pc.b * p.sn_b + (int64_t)hk * p.sn_h;
             float acc[NT][4];
@@ -297,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
             }
 #pragma unroll 1
             for (int i = 0; i < 4; ++i) {
-                const int col = 16 * t + 8 * (i & 1) + 64 * (i >> 1);
+                const int col = 32 * t + 8 * i;
                 const uint4 x = __ldg(reinterpret_cast<const uint4*>(k0 + col)), y = __ldg(reinterpret_cast<const uint4*>(k1 + col));
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
@@ -487,7 +534,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_rows_kernel(const At
                 if (tid == 0) *ticket = 0u;
             }
         }
+        fence_proxy_async_smem();  // (the next piece's copies land where the merge was)
+        n_tile += pc.g1 - pc.g0;
+        if (!ok) atomicExch(&s_failed, 1);
         __syncthreads();  // smem, s_m and s_l are free for the next piece
+        if (*(volatile int*)&s_failed) {
+            if (tid == 0) atomicExch(p.status, 1);
+            break;
+        }
     }
 }
 
@@ -496,15 +550,21 @@ size_t rows_workspace(int sms) { return (size_t)sms * kCtasPerSm * 2 * kSlot * s
 
 template <bool FP8, int NT>
 static int launch_one(const AttnParams& p, int sms, cudaStream_t stream) {
-    constexpr int kSmem = kWarps * 8 * NT * kRowStride * 4;
-    static_assert(kSmem >= 512 * 16 * 4, "the merge weights fit");
+    constexpr int kSmem = kStages * kStageBytes + 1024;
+    static_assert(kWarps * 8 * NT * kRowStride * 4 <= kStages * kStageBytes && 512 * 16 * 4 <= kStages * kStageBytes,
+                  "the merge fits the ring");
+    CUtensorMap tk, tv;
+    if (!make_page_map(&tk, p.c.k, p.c, true) || !make_page_map(&tv, p.c.v, p.c, true)) {
+        set_error("mfd_kv8_attention: could not encode the TMA tensor maps");
+        return MFD_ERR_CUDA;
+    }
     static bool opted[64];
     cudaError_t e = opt_in_smem((const void*)kv8_rows_kernel<FP8, NT>, kSmem, opted);
     if (e != cudaSuccess) {
         set_error("mfd_kv8_attention: %s", cudaGetErrorString(e));
         return MFD_ERR_CUDA;
     }
-    kv8_rows_kernel<FP8, NT><<<sms * kCtasPerSm, kThreads, kSmem, stream>>>(p);
+    kv8_rows_kernel<FP8, NT><<<sms * kCtasPerSm, kThreads, kSmem, stream>>>(tk, tv, p);
     MFD_CHECK_LAUNCH("mfd_kv8_attention");
     return MFD_OK;
 }

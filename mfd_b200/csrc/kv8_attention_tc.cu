@@ -32,9 +32,6 @@
 // over the GPU (one CTA reading all pieces of 256 rows would take longer than the attention at batch 1).
 //
 // Every mbarrier wait is bounded; a CTA whose wait gave up records status 1, stops and releases its TMEM.
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
 #include "kv8_attention.cuh"
 #include "tcgen05.cuh"
 
@@ -84,14 +81,6 @@ constexpr int kSlotRows(bool pair) { return pair ? 256 : 128; }
 // floats of a partial: m, l per row, then O as float4 chunks, chunk-major (a warp stores 512 contiguous bytes)
 constexpr int64_t kSlotFloats(bool pair) { return (int64_t)kSlotRows(pair) * (2 + kD); }
 
-__device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int head, int page) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
-        "%5}], [%6];" ::"r"(dst),
-        "l"(map), "r"(0), "r"(0), "r"(head), "r"(page), "r"(smem_addr(bar))
-        : "memory");
-}
-
 // What a piece's tiles are (of 128 keys: cached tokens first, then the nodes' own).
 struct Tiles {
     int hk, rb;       // KV head, block of rows
@@ -102,11 +91,6 @@ struct Tiles {
     int nsteps;
     uint32_t n_piece, n_tile, n_s0, n_s1;  // pieces, tiles and the groups' steps before
 };
-
-template <int N>
-__device__ __forceinline__ void bar_sync(int id) {
-    asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
-}
 
 template <bool FP8, bool PAIR>
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -639,35 +623,10 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(const AttnParams p, in
         p.lse[((int64_t)pc.b * p.n + node) * p.H + head] = ll == 0.f ? -INFINITY : 0.6931471805599453f * (mm + log2f(ll));
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-    if (!fn) {
-        void* ptr = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = (PFN_cuTensorMapEncodeTiled_v12000)ptr;
-    }
-    return fn;
-}
-
-// codes as (128, page, KV heads, pages); one page of one head a box, unswizzled (the converters read plain rows)
-bool make_map(CUtensorMap* m, const uint8_t* base, const Cache& c) {
-    auto fn = encode_fn();
-    if (!fn) return false;
-    const cuuint64_t dims[4] = {(cuuint64_t)kD, (cuuint64_t)c.page, (cuuint64_t)c.Hkv, (cuuint64_t)c.num_pages};
-    const cuuint64_t strides[3] = {(cuuint64_t)c.sc_t, (cuuint64_t)c.sc_h, (cuuint64_t)c.sc_p};
-    const cuuint32_t box[4] = {(cuuint32_t)kD, (cuuint32_t)c.page, 1, 1};
-    const cuuint32_t estr[4] = {1, 1, 1, 1};
-    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t*>(base), dims, strides, box, estr,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <bool FP8, bool PAIR>
 int launch_tc_one(const AttnParams& p, int sms, cudaStream_t stream) {
     CUtensorMap tk, tv;
-    if (!make_map(&tk, p.c.k, p.c) || !make_map(&tv, p.c.v, p.c)) {
+    if (!make_page_map(&tk, p.c.k, p.c, false) || !make_page_map(&tv, p.c.v, p.c, false)) {
         set_error("mfd_kv8_attention: could not encode the TMA tensor maps");
         return MFD_ERR_CUDA;
     }
