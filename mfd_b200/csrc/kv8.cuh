@@ -170,20 +170,17 @@ __device__ __forceinline__ int listed_rows(const int64_t* path, int64_t path_str
 }
 
 // a / b for a >= 0, b > 0.  Small ones (all but extreme cases) by a reciprocal estimate, within one of the quotient, and
-// its correction: a few instructions where the 64-bit division takes hundreds of cycles at every CTA's start.
-__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
-    if (((uint64_t)(a | b) >> 22) == 0) {
-        const int x = (int)a, y = (int)b;
-        int q = __float2int_rz(__fdividef((float)x, (float)y));
-        const int r = x - q * y;
-        q += r >= y ? 1 : (r < 0 ? -1 : 0);
-        return q;
-    }
-    return a / b;
+// its correction: every CTA starts with a few of these, one after another.
+__device__ __forceinline__ int quotient(int a, int b) {
+    if (((uint32_t)(a | b) >> 22) != 0) return (int)((uint32_t)a / (uint32_t)b);
+    int q = __float2int_rz(__fdividef((float)a, (float)b));
+    const int r = a - q * b;
+    q += r >= b ? 1 : (r < 0 ? -1 : 0);
+    return q;
 }
 
-// Work laid end to end over the requests, f(length) * mul of it for each; every warp finds its place by itself.  The
-// lengths of the first 32 requests stay in the lanes' registers.
+// Work laid end to end over the requests, f(length) * mul of it for each (below 2^31 in all: the entry points check);
+// every warp finds its place by itself.  The lengths of the first 32 requests stay in the lanes' registers.
 struct Lengths {
     const Cache& c;
     int bs, mine;
@@ -192,34 +189,35 @@ struct Lengths {
         mine = lane < bs ? seq_len(c, lane) : 0;
     }
     template <class F>
-    __device__ __forceinline__ uint32_t part(int b0, F f, int& len) const {
+    __device__ __forceinline__ int part(int b0, F f, int& len) const {
         const int b = b0 + (threadIdx.x & 31);
         len = b0 == 0 ? mine : (b < bs ? seq_len(c, b) : 0);
-        return b < bs ? (uint32_t)f(len) : 0u;
+        return b < bs ? f(len) : 0;
     }
-    // the sum over all requests, or over those before `upto`
+    // the sum over all requests
     template <class F>
-    __device__ __forceinline__ int64_t sum(F f, int upto) const {
-        int64_t total = 0;
-        for (int b0 = 0; b0 < upto; b0 += 32) {
+    __device__ __forceinline__ int sum(F f) const {
+        int total = 0;
+        for (int b0 = 0; b0 < bs; b0 += 32) {
             int len;
-            const uint32_t v = part(b0, f, len);
-            total += __reduce_add_sync(MFD_FULL_MASK, b0 + (int)(threadIdx.x & 31) < upto ? v : 0u);
+            total += __reduce_add_sync(MFD_FULL_MASK, part(b0, f, len));
         }
         return total;
     }
     // the request whose range [before, before + f * mul) contains x, its length and before; -1 behind the last
     template <class F>
-    __device__ __forceinline__ int find(int64_t x, int64_t mul, F f, int64_t& before, int& len) const {
+    __device__ __forceinline__ int find(int x, int mul, F f, int& before, int& len) const {
         const int lane = threadIdx.x & 31;
-        int64_t base = 0;
+        int base = 0;
         for (int b0 = 0; b0 < bs; b0 += 32) {
-            const uint32_t v = part(b0, f, len);
-            uint32_t inc = v;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const uint32_t o = __shfl_up_sync(MFD_FULL_MASK, inc, d);
-                if (lane >= d) inc += o;
+            const int v = part(b0, f, len);
+            int inc = v;
+            if (bs > 1) {
+#pragma unroll 1
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int o = __shfl_up_sync(MFD_FULL_MASK, inc, d);
+                    if (lane >= d) inc += o;
+                }
             }
             const uint32_t hit = __ballot_sync(MFD_FULL_MASK, (base + inc) * mul > x);
             if (hit) {
@@ -237,31 +235,28 @@ struct Lengths {
 // How the units' work is cut over `ctas` CTAs: few units (split) into pieces of `per`, at most one piece a CTA;
 // otherwise equal ranges of `per` end to end, which may begin and end inside a unit.
 struct Cut {
-    int64_t total, per;
+    int total, per;
     int per_req;  // units per request
     bool split;
 };
 template <class F>
-__device__ __forceinline__ Cut make_cut(const Lengths& lens, F f, int per_req, int ctas, int least) {
+__device__ __forceinline__ Cut make_cut(const Lengths& lens, F f, int per_req, int ctas) {
     Cut w;
     w.per_req = per_req;
-    const int64_t units = (int64_t)lens.bs * per_req;
-    w.total = lens.sum(f, lens.bs) * per_req;
-    w.split = units * 2 <= (int64_t)ctas;
-    w.per = quotient(w.total + ctas - 1, ctas);
-    if (w.per < least) w.per = least;
+    w.total = lens.sum(f) * per_req;
+    w.split = lens.bs * per_req <= ctas / 2;
+    w.per = max(1, quotient(w.total + ctas - 1, ctas));
     if (w.split) {
-        // the smallest piece (nearly: 1/16 steps) of which there are at most ctas; total / (ctas - units) always is one
-        w.per = quotient(w.per + least - 1, least) * least;
-        const int64_t step = max((int64_t)least, quotient(w.per, 16 * least) * least);
-        while (lens.sum([&](int len) { return quotient(f(len) + w.per - 1, w.per); }, lens.bs) * per_req > ctas) w.per += step;
+        // the smallest piece (nearly: 1/16 steps) of which there are at most ctas
+        const int step = max(1, w.per >> 4);
+        while (lens.sum([&](int len) { return quotient(f(len) + w.per - 1, w.per); }) * per_req > ctas) w.per += step;
     }
     return w;
 }
 // [begin, end) of CTA `cta`: a range of the work, or (split) a piece's number
-__device__ __forceinline__ void cut_range(const Cut& w, int cta, int64_t& begin, int64_t& end) {
-    begin = w.split ? cta : (int64_t)cta * w.per;
-    end = w.split ? begin + 1 : min(w.total, begin + w.per);
+__device__ __forceinline__ void cut_range(const Cut& w, int cta, int& begin, int& end) {
+    begin = w.split ? cta : (int)min((int64_t)cta * w.per, (int64_t)w.total);
+    end = w.split ? begin + 1 : (int)min((int64_t)w.total, (int64_t)begin + w.per);
 }
 
 struct Piece {
@@ -275,22 +270,21 @@ struct Piece {
 };
 // the next piece of CTA `cta` at `pos` (moved on); false at the end
 template <class F>
-__device__ __forceinline__ bool next_piece(const Lengths& lens, F f, const Cut& w, int cta, int64_t& pos, int64_t end,
-                                           Piece& pc) {
+__device__ __forceinline__ bool next_piece(const Lengths& lens, F f, const Cut& w, int cta, int& pos, int end, Piece& pc) {
     if (pos >= end) return false;
-    int64_t before;
+    int before;
     if (w.split) {
         auto pieces_of = [&](int len) { return quotient(f(len) + w.per - 1, w.per); };
         pc.b = lens.find(pos, w.per_req, pieces_of, before, pc.len);
         if (pc.b < 0) return false;
         pc.of = f(pc.len);
-        pc.pieces = (int)pieces_of(pc.len);
-        const int64_t off = pos - before;
-        pc.u = (int)quotient(off, pc.pieces);
-        const int i = (int)(off - (int64_t)pc.u * pc.pieces);
-        pc.g0 = (int)(i * w.per);
-        pc.g1 = (int)min((int64_t)pc.of, (i + 1) * w.per);
-        pc.first = (int)pos - i;
+        pc.pieces = pieces_of(pc.len);
+        const int off = pos - before;
+        pc.u = quotient(off, pc.pieces);
+        const int i = off - pc.u * pc.pieces;
+        pc.g0 = i * w.per;
+        pc.g1 = min(pc.of, pc.g0 + w.per);
+        pc.first = pos - i;
         pc.slot = 2 * cta;
         pc.second = false;
         pos = end;
@@ -298,22 +292,27 @@ __device__ __forceinline__ bool next_piece(const Lengths& lens, F f, const Cut& 
         pc.b = lens.find(pos, w.per_req, f, before, pc.len);
         if (pc.b < 0) return false;
         pc.of = f(pc.len);
-        const int64_t off = pos - before;
-        pc.u = (int)quotient(off, pc.of);
-        pc.g0 = (int)(off - (int64_t)pc.u * pc.of);
-        pc.g1 = (int)min((int64_t)pc.of, pc.g0 + (end - pos));
-        const int64_t lo = pos - pc.g0;  // where the unit begins
-        pc.first = (int)quotient(lo, w.per);
-        pc.pieces = (int)quotient(lo + pc.of - 1, w.per) - pc.first + 1;
-        pc.second = (int64_t)pc.first * w.per < lo;
-        pc.slot = 2 * cta + (pos == (int64_t)cta * w.per ? 0 : 1);
+        const int off = pos - before;
+        pc.u = quotient(off, pc.of);
+        pc.g0 = off - pc.u * pc.of;
+        pc.g1 = min(pc.of, pc.g0 + (end - pos));
+        const int lo = pos - pc.g0;  // where the unit begins
+        pc.first = quotient(lo, w.per);
+        pc.pieces = quotient(lo + pc.of - 1, w.per) - pc.first + 1;
+        pc.second = pc.first * w.per < lo;
+        pc.slot = 2 * cta + (pos == cta * w.per ? 0 : 1);
         pos += pc.g1 - pc.g0;
     }
     return true;
 }
 // the partial record of piece i of a unit
-__device__ __forceinline__ int64_t slot_of(const Piece& pc, int i) {
-    return 2 * (int64_t)(pc.first + i) + (pc.second && i == 0 ? 1 : 0);
+__device__ __forceinline__ int slot_of(const Piece& pc, int i) {
+    return 2 * (pc.first + i) + (pc.second && i == 0 ? 1 : 0);
+}
+// whether all requests at their capacity are less than 2^31 pieces of work of `tokens` each (host)
+inline bool work_fits(int64_t bs, int64_t per_req, int64_t max_pages, int64_t page, int64_t tokens) {
+    const double all = (double)bs * (double)per_req * ((double)max_pages * (double)page / (double)tokens + 2.0);
+    return all < 2147483648.0;
 }
 
 // over the lanes with the same lane % 4

@@ -94,6 +94,11 @@ extern "C" int mfd_kv8_attention(const void* q, int64_t sq_b, int64_t sq_n, int6
         set_error("%s: workspace or tickets too small", who);
         return MFD_ERR_INVALID;
     }
+    if (!kv8::work_fits(bs, num_kv_heads * ((kv8_rows_total(n, num_heads, num_kv_heads) + 15) / 16), max_pages, page_size,
+                        128) || bs * num_heads * n > 0x7fffffff) {
+        set_error("%s: the requests' capacity is beyond this build's limits", who);
+        return MFD_ERR_UNSUPPORTED;
+    }
     if (bs == 0) return MFD_OK;
     kv8::AttnParams p;
     p.c.k = (const uint8_t*)k_cache, p.c.v = (const uint8_t*)v_cache;
@@ -121,10 +126,10 @@ extern "C" int mfd_kv8_attention(const void* q, int64_t sq_b, int64_t sq_n, int6
     p.tickets = tickets;
     const int sms = kv8::sm_count(), rows = p.rows;
     cudaStream_t s = (cudaStream_t)stream;
-    if (rows <= kRowsAlone) return kv8::launch_rows(p, sms, s);
+    if (rows <= kRowsAlone && p.nn <= kv8::kRowsMaxOwn) return kv8::launch_rows(p, sms, s);
     // pairs of 128-row tiles; a remainder of a few rows goes to the register kernel instead of a tile of padding
     const int rest = rows % 256;
-    const bool tail = rows > 256 && rest > 0 && rest <= kRowsAlone;
+    const bool tail = rows > 256 && rest > 0 && rest <= kRowsAlone && p.nn <= kv8::kRowsMaxOwn;
     if (tail) p.rows = rows - rest;
     st = kv8::launch_tc(p, rows > 128, sms, s);
     if (st != MFD_OK || !tail) return st;

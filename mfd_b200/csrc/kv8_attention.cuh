@@ -44,6 +44,8 @@ __device__ __forceinline__ void bar_sync(int id) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
 }
 
+// Own keys the register kernel takes (more rows' trees go to the tensor-core kernel).
+constexpr int kRowsMaxOwn = 128;
 // rows [p.row0, p.rows) with the register kernel (16 rows a unit)
 int launch_rows(const AttnParams& p, int sms, cudaStream_t stream);
 int64_t rows_tickets(int64_t bs, int64_t hkv, int64_t rows);

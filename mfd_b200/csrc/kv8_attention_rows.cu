@@ -47,10 +47,7 @@ constexpr int kSlot = 16 * (kD + 2);  // floats of a partial: m[16], l[16], O[16
 constexpr int kCtasPerSm = 2;
 constexpr float kLift = 12.f;  // the largest weights are 2^12, and up to 2^15 before the reference moves
 constexpr float kLazy = 3.f;
-
-__device__ __forceinline__ bool not_finite_pair(uint32_t w) {  // a bf16 pair holds an infinity or a NaN
-    return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
-}
+constexpr int kMaxOwn = kRowsMaxOwn;  // own keys a request
 
 // NT: 8-row tiles a unit
 template <bool FP8, int NT>
@@ -61,8 +58,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     extern __shared__ __align__(16) unsigned char smem_raw[];
     unsigned char* ring = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     float* smem = reinterpret_cast<float*>(ring);
-    __shared__ float4 s_const[kStages][kWarps];  // of 16 keys: K scale, log2 and reciprocal of the V scale
-    __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
+    __shared__ float2 s_scale[kStages][8];     // of the tile's pages: K scale, V scale
+    __shared__ float s_own[kRows][kMaxOwn];    // scores of the nodes' own keys (log2), -inf where not visible
+    __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows], s_mm[kRows], s_ll[kRows];
     __shared__ uint2 s_q[NT][8][32];  // query operands, the same for every warp (in registers they would spill)
     __shared__ uint64_t s_full[kStages], s_empty[kStages];
     __shared__ int s_last, s_failed;
@@ -81,8 +79,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     // ---- this CTA's share of the work, in tiles
     auto tiles_of = [](int len) { return max(1, (len + kTile - 1) / kTile); };  // (one, for the own keys or to write zeros)
     const Lengths lens(p.c, p.bs);
-    const Cut cut = make_cut(lens, tiles_of, p.c.Hkv * RB, gridDim.x, 1);
-    int64_t pos, end;
+    const Cut cut = make_cut(lens, tiles_of, p.c.Hkv * RB, gridDim.x);
+    int pos, end;
     cut_range(cut, blockIdx.x, pos, end);
     __syncthreads();
 
@@ -93,47 +91,60 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         const int hk = pc.u / RB, rb = pc.u % RB, len = pc.len;
         const int base = p.row0 + rb * 16;
 
-        // ---- the producer, warp 0: tile `next`'s copies and constants.  Page ids are read two tiles ahead and scales
+        // ---- the producer, warp 0: copies of a tile, then its constants.  Page ids are read two tiles ahead and scales
         // one, so it waits for neither; a stage is free once every warp has read its codes, two tiles before.
-        const int ppt = kTile >> p.c.page_shift, gpp = p.c.page >> 4;
-        int next = pc.g0, id0, id1;
-        float sk = 0.f, sv = 1.f;
-        auto id_of = [&](int tile) {  // lane j < ppt takes page j of a tile
+        const int ppt = kTile >> p.c.page_shift;
+        int next = pc.g0, id0 = -1, id1 = -1;  // the next tile to fetch, the page ids of it and of the one after
+        float2 sc = make_float2(0.f, 0.f);     // scales of tile `next`
+        auto id_of = [&](int tile) {           // lane j < ppt takes page j of a tile
             const int pg = tile * ppt + lane;
             return lane < ppt && tile < pc.g1 && (pg << p.c.page_shift) < len ? page_id(p.c, pc.b, pg) : -1;
         };
         auto scales = [&](int id) {
-            if (id < 0) return;
-            sk = __ldg(p.c.k_scale + (int64_t)id * p.c.Hkv + hk);
-            sv = __ldg(p.c.v_scale + (int64_t)id * p.c.Hkv + hk);
+            return id < 0 ? make_float2(0.f, 0.f) : make_float2(__ldg(p.c.k_scale + (int64_t)id * p.c.Hkv + hk),
+                                                                __ldg(p.c.v_scale + (int64_t)id * p.c.Hkv + hk));
         };
-        auto produce = [&]() {
-            const uint32_t nt = n_tile + next - pc.g0, st = nt % kStages;
-            if (nt >= (uint32_t)kStages)
-                ok = __all_sync(MFD_FULL_MASK, ok & mbar_wait(&s_empty[st], (nt / kStages - 1) & 1, kTries));
-            if (!ok) return;
-            if (id0 >= 0) {
+        auto copies = [&](uint32_t nt, int id) {
+            const uint32_t st = nt % kStages;
+            if (id >= 0) {
                 const uint32_t half = (uint32_t)(p.c.page * kD), dst = smem_addr(ring) + st * kStageBytes + lane * half;
                 mbar_expect_tx(&s_full[st], 2 * half);
-                tma_page(dst, &tmk, &s_full[st], hk, id0);
-                tma_page(dst + kStageBytes / 2, &tmv, &s_full[st], hk, id0);
-                const float s = fmaxf(sv, kScaleFloor);
-                const float4 k = make_float4(sk, __log2f(s), __frcp_rn(s), 0.f);
-                for (int i = 0; i < gpp; ++i) s_const[st][lane * gpp + i] = k;
+                tma_page(dst, &tmk, &s_full[st], hk, id);
+                tma_page(dst + kStageBytes / 2, &tmv, &s_full[st], hk, id);
             }
-            __syncwarp();  // lanes without a page (8 .. 31 never have one) arrive last, after every constant is stored
-            if (id0 < 0) mbar_arrive(&s_full[st]);
-            ++next;
-            id0 = id1;
-            scales(id0);
-            id1 = id_of(next + 1);
         };
-        if (warp == 0) {
+        auto constants = [&](uint32_t nt, int id, float2 s) {
+            const uint32_t st = nt % kStages;
+            if (id >= 0) s_scale[st][lane] = s;
+            __syncwarp();  // lanes without a page (8 .. 31 never have one) arrive last, after every scale is stored
+            if (id < 0) mbar_arrive(&s_full[st]);
+        };
+        if (warp == 0) {  // the first two tiles: both ids, both tiles' copies, both tiles' scales (the stages are free)
             id0 = id_of(next);
             id1 = id_of(next + 1);
-            scales(id0);
-            for (int i = 0; i < kStages - 1 && next < pc.g1; ++i) produce();
+            const int id2 = id_of(next + 2);
+            copies(n_tile, id0);
+            if (next + 1 < pc.g1) copies(n_tile + 1, id1);
+            const float2 s0 = scales(id0), s1 = scales(id1);
+            sc = scales(id2);
+            constants(n_tile, id0, s0);
+            if (next + 1 < pc.g1) constants(n_tile + 1, id1, s1);
+            next += 2;
+            id0 = id2;
+            id1 = id_of(next + 1);
         }
+        auto produce = [&]() {
+            const uint32_t nt = n_tile + next - pc.g0;
+            if (nt >= (uint32_t)kStages)
+                ok = __all_sync(MFD_FULL_MASK, ok & mbar_wait(&s_empty[nt % kStages], (nt / kStages - 1) & 1, kTries));
+            if (!ok) return;
+            copies(nt, id0);
+            constants(nt, id0, sc);
+            ++next;
+            id0 = id1;
+            sc = scales(id0);
+            id1 = id_of(next + 1);
+        };
 
         // ---- query row g (+ 8 nt) as float16 operands, divided by a power of two; the lane's softmax rows are 2 t, 2 t + 1
         float rf[NT][2];  // score factor of rows 2 t and 2 t + 1: the power of two, the scale and log2(e)
@@ -171,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                 for (int j = 0; j < 2; ++j) {
                     const float2 f0 = bf2(w[2 * j]), f1 = bf2(w[2 * j + 1]);
                     const int ks = 2 * i + j;
-                    if (warp == 0)
+                    if (warp == 1)  // (warp 0 has the copies)
                         s_q[n][ks][lane] = make_uint2(pack_half2(f0.x * down, f0.y * down), pack_half2(f1.x * down, f1.y * down));
                 }
             }
@@ -228,6 +239,37 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                 }
         };
 
+        // ---- scores of the nodes' own keys, while the first tiles are on their way: few products, on the CUDA cores (a
+        // second set of tensor instructions for them cost more in instruction fetches than in arithmetic).  Eight lanes a
+        // (row, key) pair, 16 columns each; the weights meet the values in the merge below.
+        const int live_rows = min(16, p.rows - base);
+        const int own = pc.g1 == pc.of ? p.nn : 0;  // of a unit's last piece
+#pragma unroll 1
+        for (int e0 = 4 * warp; e0 < live_rows * own; e0 += 4 * kWarps) {
+            const int e = min(e0 + (lane >> 3), live_rows * own - 1);
+            const int r = quotient(e, own), key = e - r * own, c = lane & 7;
+            const int nd = quotient(base + r, p.G), hd = hk * p.G + base + r - nd * p.G;
+            const uint4* qp = reinterpret_cast<const uint4*>(p.q + (int64_t)pc.b * p.sq_b + (int64_t)nd * p.sq_n +
+                                                             (int64_t)hd * p.sq_h + 16 * c);
+            const uint4* kp = reinterpret_cast<const uint4*>(p.kn + (int64_t)pc.b * p.sn_b + (int64_t)key * p.sn_n +
+                                                             (int64_t)hk * p.sn_h + 16 * c);
+            float dot = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint4 x = __ldg(qp + i), y = __ldg(kp + i);
+                const uint32_t u[4] = {x.x, x.y, x.z, x.w}, v[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 f = bf2(u[j]), h = bf2(v[j]);
+                    dot = fmaf(f.x, h.x, fmaf(f.y, h.y, dot));
+                }
+            }
+#pragma unroll
+            for (int d = 1; d < 8; d <<= 1) dot += __shfl_xor_sync(MFD_FULL_MASK, dot, d);
+            const bool sees = (visible_word(p, pc.b, nd, key >> 6) >> (key & 63)) & 1ull;
+            if (c == 0) s_own[r][key] = sees ? dot * p.scale_log2 : -INFINITY;
+        }
+
         // ---- cached tokens
         const uint32_t swk = (uint32_t)(g & 7) << 4;
 #pragma unroll 1
@@ -250,7 +292,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
                     kw[h][i] = *reinterpret_cast<const uint4*>(kt + h * 8 * kD + (((uint32_t)(2 * t + i) << 4) ^ swk));
-            const float4 cst = s_const[st][warp];
+            const float2 scale = s_scale[st][(16 * warp) >> p.c.page_shift];
+            const float sv = fmaxf(scale.y, kScaleFloor), lsv = __log2f(sv);
             float acc[NT][4], acc2[NT][4];  // two chains: the instruction's latency is several times its issue
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -279,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[n][e] = fmaf(acc[n][e] + acc2[n][e], cst.x * rf[n][e & 1], cst.y);
+                for (int e = 0; e < 4; ++e) w[n][e] = fmaf(acc[n][e] + acc2[n][e], scale.x * rf[n][e & 1], lsv);
             if (tail) {  // slots past the length hold any bits (an e4m3 NaN too): their weight is 0, their codes too
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
@@ -292,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_empty[st]);  // every lane has its codes
-            step(w, cst.z);
+            step(w, __frcp_rn(sv));
             uint32_t hi[NT][2], lo[NT][2];  // keys 0 .. 7 and 8 .. 15: B operands
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -322,132 +365,47 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             }
         }
 
-        // ---- the nodes' own keys, in bf16
-        const int g_own = pc.g1 == pc.of ? (p.nn + 15) / 16 : 0;  // of a unit's last piece
-#pragma unroll 1
-        for (int gi = warp; gi < g_own; gi += kWarps) {
-            const int j0 = gi * 16;
-            const __nv_bfloat16* kn = p.kn + (int64_t)pc.b * p.sn_b + (int64_t)hk * p.sn_h;
-            const __nv_bfloat16* vn = p.vn + (int64_t)pc.b * p.sn_b + (int64_t)hk * p.sn_h;
-            float acc[NT][4];
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
-            const __nv_bfloat16* k0 = kn + (int64_t)min(j0 + g, p.nn - 1) * p.sn_n;  // past the end: the last key
-            const __nv_bfloat16* k1 = kn + (int64_t)min(j0 + g + 8, p.nn - 1) * p.sn_n;  // again, masked below
-            const __nv_bfloat16* qr[NT];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const int r = min(base + 8 * n + g, p.rows - 1), nd = r / p.G;
-                qr[n] = p.q + (int64_t)pc.b * p.sq_b + (int64_t)nd * p.sq_n + (int64_t)(hk * p.G + r - nd * p.G) * p.sq_h;
-            }
-#pragma unroll 1
-            for (int i = 0; i < 4; ++i) {
-                const int col = 32 * t + 8 * i;
-                const uint4 x = __ldg(reinterpret_cast<const uint4*>(k0 + col)), y = __ldg(reinterpret_cast<const uint4*>(k1 + col));
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const uint4 q = __ldg(reinterpret_cast<const uint4*>(qr[n] + col));
-                    mma_bf16(acc[n], x.x, y.x, x.y, y.y, q.x, q.y);
-                    mma_bf16(acc[n], x.z, y.z, x.w, y.w, q.z, q.w);
-                }
-            }
-            uint32_t see[NT][2];  // bit i: the lane's row sees own key j0 + i
-            float w[NT][4];
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int r = base + 8 * n + 2 * t + e;
-                    see[n][e] = r < p.rows ? (uint32_t)(visible_word(p, pc.b, r / p.G, j0 >> 6) >> (j0 & 63)) & 0xffffu : 0u;
-                    w[n][e] = (see[n][e] >> g) & 1u ? acc[n][e] * p.scale_log2 : -INFINITY;
-                    w[n][2 + e] = (see[n][e] >> (g + 8)) & 1u ? acc[n][2 + e] * p.scale_log2 : -INFINITY;
-                }
-            step(w, 1.f);
-            uint32_t hi[NT][2], lo[NT][2];
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    split_bf16(pk2(w[n][2 * h], w[n][2 * h + 1]), hi[n][h], lo[n][h]);
-                    hi[n][h] = transpose8(hi[n][h]);
-                    lo[n][h] = transpose8(lo[n][h]);
-                }
-            bool odd = false;  // a non-finite value among this group's
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {  // d = 16 g + 8 half .. + 7
-                uint32_t x[4][4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = min(j0 + 2 * t + (i & 1) + 8 * (i >> 1), p.nn - 1);
-                    const uint4 vx = __ldg(reinterpret_cast<const uint4*>(vn + (int64_t)key * p.sn_n + 16 * g + 8 * half));
-                    x[i][0] = vx.x, x[i][1] = vx.y, x[i][2] = vx.z, x[i][3] = vx.w;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        odd |= not_finite_pair(x[i][c]);
-                        // 0 times an infinity is not 0: such a value leaves the product and is added below
-                        if ((x[i][c] & 0x7f80u) == 0x7f80u) x[i][c] &= 0xffff0000u;
-                        if ((x[i][c] & 0x7f800000u) == 0x7f800000u) x[i][c] &= 0xffffu;
-                    }
-                }
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const uint32_t a0 = __byte_perm(x[0][c], x[1][c], 0x5410), a1 = __byte_perm(x[0][c], x[1][c], 0x7632);
-                    const uint32_t a2 = __byte_perm(x[2][c], x[3][c], 0x5410), a3 = __byte_perm(x[2][c], x[3][c], 0x7632);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        mma_bf16(o[n][4 * half + c], a0, a1, a2, a3, hi[n][0], hi[n][1]);
-                        mma_bf16(o[n][4 * half + c], a0, a1, a2, a3, lo[n][0], lo[n][1]);
-                    }
-                }
-            }
-            if (__any_sync(MFD_FULL_MASK, odd)) {
-                // rare: add the infinities and NaNs to the rows that see their key (a weight is above 0, so their
-                // size does not matter)
-#pragma unroll 1
-                for (int i = 0; i < min(16, p.nn - j0); ++i) {
-                    const __nv_bfloat16* vrow = vn + (int64_t)(j0 + i) * p.sn_n + 16 * g;
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float y = __bfloat162float(vrow[j]);
-                        if (fabsf(y) < INFINITY) continue;
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                                if ((see[n][e] >> i) & 1u) o[n][j >> 1][2 * (j & 1) + e] += y;
-                    }
-                }
-            }
-        }
-
-        // ---- the warps of the piece merge
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                l[n][e] = column_sum(l[n][e]);
-                if (g == 0) s_m[warp][8 * n + 2 * t + e] = m[n][e], s_l[warp][8 * n + 2 * t + e] = l[n][e];
-            }
-        __syncthreads();
+        // ---- the warps of the piece merge: O as it is in shared memory, their weights per row beside it
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int r = 8 * n + 2 * t + e;
-                float mm = -INFINITY;
+                l[n][e] = column_sum(l[n][e]);
+                if (g == 0) s_m[warp][r] = m[n][e], s_l[warp][r] = l[n][e];
+            }
+        __syncthreads();  // (and every warp is past the ring)
+#pragma unroll 1
+        for (int r = warp; r < kRows; r += kWarps) {  // a warp a row: the warps' (m, l), then the own keys
+            float mm = lane < kWarps ? s_m[lane][r] : -INFINITY;
+            for (int j = lane; j < own; j += 32) mm = fmaxf(mm, s_own[r][j]);
+            mm = warp_max_f32(mm);
+            float ll = 0.f;
+            if (lane < kWarps) {
+                const float a = s_m[lane][r] == -INFINITY ? 0.f : fast_exp2(s_m[lane][r] - mm);
+                ll = s_l[lane][r] * a;  // (a NaN sum stays one)
+                s_m[lane][r] = a;
+            }
+            for (int j = lane; j < own; j += 32) {
+                const float a = s_own[r][j] == -INFINITY ? 0.f : fast_exp2(s_own[r][j] - mm);
+                ll += a;
+                s_own[r][j] = a;
+            }
+#pragma unroll 1
+            for (int d = 16; d; d >>= 1) ll += __shfl_xor_sync(MFD_FULL_MASK, ll, d);
+            if (lane == 0) s_mm[r] = mm, s_ll[r] = ll;
+        }
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w][r]);
-                const float a = m[n][e] == -INFINITY ? 0.f : fast_exp2(m[n][e] - mm);
-                float* row = smem + (warp * kRows + r) * kRowStride + g * kDBlock;
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float* row = smem + (warp * kRows + 8 * n + 2 * t + e) * kRowStride + g * kDBlock;
 #pragma unroll
                 for (int j = 0; j < 8; j += 2)
-                    *reinterpret_cast<float4*>(row + 2 * j) = make_float4(o[n][j][e] * a, o[n][j][2 + e] * a,
-                                                                          o[n][j + 1][e] * a, o[n][j + 1][2 + e] * a);
+                    *reinterpret_cast<float4*>(row + 2 * j) = make_float4(o[n][j][e], o[n][j][2 + e], o[n][j + 1][e],
+                                                                          o[n][j + 1][2 + e]);
             }
         __syncthreads();
-        const int live_rows = min(16, p.rows - base);
         const bool whole = pc.pieces == 1;
         float* slot = p.part + (int64_t)pc.slot * kSlot;
         auto store = [&](int r, int col, float4 v, float mm, float ll) {  // columns col .. col + 3 of row r, and lse
@@ -458,24 +416,31 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             if (p.lse && col == 0)
                 p.lse[((int64_t)pc.b * p.n + nd) * p.H + hd] = ll == 0.f ? -INFINITY : 0.6931471805599453f * (mm + log2f(ll));
         };
+#pragma unroll 1
         for (int e = tid; e < live_rows * 32; e += kThreads) {
             const int r = e >> 5, c4 = e & 31;
-            float mm = -INFINITY, ll = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w][r]);
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
+#pragma unroll 2
             for (int w = 0; w < kWarps; ++w) {
-                const float mw = s_m[w][r];
-                ll += s_l[w][r] * (mw == -INFINITY ? 0.f : fast_exp2(mw - mm));  // (a NaN sum stays one)
+                const float a = s_m[w][r];
                 const float4 x = *reinterpret_cast<const float4*>(smem + (w * kRows + r) * kRowStride + (c4 >> 2) * kDBlock +
                                                                   (c4 & 3) * 4);
-                v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+                v.x = fmaf(a, x.x, v.x), v.y = fmaf(a, x.y, v.y), v.z = fmaf(a, x.z, v.z), v.w = fmaf(a, x.w, v.w);
+            }
+#pragma unroll 4
+            for (int j = 0; j < own; ++j) {
+                const float a = s_own[r][j];
+                uint2 y = make_uint2(0u, 0u);  // a value the row does not see has no effect, an infinite one neither
+                if (a != 0.f)
+                    y = __ldg(reinterpret_cast<const uint2*>(p.vn + (int64_t)pc.b * p.sn_b + (int64_t)j * p.sn_n +
+                                                             (int64_t)hk * p.sn_h + 4 * c4));
+                const float2 f = bf2(y.x), h = bf2(y.y);
+                v.x = fmaf(a, f.x, v.x), v.y = fmaf(a, f.y, v.y), v.z = fmaf(a, h.x, v.z), v.w = fmaf(a, h.y, v.w);
             }
             if (whole) {
-                store(r, 4 * c4, v, mm, ll);
+                store(r, 4 * c4, v, s_mm[r], s_ll[r]);
             } else {
-                if (c4 == 0) slot[r] = mm, slot[16 + r] = ll;
+                if (c4 == 0) slot[r] = s_mm[r], slot[16 + r] = s_ll[r];
                 *reinterpret_cast<float4*>(slot + 32 + r * kD + 4 * c4) = v;
             }
         }
@@ -488,8 +453,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             __syncthreads();
             if (s_last) {
                 __threadfence();
-                auto record = [&](int i) { return p.part + slot_of(pc, i) * kSlot; };
-                float* wgt = smem;  // [pieces][16] weights in turn, the rows' (m, l) in s_m[0], s_l[0]
+                auto record = [&](int i) { return p.part + (int64_t)slot_of(pc, i) * kSlot; };
+                float* wgt = smem;  // [pieces][16] weights
                 constexpr int kBatch = 512;
                 float4 v[2];
                 v[0] = v[1] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -506,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                     }
 #pragma unroll
                     for (int d = 16; d; d >>= 1) ll += __shfl_xor_sync(MFD_FULL_MASK, ll, d);
-                    if (lane == 0) s_m[0][r] = mm, s_l[0][r] = ll;
+                    if (lane == 0) s_mm[r] = mm, s_ll[r] = ll;
                 }
                 __syncthreads();
 #pragma unroll
@@ -522,13 +487,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                                 a = wgt[i * 16 + r];
                             } else {
                                 const float mi = __ldcg(sl + r);
-                                a = mi == -INFINITY ? 0.f : fast_exp2(mi - s_m[0][r]);
+                                a = mi == -INFINITY ? 0.f : fast_exp2(mi - s_mm[r]);
                             }
                             const float4 x = __ldcg(reinterpret_cast<const float4*>(sl + 32 + r * kD + 4 * c4));
                             v[u].x = fmaf(a, x.x, v[u].x), v[u].y = fmaf(a, x.y, v[u].y);
                             v[u].z = fmaf(a, x.z, v[u].z), v[u].w = fmaf(a, x.w, v[u].w);
                         }
-                        store(r, 4 * c4, v[u], s_m[0][r], s_l[0][r]);
+                        store(r, 4 * c4, v[u], s_mm[r], s_ll[r]);
                     }
                 }
                 if (tid == 0) *ticket = 0u;

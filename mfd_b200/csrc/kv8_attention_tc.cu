@@ -139,8 +139,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int RB = (p.rows - p.row0 + 128 * L::kRowTiles - 1) / (128 * L::kRowTiles);
     auto tiles_of = [&](int len) { return max(1, (len + kKt - 1) / kKt + (p.nn + kKt - 1) / kKt); };
     const Lengths lens(p.c, p.bs);
-    const Cut cut = make_cut(lens, tiles_of, p.c.Hkv * RB, gridDim.x, 1);
-    int64_t pos, end;
+    const Cut cut = make_cut(lens, tiles_of, p.c.Hkv * RB, gridDim.x);
+    int pos, end;
     cut_range(cut, blockIdx.x, pos, end);
 
     // Every role walks the CTA's pieces in its own loop (below), all meeting at the end of each.
@@ -178,20 +178,25 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         pieces([&](const Piece& pc, const Tiles& x) {
             // ------------------------------------------------------------ queries into their operand layout
-            for (int rtile = 0; rtile < x.ntl; ++rtile) {
-                uint4 qv[8];
+#pragma unroll 1
+            for (int r0 = 0; r0 < 128 * x.ntl; r0 += 64) {
+                uint4 qv[4];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int r = (tid >> 4) + 16 * j, c = tid & 15, row = x.row_base + 128 * rtile + r;
+                for (int j = 0; j < 4; ++j) {
+                    const int row = x.row_base + r0 + (tid >> 4) + 16 * j;
+                    const int node = quotient(row, p.G);
                     qv[j] = make_uint4(0u, 0u, 0u, 0u);
                     if (row < p.rows)
-                        qv[j] = __ldg(reinterpret_cast<const uint4*>(p.q + (int64_t)pc.b * p.sq_b + (int64_t)(row / p.G) * p.sq_n +
-                                                                    (int64_t)(x.hk * p.G + row % p.G) * p.sq_h + c * 8));
+                        qv[j] = __ldg(reinterpret_cast<const uint4*>(p.q + (int64_t)pc.b * p.sq_b + (int64_t)node * p.sq_n +
+                                                                     (int64_t)(x.hk * p.G + row - node * p.G) * p.sq_h +
+                                                                     (tid & 15) * 8));
                 }
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    *reinterpret_cast<uint4*>(smem + L::kOffQ + rtile * kTileBytes +
-                                              sw128_offset((tid >> 4) + 16 * j, (tid & 15) * 8, 128)) = qv[j];
+                for (int j = 0; j < 4; ++j) {
+                    const int r = r0 + (tid >> 4) + 16 * j;
+                    *reinterpret_cast<uint4*>(smem + L::kOffQ + (r >> 7) * kTileBytes +
+                                              sw128_offset(r & 127, (tid & 15) * 8, 128)) = qv[j];
+                }
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -581,8 +586,8 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(const AttnParams p, in
     const int RB = (p.rows - p.row0 + kRowsU - 1) / kRowsU;
     auto tiles_of = [&](int len) { return max(1, (len + kKt - 1) / kKt + (p.nn + kKt - 1) / kKt); };
     const Lengths lens(p.c, p.bs);
-    const Cut cut = make_cut(lens, tiles_of, p.c.Hkv * RB, ctas, 1);
-    int64_t pos, end;
+    const Cut cut = make_cut(lens, tiles_of, p.c.Hkv * RB, ctas);
+    int pos, end;
     cut_range(cut, cta, pos, end);
     Piece pc;
     if (!next_piece(lens, tiles_of, cut, cta, pos, end, pc)) return;
@@ -591,14 +596,14 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(const AttnParams p, in
     const int r = blockIdx.y * 32 + lane, row = p.row0 + rb * kRowsU + r;
     if (row - lane >= p.rows) return;
     float mm = -INFINITY;
-    for (int i = 0; i < pc.pieces; ++i) mm = fmaxf(mm, __ldg(p.part + slot_of(pc, i) * kSlotFloats(PAIR) + r));
+    for (int i = 0; i < pc.pieces; ++i) mm = fmaxf(mm, __ldg(p.part + (int64_t)slot_of(pc, i) * kSlotFloats(PAIR) + r));
     float ll = 0.f;
     float4 v[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 2
     for (int i = 0; i < pc.pieces; ++i) {
-        const float* s = p.part + slot_of(pc, i) * kSlotFloats(PAIR);
+        const float* s = p.part + (int64_t)slot_of(pc, i) * kSlotFloats(PAIR);
         const float mi = __ldg(s + r), li = __ldg(s + kRowsU + r);
         const float a = mi == -INFINITY ? 0.f : fast_exp2(mi - mm);
         ll = fmaf(a, li, ll);

@@ -53,21 +53,20 @@ __global__ void __launch_bounds__(kWThreads, kWCtasPerSm) kv8_weights_kernel(con
     const int Hkv = p.c.Hkv;
     auto tasks_of = [&](int len) { return max(1, (len + 31) / 32); };
     const Lengths lens(p.c, p.bs);
-    const int64_t total = lens.sum(tasks_of, p.bs) * Hkv;
-    int64_t per = quotient(total + gridDim.x - 1, gridDim.x);
+    const int total = lens.sum(tasks_of) * Hkv;
+    int per = quotient(total + gridDim.x - 1, gridDim.x);
     if (per < kWWarps) per = kWWarps;
-    int64_t pos = (int64_t)blockIdx.x * per;
-    const int64_t end = pos + per < total ? pos + per : total;
+    int pos = (int)min((int64_t)blockIdx.x * per, (int64_t)total);
+    const int end = (int)min((int64_t)total, (int64_t)pos + per);
 
     while (pos < end) {
-        int64_t before;
-        int len;
+        int before, len;
         const int b = lens.find(pos, Hkv, tasks_of, before, len);
         if (b < 0) return;
         const int tasks = tasks_of(len);
-        const int64_t off = pos - before;
-        const int hk = (int)quotient(off, tasks), t0 = (int)(off - (int64_t)hk * tasks);
-        const int t1 = (int)min((int64_t)tasks, t0 + (end - pos));
+        const int off = pos - before;
+        const int hk = quotient(off, tasks), t0 = off - hk * tasks;
+        const int t1 = min(tasks, t0 + (end - pos));
         const int listed = listed_rows(p.path, p.path_stride, p.rows, p.counts, p.n, b);
         const int nrows = listed * p.G;
         float* part = p.part + (int64_t)b * p.groups_max * Hkv + hk;
@@ -190,9 +189,8 @@ __global__ void __launch_bounds__(kWThreads, kWCtasPerSm) kv8_weights_kernel(con
         }
         pos += t1 - t0;
         // ---- the request's last CTA adds up its pages
-        if (pos >= end || pos >= before + (int64_t)tasks * Hkv) {
-            const int64_t last = before + (int64_t)tasks * Hkv - 1;
-            const int pieces = (int)(quotient(last, per) - quotient(before, per)) + 1;
+        if (pos >= end || pos >= before + tasks * Hkv) {
+            const int pieces = quotient(before + tasks * Hkv - 1, per) - quotient(before, per) + 1;
             __threadfence();
             __syncthreads();
             if (tid == 0) s_last = pieces == 1 || atomicAdd(p.tickets + b, 1u) == (unsigned)(pieces - 1);
@@ -264,6 +262,10 @@ extern "C" int mfd_kv8_page_weights(const void* q, int64_t sq_b, int64_t sq_n, i
     if (workspace_bytes < mfd_kv8_page_weights_workspace(bs, max_pages, page_size, num_kv_heads) || tickets_len < bs) {
         set_error("%s: workspace or tickets too small", who);
         return MFD_ERR_INVALID;
+    }
+    if (!kv8::work_fits(bs, num_kv_heads, max_pages, page_size, 32)) {
+        set_error("%s: the requests' capacity is beyond this build's limits", who);
+        return MFD_ERR_UNSUPPORTED;
     }
     if (bs == 0) return MFD_OK;
     kv8::WeightParams p;
