@@ -240,22 +240,24 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         };
 
         // ---- scores of the nodes' own keys, while the first tiles are on their way: few products, on the CUDA cores (a
-        // second set of tensor instructions for them cost more in instruction fetches than in arithmetic).  Eight lanes a
-        // (row, key) pair, 16 columns each; the weights meet the values in the merge below.
+        // second set of tensor instructions for them cost more in instruction fetches than in arithmetic).  The weights meet the
+        // values in the merge below.
         const int live_rows = min(16, p.rows - base);
         const int own = pc.g1 == pc.of ? p.nn : 0;  // of a unit's last piece
-#pragma unroll 1
-        for (int e0 = 4 * warp; e0 < live_rows * own; e0 += 4 * kWarps) {
-            const int e = min(e0 + (lane >> 3), live_rows * own - 1);
-            const int r = quotient(e, own), key = e - r * own, c = lane & 7;
+        auto score = [&](int r, int key, float dot) {
+            const int nd = quotient(base + r, p.G);
+            const bool sees = (visible_word(p, pc.b, nd, key >> 6) >> (key & 63)) & 1ull;
+            s_own[r][key] = sees ? dot * p.scale_log2 : -INFINITY;
+        };
+        auto pair_dot = [&](int r, int key, int c, int chunks) {  // of 8-column chunks c ..
             const int nd = quotient(base + r, p.G), hd = hk * p.G + base + r - nd * p.G;
             const uint4* qp = reinterpret_cast<const uint4*>(p.q + (int64_t)pc.b * p.sq_b + (int64_t)nd * p.sq_n +
-                                                             (int64_t)hd * p.sq_h + 16 * c);
+                                                             (int64_t)hd * p.sq_h) + c;
             const uint4* kp = reinterpret_cast<const uint4*>(p.kn + (int64_t)pc.b * p.sn_b + (int64_t)key * p.sn_n +
-                                                             (int64_t)hk * p.sn_h + 16 * c);
+                                                             (int64_t)hk * p.sn_h) + c;
             float dot = 0.f;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
+#pragma unroll 2
+            for (int i = 0; i < chunks; ++i) {
                 const uint4 x = __ldg(qp + i), y = __ldg(kp + i);
                 const uint32_t u[4] = {x.x, x.y, x.z, x.w}, v[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
@@ -264,10 +266,20 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                     dot = fmaf(f.x, h.x, fmaf(f.y, h.y, dot));
                 }
             }
-#pragma unroll
-            for (int d = 1; d < 8; d <<= 1) dot += __shfl_xor_sync(MFD_FULL_MASK, dot, d);
-            const bool sees = (visible_word(p, pc.b, nd, key >> 6) >> (key & 63)) & 1ull;
-            if (c == 0) s_own[r][key] = sees ? dot * p.scale_log2 : -INFINITY;
+            return dot;
+        };
+        // eight lanes a (row, key) pair, or (the last rows of a tree, whose own keys are all its nodes) a thread
+        const int lanes = own > 16 ? 1 : 8;
+#pragma unroll 1
+        for (int e0 = tid / lanes; e0 - (lane / lanes) < live_rows * own; e0 += kThreads / lanes) {
+            const int e = min(e0, live_rows * own - 1);
+            const int key = quotient(e, live_rows), r = e - key * live_rows, c = lane & (lanes - 1);
+            float dot = pair_dot(r, key, 2 * c, 16 / lanes);
+            if (lanes > 1) {
+#pragma unroll 1
+                for (int d = 1; d < 8; d <<= 1) dot += __shfl_xor_sync(MFD_FULL_MASK, dot, d);
+            }
+            if (c == 0) score(r, key, dot);
         }
 
         // ---- cached tokens
@@ -427,13 +439,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                                                                   (c4 & 3) * 4);
                 v.x = fmaf(a, x.x, v.x), v.y = fmaf(a, x.y, v.y), v.z = fmaf(a, x.z, v.z), v.w = fmaf(a, x.w, v.w);
             }
-#pragma unroll 4
+#pragma unroll 8
             for (int j = 0; j < own; ++j) {
                 const float a = s_own[r][j];
-                uint2 y = make_uint2(0u, 0u);  // a value the row does not see has no effect, an infinite one neither
-                if (a != 0.f)
-                    y = __ldg(reinterpret_cast<const uint2*>(p.vn + (int64_t)pc.b * p.sn_b + (int64_t)j * p.sn_n +
-                                                             (int64_t)hk * p.sn_h + 4 * c4));
+                uint2 y = __ldg(reinterpret_cast<const uint2*>(p.vn + (int64_t)pc.b * p.sn_b + (int64_t)j * p.sn_n +
+                                                               (int64_t)hk * p.sn_h + 4 * c4));
+                if (a == 0.f) y = make_uint2(0u, 0u);  // what the row does not see has no effect, an infinite value neither
                 const float2 f = bf2(y.x), h = bf2(y.y);
                 v.x = fmaf(a, f.x, v.x), v.y = fmaf(a, f.y, v.y), v.z = fmaf(a, h.x, v.z), v.w = fmaf(a, h.y, v.w);
             }
