@@ -510,6 +510,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                 if (tid == 0) *ticket = 0u;
             }
         }
+        if (!ok && warp == 0)  // copies in flight end before the CTA does (bounded)
+            for (uint32_t f = n_tile + next - pc.g0, i = f > kStages ? f - kStages : 0u; i < f; ++i)
+                mbar_wait(&s_full[i % kStages], (i / kStages) & 1, 1u << 14);
         fence_proxy_async_smem();  // (the next piece's copies land where the merge was)
         n_tile += pc.g1 - pc.g0;
         if (!ok) atomicExch(&s_failed, 1);

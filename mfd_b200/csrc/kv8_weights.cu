@@ -6,23 +6,31 @@
 // maximum, no second product.  Scores are formed as in the attention (codes exact in float16, query rows divided by a
 // power of two, float32 sums); every weight and sum is float32.
 //
-// Bound: K's bytes (128 codes a token and KV head), next the tensor instructions (2 * 128 flop per listed row and
-// token) and the shared-memory reads of the query operands.  A warp takes 32 tokens of one KV head, their codes in
-// registers as operands, and runs all listed rows past them, 16 at a time from shared memory; twice the tokens a warp
-// halve those reads, and 64 tokens do not fit the registers of two CTAs an SM.
+// Bound: K's bytes (128 codes a token and KV head); next, instructions: the scores' products of 2 * 128 flop and an
+// exponential per listed row and token.  As in kv8_attention_rows.cu the 16 tokens are the wide operand of the tensor
+// instruction and 8 query rows the narrow one, and the codes come by TMA, a page a copy, into a ring of two 32 KB stages
+// (256 tokens; two CTAs an SM).  A warp turns 32 tokens' codes into operands once and runs all listed rows past them, 8 at a
+// time from shared memory: 32 tokens rather than 16 halve those reads, which would otherwise take as long as the codes.
 //
-// Split: the 32-token tasks of all (request, KV head) units are laid end to end and cut into equal ranges, one per CTA,
-// so ragged lengths balance.  Each 16 tokens' sum goes to the workspace; the CTA that finishes a request last adds
-// them up per page, in a fixed order over tokens and heads (no float atomics).
-#include "kv8.cuh"
+// Split: the tiles of all (request, KV head) units are laid end to end and cut into equal ranges, one per CTA, so ragged
+// lengths balance.  Each 16 tokens' sum goes to the workspace; the CTA that finishes a request last adds them up per
+// page, in a fixed order over tokens and heads (no float atomics).
+//
+// Every mbarrier wait is bounded; a CTA whose wait gave up stores NaN sums, so the masses show it.
+#include "kv8_attention.cuh"
+#include "tcgen05.cuh"
 
 namespace mfd {
 namespace kv8 {
 
 constexpr int kWWarps = 8;
 constexpr int kWThreads = 32 * kWWarps;
-constexpr int kWTiles = 8;      // 16-row tiles staged at a time
+constexpr int kWTile = 256;     // tokens a stage
+constexpr int kWStages = 2;
+constexpr int kWStageBytes = kWTile * kD;
+constexpr int kWRowTiles = 16;  // 8-row tiles staged at a time
 constexpr int kWCtasPerSm = 2;
+constexpr uint32_t kWTries = 1u << 20;
 
 struct WeightParams {
     Cache c;
@@ -44,153 +52,218 @@ struct WeightParams {
 };
 
 template <bool FP8>
-__global__ void __launch_bounds__(kWThreads, kWCtasPerSm) kv8_weights_kernel(const WeightParams p) {
-    __shared__ uint4 s_q[kWTiles][8][32];           // query operands: tile, 16-column step, lane
-    __shared__ float s_rf[kWTiles * 16], s_lse[kWTiles * 16];
+__global__ void __launch_bounds__(kWThreads, kWCtasPerSm)
+    kv8_weights_kernel(const __grid_constant__ CUtensorMap tmk, const WeightParams p) {
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    unsigned char* ring = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+    auto s_q = reinterpret_cast<uint2(*)[8][32]>(ring + kWStages * kWStageBytes);  // query operands: tile, step, lane
+    __shared__ __align__(16) float2 s_row[kWRowTiles][8];  // score factor and -log2(e) * log-sum-exp of a row
+    __shared__ float s_scale[kWStages][16];  // K scales of the tile's pages
+    __shared__ uint64_t s_full[kWStages], s_empty[kWStages];
     __shared__ int s_last;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
+    if (tid == 0) {
+        for (int i = 0; i < kWStages; ++i) {
+            mbar_init(&s_full[i], 32);
+            mbar_init(&s_empty[i], kWWarps);
+        }
+        mbar_fence_init();
+    }
     const int Hkv = p.c.Hkv;
-    auto tasks_of = [&](int len) { return max(1, (len + 31) / 32); };
+    auto tiles_of = [&](int len) { return max(1, (len + kWTile - 1) / kWTile); };
     const Lengths lens(p.c, p.bs);
-    const int total = lens.sum(tasks_of) * Hkv;
-    int per = quotient(total + gridDim.x - 1, gridDim.x);
-    if (per < kWWarps) per = kWWarps;
+    const int total = lens.sum(tiles_of) * Hkv;
+    const int per = max(1, quotient(total + gridDim.x - 1, gridDim.x));
     int pos = (int)min((int64_t)blockIdx.x * per, (int64_t)total);
     const int end = (int)min((int64_t)total, (int64_t)pos + per);
+    __syncthreads();
 
+    uint32_t n_tile = 0;  // tiles fetched before: the barriers' phases
+    bool ok = true;
     while (pos < end) {
         int before, len;
-        const int b = lens.find(pos, Hkv, tasks_of, before, len);
+        const int b = lens.find(pos, Hkv, tiles_of, before, len);
         if (b < 0) return;
-        const int tasks = tasks_of(len);
+        const int tiles = tiles_of(len);
         const int off = pos - before;
-        const int hk = quotient(off, tasks), t0 = off - hk * tasks;
-        const int t1 = min(tasks, t0 + (end - pos));
+        const int hk = quotient(off, tiles), t0 = off - hk * tiles;
+        const int t1 = min(tiles, t0 + (end - pos));
         const int listed = listed_rows(p.path, p.path_stride, p.rows, p.counts, p.n, b);
         const int nrows = listed * p.G;
         float* part = p.part + (int64_t)b * p.groups_max * Hkv + hk;
 
+        // ---- the producer, warp 0: a tile's copies, then its scales; ids two tiles and scales one tile ahead
+        const int ppt = kWTile >> p.c.page_shift;  // at most 16
+        int next = 0, id0 = -1, id1 = -1;
+        float sc = 0.f;
+        auto id_of = [&](int tile) {
+            const int pg = tile * ppt + lane;
+            return lane < ppt && tile < t1 && (pg << p.c.page_shift) < len ? page_id(p.c, b, pg) : -1;
+        };
+        auto scale_of = [&](int id) { return id < 0 ? 0.f : __ldg(p.c.k_scale + (int64_t)id * Hkv + hk); };
+        auto produce = [&]() {
+            const uint32_t nt = n_tile + next - t0, st = nt % kWStages;
+            if (nt >= (uint32_t)kWStages)
+                ok = __all_sync(MFD_FULL_MASK, ok & mbar_wait(&s_empty[st], (nt / kWStages - 1) & 1, kWTries));
+            if (!ok) return;
+            if (id0 >= 0) {
+                const uint32_t bytes = (uint32_t)(p.c.page * kD);
+                mbar_expect_tx(&s_full[st], bytes);
+                tma_page(smem_addr(ring) + st * kWStageBytes + lane * bytes, &tmk, &s_full[st], hk, id0);
+                s_scale[st][lane] = sc;
+            }
+            __syncwarp();  // lanes without a page (16 .. 31 never have one) arrive last, after every scale is stored
+            if (id0 < 0) mbar_arrive(&s_full[st]);
+            ++next;
+            id0 = id1;
+            sc = scale_of(id0);
+            id1 = id_of(next + 1);
+        };
+
         // one pass in all but extreme cases: 128 rows are staged at a time
-        for (int r0 = 0; r0 == 0 || r0 < nrows; r0 += kWTiles * 16) {
-            const int tiles = min(kWTiles, (nrows - r0 + 15) / 16);
-            __syncthreads();
-            if (warp < tiles) {
+#pragma unroll 1
+        for (int r0 = 0; r0 == 0 || r0 < nrows; r0 += kWRowTiles * 8) {
+            const int row_tiles = min(kWRowTiles, (nrows - r0 + 7) / 8);
+            if (warp == 0) {
+                next = t0;
+                id0 = id_of(t0), id1 = id_of(t0 + 1);
+                sc = scale_of(id0);
+                for (int i = 0; i < kWStages && next < t1; ++i) produce();
+            }
+            // ---- the listed rows as operands: row g of tile w for warp w
+#pragma unroll 1
+            for (int rt = kWWarps - 1 - warp; rt < row_tiles; rt += kWWarps) {  // (warp 0, the producer, last)
+                const int r = r0 + rt * 8 + g;
+                const bool live = r < nrows;
+                const int i = live ? quotient(r, p.G) : 0;
+                const int64_t node = live && p.path ? __ldg((const long long*)p.path + (int64_t)b * p.path_stride + i) : i;
+                const int head = hk * p.G + (live ? r - i * p.G : 0);
+                const uint4* row = reinterpret_cast<const uint4*>(p.q + (int64_t)b * p.sq_b + node * p.sq_n +
+                                                                  (int64_t)head * p.sq_h + 32 * t);
+                uint4 x[4];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int r = r0 + warp * 16 + g + 8 * h;
-                    const bool live = r < nrows;
-                    const int i = live ? r / p.G : 0;
-                    const int64_t node = live && p.path ? __ldg((const long long*)p.path + (int64_t)b * p.path_stride + i) : i;
-                    const int head = hk * p.G + (live ? r % p.G : 0);
-                    const __nv_bfloat16* row = p.q + (int64_t)b * p.sq_b + node * p.sq_n + (int64_t)head * p.sq_h;
-                    uint4 x[4];
+                for (int u = 0; u < 4; ++u) {
+                    x[u] = make_uint4(0u, 0u, 0u, 0u);
+                    if (live) x[u] = __ldg(row + u);
+                }
+                const float ls = live ? __ldg(p.lse + ((int64_t)b * p.n + node) * p.H + head) : -INFINITY;
+                float mx = 0.f;
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        x[u] = make_uint4(0u, 0u, 0u, 0u);
-                        if (live) x[u] = __ldg(reinterpret_cast<const uint4*>(row + 16 * t + 8 * (u & 1) + 64 * (u >> 1)));
-                    }
-                    float mx = 0.f;
+                for (int u = 0; u < 4; ++u) {
+                    const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float2 f = bf2(w[j]);
-                            mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
-                        }
-                    }
-                    mx = quad_max(mx);
-                    float down, up;
-                    row_power(mx, down, up);
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const float2 f0 = bf2(w[2 * j]), f1 = bf2(w[2 * j + 1]);
-                            const int ks = 4 * (u >> 1) + 2 * (u & 1) + j;
-                            uint32_t* dst = reinterpret_cast<uint32_t*>(&s_q[warp][ks][lane]);
-                            dst[h] = pack_half2(f0.x * down, f0.y * down);       // operand registers: rows g, g + 8 at
-                            dst[2 + h] = pack_half2(f1.x * down, f1.y * down);   // columns k, then both at k + 8
-                        }
-                    }
-                    if (t == 0) {
-                        const float ls = live ? __ldg(p.lse + ((int64_t)b * p.n + node) * p.H + head) : -INFINITY;
-                        s_rf[warp * 16 + g + 8 * h] = live ? up * p.scale_log2 : 0.f;
-                        // a row that saw nothing, or padding, weighs nothing
-                        s_lse[warp * 16 + g + 8 * h] = ls == -INFINITY ? -INFINITY : -ls * kLog2e;
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 f = bf2(w[j]);
+                        mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
                     }
                 }
+                mx = quad_max(mx);
+                float down, up;
+                row_power(mx, down, up);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float2 f0 = bf2(w[2 * j]), f1 = bf2(w[2 * j + 1]);
+                        s_q[rt][2 * u + j][lane] =
+                            make_uint2(pack_half2(f0.x * down, f0.y * down), pack_half2(f1.x * down, f1.y * down));
+                    }
+                }
+                // a row that saw nothing, or padding, weighs nothing
+                if (t == 0)
+                    s_row[rt][g] = make_float2(live ? up * p.scale_log2 : 0.f, ls == -INFINITY ? -INFINITY : -ls * kLog2e);
             }
             __syncthreads();
-            for (int task = t0 + warp; task < t1; task += kWWarps) {
-                uint32_t kb[4][8][2];  // 8-token tiles: operands of the 8 steps
+#pragma unroll 1
+            for (int tile = t0; tile < t1; ++tile) {
+                const uint32_t nt = n_tile + tile - t0, st = nt % kWStages;
+                ok = __all_sync(MFD_FULL_MASK, ok & mbar_wait(&s_full[st], (nt / kWStages) & 1, kWTries));
+                if (!ok) break;
+                const int key0 = tile * kWTile + 32 * warp;
+                uint4 raw[2][2][2];  // of 16 tokens each: token g, g + 8; chunks 2 t, 2 t + 1
                 float sk[2];
-                uint4 raw[4][2];
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-                    const int key0 = task * 32 + 16 * q;
-                    const int id = key0 < len ? page_id(p.c, b, key0 >> p.c.page_shift) : 0;
-                    sk[q] = key0 < len ? __ldg(p.c.k_scale + (int64_t)id * Hkv + hk) : 0.f;
-                    const uint8_t* src = p.c.k + (int64_t)id * p.c.sc_p + (int64_t)hk * p.c.sc_h +
-                                         (int64_t)((key0 & (p.c.page - 1)) + g) * p.c.sc_t + 16 * t;
+                    const unsigned char* kt = ring + st * kWStageBytes + (32 * warp + 16 * q + g) * kD;
 #pragma unroll
-                    for (int kt = 0; kt < 2; ++kt)
+                    for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            raw[2 * q + kt][i] = make_uint4(0u, 0u, 0u, 0u);
-                            if (key0 < len) raw[2 * q + kt][i] = ldg_stream_u4(src + (int64_t)(8 * kt) * p.c.sc_t + 64 * i);
-                        }
+                        for (int i = 0; i < 2; ++i)
+                            raw[q][h][i] = *reinterpret_cast<const uint4*>(kt + h * 8 * kD +
+                                                                           (((uint32_t)(2 * t + i) << 4) ^ ((uint32_t)(g & 7) << 4)));
+                    sk[q] = s_scale[st][(32 * warp + 16 * q) >> p.c.page_shift];
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s_empty[st]);
+                if (warp == 0 && next < t1) produce();
+                if (key0 >= len) continue;
+                uint32_t a[2][8][4];
 #pragma unroll
-                for (int kt = 0; kt < 4; ++kt) {
-                    const uint32_t w[8] = {raw[kt][0].x, raw[kt][0].y, raw[kt][0].z, raw[kt][0].w,
-                                           raw[kt][1].x, raw[kt][1].y, raw[kt][1].z, raw[kt][1].w};
-#pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) halves<FP8>(w[ks], kb[kt][ks][0], kb[kt][ks][1]);
-                }
-                float sum[2] = {0.f, 0.f};
-                const int key = task * 32 + 2 * t;  // this lane's tokens: key, key + 1 of every 8-token tile
-                for (int tl = 0; tl < tiles; ++tl) {
-                    float acc[4][4];
-#pragma unroll
-                    for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[kt][e] = 0.f;
-#pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) {
-                        const uint4 a = s_q[tl][ks][lane];
-#pragma unroll
-                        for (int kt = 0; kt < 4; ++kt) mma_f16(acc[kt], a.x, a.y, a.z, a.w, kb[kt][ks][0], kb[kt][ks][1]);
-                    }
+                for (int q = 0; q < 2; ++q)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const float rf = s_rf[tl * 16 + g + 8 * h], nl = s_lse[tl * 16 + g + 8 * h];
+                        const uint32_t w[8] = {raw[q][h][0].x, raw[q][h][0].y, raw[q][h][0].z, raw[q][h][0].w,
+                                               raw[q][h][1].x, raw[q][h][1].y, raw[q][h][1].z, raw[q][h][1].w};
 #pragma unroll
-                        for (int kt = 0; kt < 4; ++kt)
+                        for (int ks = 0; ks < 8; ++ks) halves<FP8>(w[ks], a[q][ks][h], a[q][ks][2 + h]);
+                    }
+                float sum[2] = {0.f, 0.f};
+                const bool tail = key0 + 32 > len;
+#pragma unroll 1
+                for (int rt = 0; rt < row_tiles; ++rt) {
+                    float acc[2][4];
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const float w = fast_exp2(fmaf(acc[kt][2 * h + e], rf * sk[kt >> 1], nl));
-                                sum[kt >> 1] += key + 8 * kt + e < len ? w : 0.f;
-                            }
+                    for (int q = 0; q < 2; ++q)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[q][e] = 0.f;
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks) {
+                        const uint2 x = s_q[rt][ks][lane];
+#pragma unroll
+                        for (int q = 0; q < 2; ++q)
+                            mma_f16(acc[q], a[q][ks][0], a[q][ks][1], a[q][ks][2], a[q][ks][3], x.x, x.y);
+                    }
+                    const float4 f = *reinterpret_cast<const float4*>(&s_row[rt][2 * t]);  // rows 2 t and 2 t + 1
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const float fx = f.x * sk[q], fz = f.z * sk[q];
+                        float w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            w[e] = fast_exp2(fmaf(acc[q][e], (e & 1) ? fz : fx, (e & 1) ? f.w : f.y));
+                        if (tail) {
+                            if (key0 + 16 * q + g >= len) w[0] = w[1] = 0.f;
+                            if (key0 + 16 * q + g + 8 >= len) w[2] = w[3] = 0.f;
+                        }
+                        sum[q] += (w[0] + w[1]) + (w[2] + w[3]);
                     }
                 }
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-#pragma unroll
+#pragma unroll 1
                     for (int d = 16; d; d >>= 1) sum[q] += __shfl_xor_sync(MFD_FULL_MASK, sum[q], d);
-                    if (lane == 0 && task * 32 + 16 * q < len) {
-                        float* dst = part + (int64_t)(2 * task + q) * Hkv;
+                    if (lane == 0 && key0 + 16 * q < len) {
+                        float* dst = part + (int64_t)((key0 >> 4) + q) * Hkv;
                         *dst = r0 == 0 ? sum[q] : *dst + sum[q];
                     }
                 }
             }
+            if (!ok)
+                for (int i = tid; i < (t1 - t0) * (kWTile / 16); i += kWThreads)
+                    if ((t0 * kWTile + 16 * i) < len) part[(int64_t)(t0 * (kWTile / 16) + i) * Hkv] = NAN;
+            if (!ok && warp == 0)  // copies in flight end before the CTA does (bounded)
+                for (uint32_t f = n_tile + next - t0, i = f > kWStages ? f - kWStages : 0u; i < f; ++i)
+                    mbar_wait(&s_full[i % kWStages], (i / kWStages) & 1, 1u << 14);
+            n_tile += t1 - t0;
+            ok = __syncthreads_and(ok);  // the staged rows are done with
+            if (!ok) break;
         }
         pos += t1 - t0;
         // ---- the request's last CTA adds up its pages
-        if (pos >= end || pos >= before + tasks * Hkv) {
-            const int pieces = quotient(before + tasks * Hkv - 1, per) - quotient(before, per) + 1;
+        if (pos >= end || pos >= before + tiles * Hkv) {
+            const int pieces = quotient(before + tiles * Hkv - 1, per) - quotient(before, per) + 1;
             __threadfence();
             __syncthreads();
             if (tid == 0) s_last = pieces == 1 || atomicAdd(p.tickets + b, 1u) == (unsigned)(pieces - 1);
@@ -213,6 +286,7 @@ __global__ void __launch_bounds__(kWThreads, kWCtasPerSm) kv8_weights_kernel(con
                 if (tid == 0 && pieces > 1) p.tickets[b] = 0u;
             }
         }
+        if (!ok) return;
     }
 }
 
@@ -263,7 +337,7 @@ extern "C" int mfd_kv8_page_weights(const void* q, int64_t sq_b, int64_t sq_n, i
         set_error("%s: workspace or tickets too small", who);
         return MFD_ERR_INVALID;
     }
-    if (!kv8::work_fits(bs, num_kv_heads, max_pages, page_size, 32)) {
+    if (!kv8::work_fits(bs, num_kv_heads, max_pages, page_size, 256)) {
         set_error("%s: the requests' capacity is beyond this build's limits", who);
         return MFD_ERR_UNSUPPORTED;
     }
@@ -288,8 +362,22 @@ extern "C" int mfd_kv8_page_weights(const void* q, int64_t sq_b, int64_t sq_n, i
     p.groups_max = (int)(max_pages * (page_size / 16));
     p.tickets = tickets;
     const int grid = kv8::sm_count() * kv8::kWCtasPerSm;
-    if (code_dtype == MFD_E4M3) kv8::kv8_weights_kernel<true><<<grid, kv8::kWThreads, 0, (cudaStream_t)stream>>>(p);
-    else kv8::kv8_weights_kernel<false><<<grid, kv8::kWThreads, 0, (cudaStream_t)stream>>>(p);
+    constexpr int kSmem = kv8::kWStages * kv8::kWStageBytes + kv8::kWRowTiles * 8 * 32 * 8 + 1024;
+    CUtensorMap tk;
+    if (!kv8::make_page_map(&tk, p.c.k, p.c, true)) {
+        set_error("%s: could not encode the TMA tensor map", who);
+        return MFD_ERR_CUDA;
+    }
+    static bool opted[2][64];
+    const bool fp8 = code_dtype == MFD_E4M3;
+    const void* kernel = fp8 ? (const void*)kv8::kv8_weights_kernel<true> : (const void*)kv8::kv8_weights_kernel<false>;
+    cudaError_t e = kv8::opt_in_smem(kernel, kSmem, opted[fp8]);
+    if (e != cudaSuccess) {
+        set_error("%s: %s", who, cudaGetErrorString(e));
+        return MFD_ERR_CUDA;
+    }
+    if (fp8) kv8::kv8_weights_kernel<true><<<grid, kv8::kWThreads, kSmem, (cudaStream_t)stream>>>(tk, p);
+    else kv8::kv8_weights_kernel<false><<<grid, kv8::kWThreads, kSmem, (cudaStream_t)stream>>>(tk, p);
     MFD_CHECK_LAUNCH(who);
     return MFD_OK;
 }
