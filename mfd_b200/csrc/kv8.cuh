@@ -151,6 +151,19 @@ __device__ __forceinline__ uint4 ldg_stream_u4(const void* p) {
     return r;
 }
 
+// One asynchronous 16-byte copy into shared memory, and the groups they are waited for in.
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {  // all but the last N groups have landed
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// Where a warp keeps rows of 128 codes in shared memory: 16-byte chunk c of row r.  The eight lanes of a 16-byte access
+// that read chunks 2 t (+ 1) of two neighbouring rows, or one chunk of every other row, hit eight different bank groups.
+__device__ __forceinline__ int chunk_at(int r, int c) { return r * kD + ((c ^ (r & 7)) << 4); }
+
 // Rows a request lists: counts[b] (or `rows`), cut at the first path entry outside [0, n).  Called by whole warps.
 __device__ __forceinline__ int listed_rows(const int64_t* path, int64_t path_stride, int rows, const int32_t* counts,
                                            int n, int b) {

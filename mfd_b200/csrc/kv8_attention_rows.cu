@@ -17,18 +17,16 @@
 //   values   m16n8k16: A = 16 columns of the values x 16 keys, B = the weights (the scores' registers transposed by
 //            movmatrix); lane (g, t) holds d = 16 g .. 16 g + 15 of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 and interleaves
 //            the bytes of two keys before they become float16 pairs; column tile j is d = 16 g + 2 j and the next
-// Tiles of 128 keys come by TMA, a page a copy, into a ring of three 32 KB stages (two CTAs an SM: 192 KB in flight; loads
-// straight to registers kept too few bytes in flight and reached half the bandwidth).  The 128-byte swizzle of the copies
-// makes both register layouts' 16-byte shared-memory loads free of bank conflicts.  Warp 0 issues the copies of the tile two
-// ahead (a ninth warp would cost every thread a quarter of its registers).  The 8 warps take 16 keys of every tile each
-// (one page has all 16: one scale), with their own (m, l, O), and merge in shared memory at the end of the piece.
+// A warp takes every eighth group of 16 keys (one page has all 16: one scale), with its own (m, l, O), and copies its codes
+// itself, asynchronously, two groups ahead into a ring of its own in shared memory (8 warps x 3 x 4 KB, two CTAs an SM:
+// 128 KB in flight; loads straight to registers kept too few bytes in flight).  Nothing in the loop waits for another
+// warp.  TMA copies of whole pages ran no faster, and encoding their two tensor maps cost every call 4 us on the host.
+// The warps merge in shared memory at the end of the piece.
 //
 // Split: the tiles of all (request, KV head, 16 rows) units are laid end to end and cut into equal pieces, one per CTA, so
 // ragged lengths balance and one long request fills the GPU; the lengths are read on the device.  The nodes' own keys
 // belong to a unit's last piece.  A unit cut into pieces is merged by the CTA that finishes last (its partial (m, l, O) in
 // the workspace, a ticket per unit; the pieces are added in their order, so the result does not depend on who merges).
-//
-// Every mbarrier wait is bounded; a CTA whose wait gave up records status 1 and stops.
 #include "kv8_attention.cuh"
 #include "tcgen05.cuh"
 
@@ -37,10 +35,10 @@ namespace kv8 {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kTile = 128;             // keys a stage
+constexpr int kTile = 16 * kWarps;       // keys the warps take side by side
 constexpr int kStages = 3;
-constexpr int kStageBytes = 2 * kTile * kD;  // K, then V
-constexpr uint32_t kTries = 1u << 20;
+constexpr int kStageBytes = 2 * 16 * kD;  // of a warp: 16 rows of K, then of V
+constexpr int kRingBytes = kWarps * kStages * kStageBytes;
 // floats: a lane's 16 columns, padded so that the 8 lanes of a store hit different banks
 constexpr int kDBlock = 20, kRowStride = 8 * kDBlock + 4;
 constexpr int kSlot = 16 * (kD + 2);  // floats of a partial: m[16], l[16], O[16][128]
@@ -52,28 +50,17 @@ constexpr int kMaxOwn = kRowsMaxOwn;  // own keys a request
 // NT: 8-row tiles a unit
 template <bool FP8, int NT>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)
-    kv8_rows_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const AttnParams p) {
+    kv8_rows_kernel(const AttnParams p) {
     constexpr int kRows = 8 * NT;
-    // the ring; at a piece's end [kWarps][kRows][kRowStride] floats, then the merge weights
-    extern __shared__ __align__(16) unsigned char smem_raw[];
-    unsigned char* ring = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
+    // the warps' rings; at a piece's end [kWarps][kRows][kRowStride] floats, then the merge weights
+    extern __shared__ __align__(128) unsigned char ring[];
     float* smem = reinterpret_cast<float*>(ring);
-    __shared__ float2 s_scale[kStages][8];     // of the tile's pages: K scale, V scale
     __shared__ float s_own[kRows][kMaxOwn];    // scores of the nodes' own keys (log2), -inf where not visible
     __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows], s_mm[kRows], s_ll[kRows];
     __shared__ uint2 s_q[NT][8][32];  // query operands, the same for every warp (in registers they would spill)
-    __shared__ uint64_t s_full[kStages], s_empty[kStages];
-    __shared__ int s_last, s_failed;
+    __shared__ int s_last;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
-    if (tid == 0) {
-        for (int i = 0; i < kStages; ++i) {
-            mbar_init(&s_full[i], 32);
-            mbar_init(&s_empty[i], kWarps);
-        }
-        s_failed = 0;
-        mbar_fence_init();
-    }
     const int nrows = p.rows - p.row0;
     const int RB = (nrows + 15) / 16;
     // ---- this CTA's share of the work, in tiles
@@ -82,69 +69,40 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     const Cut cut = make_cut(lens, tiles_of, p.c.Hkv * RB, gridDim.x);
     int pos, end;
     cut_range(cut, blockIdx.x, pos, end);
-    __syncthreads();
 
     Piece pc;
-    uint32_t n_tile = 0;  // tiles of the CTA's earlier pieces: the barriers' phases
-    bool ok = true;
     while (next_piece(lens, tiles_of, cut, blockIdx.x, pos, end, pc)) {
         const int hk = pc.u / RB, rb = pc.u % RB, len = pc.len;
         const int base = p.row0 + rb * 16;
 
-        // ---- the producer, warp 0: copies of a tile, then its constants.  Page ids are read two tiles ahead and scales
-        // one, so it waits for neither; a stage is free once every warp has read its codes, two tiles before.
-        const int ppt = kTile >> p.c.page_shift;
-        int next = pc.g0, id0 = -1, id1 = -1;  // the next tile to fetch, the page ids of it and of the one after
-        float2 sc = make_float2(0.f, 0.f);     // scales of tile `next`
-        auto id_of = [&](int tile) {           // lane j < ppt takes page j of a tile
-            const int pg = tile * ppt + lane;
-            return lane < ppt && tile < pc.g1 && (pg << p.c.page_shift) < len ? page_id(p.c, pc.b, pg) : -1;
-        };
-        auto scales = [&](int id) {
-            return id < 0 ? make_float2(0.f, 0.f) : make_float2(__ldg(p.c.k_scale + (int64_t)id * p.c.Hkv + hk),
-                                                                __ldg(p.c.v_scale + (int64_t)id * p.c.Hkv + hk));
-        };
-        auto copies = [&](uint32_t nt, int id) {
-            const uint32_t st = nt % kStages;
-            if (id >= 0) {
-                const uint32_t half = (uint32_t)(p.c.page * kD), dst = smem_addr(ring) + st * kStageBytes + lane * half;
-                mbar_expect_tx(&s_full[st], 2 * half);
-                tma_page(dst, &tmk, &s_full[st], hk, id);
-                tma_page(dst + kStageBytes / 2, &tmv, &s_full[st], hk, id);
+        // ---- this warp's copies: lane l takes chunk l % 8 of rows l / 8 + 4 i; the page id is read a tile ahead, the scales
+        // with the copies, two tiles before they are used
+        unsigned char* mine = ring + warp * (kStages * kStageBytes);
+        const int64_t lane_off = (int64_t)hk * p.c.sc_h + (int64_t)(lane >> 3) * p.c.sc_t + (lane & 7) * 16;
+        auto key_of = [&](int tile) { return tile * kTile + 16 * warp; };
+        auto inside = [&](int tile) { return tile < pc.g1 && key_of(tile) < len; };
+        auto id_of = [&](int tile) { return inside(tile) ? page_id(p.c, pc.b, key_of(tile) >> p.c.page_shift) : 0; };
+        float2 sc0 = make_float2(0.f, 1.f), sc1 = sc0, sc2 = sc0;  // scales of this tile and of the next two
+        auto fetch = [&](int tile, int id) {
+            float2 sc = make_float2(0.f, 1.f);
+            if (inside(tile)) {
+                const int64_t off = (int64_t)id * p.c.sc_p + (int64_t)(key_of(tile) & (p.c.page - 1)) * p.c.sc_t + lane_off;
+                unsigned char* dst = mine + (tile - pc.g0) % kStages * kStageBytes;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = (lane >> 3) + 4 * i;
+                    copy16(dst + chunk_at(r, lane & 7), p.c.k + off + (int64_t)(4 * i) * p.c.sc_t);
+                    copy16(dst + 16 * kD + chunk_at(r, lane & 7), p.c.v + off + (int64_t)(4 * i) * p.c.sc_t);
+                }
+                sc = make_float2(__ldg(p.c.k_scale + (int64_t)id * p.c.Hkv + hk), __ldg(p.c.v_scale + (int64_t)id * p.c.Hkv + hk));
             }
+            copies_commit();
+            return sc;
         };
-        auto constants = [&](uint32_t nt, int id, float2 s) {
-            const uint32_t st = nt % kStages;
-            if (id >= 0) s_scale[st][lane] = s;
-            __syncwarp();  // lanes without a page (8 .. 31 never have one) arrive last, after every scale is stored
-            if (id < 0) mbar_arrive(&s_full[st]);
-        };
-        if (warp == 0) {  // the first two tiles: both ids, both tiles' copies, both tiles' scales (the stages are free)
-            id0 = id_of(next);
-            id1 = id_of(next + 1);
-            const int id2 = id_of(next + 2);
-            copies(n_tile, id0);
-            if (next + 1 < pc.g1) copies(n_tile + 1, id1);
-            const float2 s0 = scales(id0), s1 = scales(id1);
-            sc = scales(id2);
-            constants(n_tile, id0, s0);
-            if (next + 1 < pc.g1) constants(n_tile + 1, id1, s1);
-            next += 2;
-            id0 = id2;
-            id1 = id_of(next + 1);
-        }
-        auto produce = [&]() {
-            const uint32_t nt = n_tile + next - pc.g0;
-            if (nt >= (uint32_t)kStages)
-                ok = __all_sync(MFD_FULL_MASK, ok & mbar_wait(&s_empty[nt % kStages], (nt / kStages - 1) & 1, kTries));
-            if (!ok) return;
-            copies(nt, id0);
-            constants(nt, id0, sc);
-            ++next;
-            id0 = id1;
-            sc = scales(id0);
-            id1 = id_of(next + 1);
-        };
+        int id = id_of(pc.g0), id_next = id_of(pc.g0 + 1);
+        sc0 = fetch(pc.g0, id);
+        id = id_of(pc.g0 + 2);
+        sc1 = fetch(pc.g0 + 1, id_next);
 
         // ---- query row g (+ 8 nt) as float16 operands, divided by a power of two; the lane's softmax rows are 2 t, 2 t + 1
         float rf[NT][2];  // score factor of rows 2 t and 2 t + 1: the power of two, the scale and log2(e)
@@ -182,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                 for (int j = 0; j < 2; ++j) {
                     const float2 f0 = bf2(w[2 * j]), f1 = bf2(w[2 * j + 1]);
                     const int ks = 2 * i + j;
-                    if (warp == 1)  // (warp 0 has the copies)
+                    if (warp == 0)
                         s_q[n][ks][lane] = make_uint2(pack_half2(f0.x * down, f0.y * down), pack_half2(f1.x * down, f1.y * down));
                 }
             }
@@ -283,29 +241,25 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         }
 
         // ---- cached tokens
-        const uint32_t swk = (uint32_t)(g & 7) << 4;
 #pragma unroll 1
         for (int tile = pc.g0; tile < pc.g1; ++tile) {
-            if (warp == 0 && next < pc.g1) produce();
-            const uint32_t nt = n_tile + tile - pc.g0, st = nt % kStages;
-            ok = __all_sync(MFD_FULL_MASK, ok & mbar_wait(&s_full[st], (nt / kStages) & 1, kTries));
-            if (!ok) break;
-            const int key0 = tile * kTile + 16 * warp;
-            if (key0 >= len) {  // (a tile's last warps, behind the request's end)
-                if (lane == 0) mbar_arrive(&s_empty[st]);
-                continue;
-            }
+            __syncwarp();  // (every lane has read the stage that the copies below overwrite)
+            sc2 = fetch(tile + 2, id);
+            id = id_of(tile + 3);
+            copies_wait<2>();
+            __syncwarp();
+            const int key0 = key_of(tile);
+            if (key0 >= len) break;
             const bool tail = key0 + 16 > len;
-            const unsigned char* kt = ring + st * kStageBytes + (16 * warp + g) * kD;  // key g's row; g + 8: 1 KB on
-            const unsigned char* vt = ring + st * kStageBytes + kStageBytes / 2 + (16 * warp + 2 * t) * kD;
+            const unsigned char* kt = mine + (tile - pc.g0) % kStages * kStageBytes;
             uint4 kw[2][2], vw[4];  // K: key g, g + 8; chunk 2 t, 2 t + 1.  V: keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    kw[h][i] = *reinterpret_cast<const uint4*>(kt + h * 8 * kD + (((uint32_t)(2 * t + i) << 4) ^ swk));
-            const float2 scale = s_scale[st][(16 * warp) >> p.c.page_shift];
-            const float sv = fmaxf(scale.y, kScaleFloor), lsv = __log2f(sv);
+                    kw[h][i] = *reinterpret_cast<const uint4*>(kt + chunk_at(g + 8 * h, 2 * t + i));
+            const float sv = fmaxf(sc0.y, kScaleFloor), lsv = __log2f(sv), skc = sc0.x;
+            sc0 = sc1, sc1 = sc2;
             float acc[NT][4], acc2[NT][4];  // two chains: the instruction's latency is several times its issue
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -326,15 +280,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = 2 * t + (i & 1);
-                vw[i] = *reinterpret_cast<const uint4*>(vt + ((i & 1) + 8 * (i >> 1)) * kD + ((uint32_t)(g ^ r) << 4));
-            }
+            for (int i = 0; i < 4; ++i)
+                vw[i] = *reinterpret_cast<const uint4*>(kt + 16 * kD + chunk_at(2 * t + (i & 1) + 8 * (i >> 1), g));
             float w[NT][4];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[n][e] = fmaf(acc[n][e] + acc2[n][e], scale.x * rf[n][e & 1], lsv);
+                for (int e = 0; e < 4; ++e) w[n][e] = fmaf(acc[n][e] + acc2[n][e], skc * rf[n][e & 1], lsv);
             if (tail) {  // slots past the length hold any bits (an e4m3 NaN too): their weight is 0, their codes too
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
@@ -345,8 +297,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                 for (int i = 0; i < 4; ++i)
                     if (key0 + 2 * t + (i & 1) + 8 * (i >> 1) >= len) vw[i] = make_uint4(0u, 0u, 0u, 0u);
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s_empty[st]);  // every lane has its codes
             step(w, __frcp_rn(sv));
             uint32_t hi[NT][2], lo[NT][2];  // keys 0 .. 7 and 8 .. 15: B operands
 #pragma unroll
@@ -377,6 +327,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             }
         }
 
+        copies_wait<0>();
         // ---- the warps of the piece merge: O as it is in shared memory, their weights per row beside it
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -510,17 +461,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                 if (tid == 0) *ticket = 0u;
             }
         }
-        if (!ok && warp == 0)  // copies in flight end before the CTA does (bounded)
-            for (uint32_t f = n_tile + next - pc.g0, i = f > kStages ? f - kStages : 0u; i < f; ++i)
-                mbar_wait(&s_full[i % kStages], (i / kStages) & 1, 1u << 14);
-        fence_proxy_async_smem();  // (the next piece's copies land where the merge was)
-        n_tile += pc.g1 - pc.g0;
-        if (!ok) atomicExch(&s_failed, 1);
         __syncthreads();  // smem, s_m and s_l are free for the next piece
-        if (*(volatile int*)&s_failed) {
-            if (tid == 0) atomicExch(p.status, 1);
-            break;
-        }
     }
 }
 
@@ -529,21 +470,14 @@ size_t rows_workspace(int sms) { return (size_t)sms * kCtasPerSm * 2 * kSlot * s
 
 template <bool FP8, int NT>
 static int launch_one(const AttnParams& p, int sms, cudaStream_t stream) {
-    constexpr int kSmem = kStages * kStageBytes + 1024;
-    static_assert(kWarps * 8 * NT * kRowStride * 4 <= kStages * kStageBytes && 512 * 16 * 4 <= kStages * kStageBytes,
-                  "the merge fits the ring");
-    CUtensorMap tk, tv;
-    if (!make_page_map(&tk, p.c.k, p.c, true) || !make_page_map(&tv, p.c.v, p.c, true)) {
-        set_error("mfd_kv8_attention: could not encode the TMA tensor maps");
-        return MFD_ERR_CUDA;
-    }
+    static_assert(kWarps * 8 * NT * kRowStride * 4 <= kRingBytes && 512 * 16 * 4 <= kRingBytes, "the merge fits the ring");
     static bool opted[64];
-    cudaError_t e = opt_in_smem((const void*)kv8_rows_kernel<FP8, NT>, kSmem, opted);
+    cudaError_t e = opt_in_smem((const void*)kv8_rows_kernel<FP8, NT>, kRingBytes, opted);
     if (e != cudaSuccess) {
         set_error("mfd_kv8_attention: %s", cudaGetErrorString(e));
         return MFD_ERR_CUDA;
     }
-    kv8_rows_kernel<FP8, NT><<<sms * kCtasPerSm, kThreads, kSmem, stream>>>(tk, tv, p);
+    kv8_rows_kernel<FP8, NT><<<sms * kCtasPerSm, kThreads, kRingBytes, stream>>>(p);
     MFD_CHECK_LAUNCH("mfd_kv8_attention");
     return MFD_OK;
 }

@@ -601,12 +601,14 @@ def _kv8_check(what: str, k_cache, v_cache, k_scale, v_scale, page_table, seq_le
         raise RuntimeError(f"{what}: cache codes must be int8 or float8_e4m3fn, got {k_cache.dtype}")
     if len(shape) != 4 or strides[3] != 1:
         raise RuntimeError(f"{what}: caches must be [pages, KV heads, page_size, D] with a contiguous last dim")
-    if v_cache is not k_cache and (v_cache.shape != shape or v_cache.dtype != k_cache.dtype
-                                   or v_cache.stride() != strides):
+    if v_cache is not None and (v_cache.shape != shape or v_cache.dtype != k_cache.dtype
+                                or v_cache.stride() != strides):
         raise RuntimeError(f"{what}: k_cache and v_cache need the same dtype, shape and strides")
-    for s in (k_scale, v_scale) if v_scale is not k_scale else (k_scale,):
-        if s.dtype != torch.float32 or s.shape != shape[:2] or not s.is_contiguous():
-            raise RuntimeError(f"{what}: scales must be contiguous float32 [pages, KV heads]")
+    pages = shape[:2]
+    if (k_scale.dtype != torch.float32 or k_scale.shape != pages or not k_scale.is_contiguous()
+            or (v_scale is not None and (v_scale.dtype != torch.float32 or v_scale.shape != pages
+                                         or not v_scale.is_contiguous()))):
+        raise RuntimeError(f"{what}: scales must be contiguous float32 [pages, KV heads]")
     if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1:
         raise RuntimeError(f"{what}: page_table must be int32 [bs, max_pages] with a contiguous last dim")
     if seq_lens.dtype != torch.int32 or seq_lens.shape != page_table.shape[:1] or not seq_lens.is_contiguous():
@@ -626,8 +628,8 @@ def _kv8_rows(what: str, rows: torch.Tensor, name: str, shape):
 
 def _kv8_new(what: str, k_new: torch.Tensor, v_new: torch.Tensor, shape):
     strides = _kv8_rows(what, k_new, "k_new", shape)
-    if _kv8_rows(what, v_new, "v_new", shape) != strides:
-        raise RuntimeError(f"{what}: k_new and v_new need the same strides")
+    if v_new.stride() != strides or v_new.shape != shape or v_new.dtype != torch.bfloat16:
+        raise RuntimeError(f"{what}: v_new must be bfloat16 {tuple(shape)} with the strides of k_new")
     return strides
 
 
@@ -670,14 +672,24 @@ def kv8_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tens
     return new_lens
 
 
-_KV8_WORK: dict = {}
+_KV8_SIZES: dict = {}
 
 
-def _kv8_scratch(dev: torch.device, stream: int, purpose: str, nbytes: int, tickets: int):
-    """Workspace and zeroed ticket words of one stream: calls on different streams may overlap on the GPU, so the
-    operators of the 8-bit cache share neither between streams."""
-    return (Workspace.get(dev, (purpose, stream), nbytes),
-            Workspace.get(dev, (purpose, "tickets", stream), 4 * tickets))
+def _kv8_scratch(dev: torch.device, stream: int, purpose: str, sizes: tuple, size_of):
+    """(workspace, its bytes, ticket words, their number) of one stream, as addresses: calls on different streams may
+    overlap on the GPU, so the operators of the 8-bit cache share no scratch between streams.  size_of() -> (bytes,
+    tickets) is asked once for each tuple of sizes."""
+    key = (purpose, dev.index, *sizes)
+    need = _KV8_SIZES.get(key)
+    if need is None:
+        with torch.cuda.device(dev):
+            need = size_of()
+        if len(_KV8_SIZES) >= 4096:
+            _KV8_SIZES.clear()
+        _KV8_SIZES[key] = need
+    ws = Workspace.get(dev, (purpose, stream), need[0])
+    tk = Workspace.get(dev, (purpose, "tickets", stream), 4 * need[1])
+    return ws.data_ptr(), ws.numel(), tk.data_ptr(), tk.numel() // 4
 
 
 def kv8_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -711,24 +723,22 @@ def kv8_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
         ab, words = anc.data_ptr(), anc.shape[2]
     if out is None:
         out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
-    so = _kv8_rows("kv8_attention", out, "out", shape)
-    lse = torch.empty(shape[:3], dtype=torch.float32, device=q.device) if return_lse else None
+        so = (n * H * d, H * d, d)
+    else:
+        so = _kv8_rows("kv8_attention", out, "out", shape)
+    lse, lse_ptr = None, None
+    if return_lse:
+        lse = torch.empty((bs, n, H), dtype=torch.float32, device=q.device)
+        lse_ptr = lse.data_ptr()
     L = _lib.lib()
-    key = (dev, bs, n, H, hkv)
-    need = _KV8_WORK.get(key)
-    if need is None:
-        with torch.cuda.device(dev):
-            need = (L.mfd_kv8_attention_workspace(bs, n, H, hkv), L.mfd_kv8_attention_tickets(bs, n, H, hkv))
-        if len(_KV8_WORK) >= 4096:
-            _KV8_WORK.clear()
-        _KV8_WORK[key] = need
     stream = raw_stream(dev)
-    ws, tk = _kv8_scratch(q.device, stream, "kv8_attn", *need)
+    scratch = _kv8_scratch(q.device, stream, "kv8_attn", (bs, n, H, hkv),
+                           lambda: (L.mfd_kv8_attention_workspace(bs, n, H, hkv),
+                                    L.mfd_kv8_attention_tickets(bs, n, H, hkv)))
     rc = L.mfd_kv8_attention(q.data_ptr(), sq[0], sq[1], sq[2], k_cache.data_ptr(), v_cache.data_ptr(), sc[0], sc[1],
                              sc[2], code, k_scale.data_ptr(), v_scale.data_ptr(), pages, page, page_table.data_ptr(),
                              page_table.stride(0), width, seq_lens.data_ptr(), kn, vn, sn[0], sn[1], sn[2], ab, words,
-                             bs, n, H, hkv, d, scale, out.data_ptr(), so[0], so[1], so[2], ptr(lse), ws.data_ptr(),
-                             ws.numel(), tk.data_ptr(), tk.numel() // 4, stream)
+                             bs, n, H, hkv, d, scale, out.data_ptr(), so[0], so[1], so[2], lse_ptr, *scratch, stream)
     check(rc, "mfd_kv8_attention")
     return (out, lse) if return_lse else out
 
@@ -754,7 +764,7 @@ def kv8_page_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, 
     the page's tokens; 0 past a request's pages.  lse f32 [bs, n, H] from kv8_attention on the same cache (before the
     nodes are appended); mass f32 [bs, max_pages]; out may be mass.  The sums run in a fixed order."""
     dev = device_index(q, lse, k_cache, k_scale, page_table, seq_lens, mass, path, counts, out)
-    (pages, hkv, page, d), sc, code = _kv8_check("kv8_page_weights", k_cache, k_cache, k_scale, k_scale, page_table,
+    (pages, hkv, page, d), sc, code = _kv8_check("kv8_page_weights", k_cache, None, k_scale, None, page_table,
                                                  seq_lens)
     table_shape = page_table.shape
     bs, width = table_shape
@@ -774,12 +784,13 @@ def kv8_page_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, 
         raise RuntimeError("kv8_page_weights: out must be contiguous float32 [bs, max_pages]")
     L = _lib.lib()
     stream = raw_stream(dev)
-    ws, tk = _kv8_scratch(q.device, stream, "kv8_weights", L.mfd_kv8_page_weights_workspace(bs, width, page, hkv), bs)
+    scratch = _kv8_scratch(q.device, stream, "kv8_weights", (bs, width, page, hkv),
+                           lambda: (L.mfd_kv8_page_weights_workspace(bs, width, page, hkv), bs))
     rc = L.mfd_kv8_page_weights(q.data_ptr(), sq[0], sq[1], sq[2], lse.data_ptr(), k_cache.data_ptr(), sc[0], sc[1],
                                 sc[2], code, k_scale.data_ptr(), pages, page, page_table.data_ptr(),
                                 page_table.stride(0), width, seq_lens.data_ptr(), ptr(path), path_stride, rows,
-                                ptr(counts), bs, n, H, hkv, d, scale, decay, mass.data_ptr(), out.data_ptr(), width,
-                                ws.data_ptr(), ws.numel(), tk.data_ptr(), tk.numel() // 4, stream)
+                                ptr(counts), bs, n, H, hkv, d, scale, decay, mass.data_ptr(), out.data_ptr(), width, *scratch,
+                                stream)
     check(rc, "mfd_kv8_page_weights")
     return out
 
