@@ -211,8 +211,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int node = live ? row / p.G : 0;
             const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
             const uint32_t s_tm = tmem + lane_off + 256 + 128 * grp, o_tm = tmem + lane_off + 128 * grp;
-            float m = -INFINITY, l = 0.f;
+            // O and l are relative to 2^m; m_next is what m should be (the tiles' maxima).  A tile's weights are formed
+            // in one pass against the m of the tiles before it, which bf16's range allows: m only follows when the
+            // maximum has passed it by 2^8, before the next tile, and at once where a chunk passes it by 2^60.
+            float m = -INFINITY, m_next = -INFINITY, l = 0.f;
             int done = 0;  // steps of this group
+            auto rescale_o = [&](float alpha) {  // (S of this step is there, so the group's last product is complete)
+#pragma unroll 1
+                for (int oc = 0; oc < kD; oc += 32) {
+                    float o[32];
+                    tmem_ld32(o_tm + oc, o);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) o[j] *= alpha;
+                    tmem_st32(o_tm + oc, o);
+                }
+            };
             for (int s = grp; s < x.nsteps; s += 2, ++done) {
                 const int tile = pc.g0 + (x.alternate ? s : s >> 1);
                 ok = __all_sync(MFD_FULL_MASK, ok & mbar_wait(&bars[L::kSFull + grp], ((grp ? x.n_s1 : x.n_s0) + done) & 1, kTries));
@@ -228,9 +241,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         const uint64_t v = live ? visible_word(p, pc.b, node, 2 * (tile - x.tp) + (c >> 1)) : 0ull;
                         return (uint32_t)(v >> (32 * (c & 1)));
                     };
-                    float mx = -INFINITY;
+                    const bool behind = m_next > m + 8.f;
+                    if (__any_sync(MFD_FULL_MASK, behind)) {
+                        const float alpha = behind ? fast_exp2(m - m_next) : 1.f;  // (m is finite: see below)
+                        if (behind) m = m_next;
+                        l *= alpha;
+                        rescale_o(alpha);
+                    }
+                    uint64_t acc[2] = {0ull, 0ull};
 #pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {  // (rolled: the unrolled step misses the instruction cache)
+                    for (int c = 0; c < 4; ++c) {  // (rolled: an unrolled step misses the instruction cache)
                         uint32_t u[1][32];
                         tmem_ld32_issue(s_tm + 32 * c, u[0]);
                         tmem_ld_wait(u);
@@ -240,42 +260,50 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             for (int j = 0; j < 32; ++j)
                                 if (!((vis >> j) & 1u)) u[0][j] = 0xff800000u;
                         }
+                        const float4 k0 = cst[2 * c], k1 = cst[2 * c + 1];  // of 16 keys: one page
+                        float top[2];
 #pragma unroll
-                        for (int q = 0; q < 2; ++q) {  // 16 keys: one page
+                        for (int q = 0; q < 2; ++q) {
                             float a[6];
 #pragma unroll
                             for (int j = 0; j < 5; ++j)
                                 a[j] = fmax3(__uint_as_float(u[0][16 * q + 3 * j]), __uint_as_float(u[0][16 * q + 3 * j + 1]),
                                              __uint_as_float(u[0][16 * q + 3 * j + 2]));
                             a[5] = __uint_as_float(u[0][16 * q + 15]);
-                            const float top = fmaxf(fmax3(a[0], a[1], a[2]), fmax3(a[3], a[4], a[5]));
-                            const float2 k = *reinterpret_cast<const float2*>(cst + 2 * c + q);
-                            mx = fmaxf(mx, top == -INFINITY ? top : fmaf(top, k.x, k.y));
+                            top[q] = fmaxf(fmax3(a[0], a[1], a[2]), fmax3(a[3], a[4], a[5]));
                         }
-                    }
-                    float alpha = 1.f;
-                    bool rescale = false;
-                    if (mx > m + 8.f) {  // lazy: the running reference moves only when the maximum passes it by 2^8
-                        if (m != -INFINITY) alpha = fast_exp2(m - mx), rescale = true;
-                        m = mx;
-                    }
-                    const float mr = m == -INFINITY ? 0.f : m;
-                    uint64_t acc[2] = {0ull, 0ull};
+                        const float mx = fmaxf(top[0] == -INFINITY ? top[0] : fmaf(top[0], k0.x, k0.y),
+                                               top[1] == -INFINITY ? top[1] : fmaf(top[1], k1.x, k1.y));
+                        m_next = fmaxf(m_next, mx);
+                        const bool far = mx > m + 60.f;
+                        if (__any_sync(MFD_FULL_MASK, far)) {
+                            // a row's first keys, or scores that leap: the reference moves now, by a power of two, so that the
+                            // weights already written scale exactly
+                            const float up = far ? (m == -INFINITY ? mx : m + ceilf(mx - m)) : m;
+                            const float alpha = up == m ? 1.f : fast_exp2(m - up);
+                            m = up;
+                            l *= alpha;
+                            acc[0] = mul2(acc[0], dup2(alpha)), acc[1] = mul2(acc[1], dup2(alpha));
+                            if (done >= 1) rescale_o(alpha);
+                            const __nv_bfloat162 a2 = __float2bfloat162_rn(alpha);
 #pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t u[1][32];
-                        tmem_ld32_issue(s_tm + 32 * c, u[0]);
-                        tmem_ld_wait(u);
-                        if (masked) {
-                            const uint32_t vis = visible(c);
+                            for (int d = 0; d < c; ++d) {
+                                uint32_t w[1][32];
+                                tmem_ld32_issue(s_tm + 32 * d, w[0]);
+                                tmem_ld_wait(w);
 #pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (!((vis >> j) & 1u)) u[0][j] = 0xff800000u;
+                                for (int j = 0; j < 32; ++j) {
+                                    const __nv_bfloat162 v = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&w[0][j]), a2);
+                                    w[0][j] = *reinterpret_cast<const uint32_t*>(&v);
+                                }
+                                tmem_st32u(s_tm + 32 * d, w[0]);
+                            }
                         }
+                        const float mr = m == -INFINITY ? 0.f : m;
                         uint32_t hl[32];  // hi pairs, then lo pairs
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
-                            const float4 k = cst[2 * c + q];
+                            const float4 k = q ? k1 : k0;
                             const uint64_t kc = dup2(k.x), kd = dup2(k.y - mr), ki = dup2(k.z);
 #pragma unroll
                             for (int j = 0; j < 8; ++j) {
@@ -291,22 +319,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                     float a0, a1;
                     upk2(add2(acc[0], acc[1]), a0, a1);
-                    l = fmaf(l, alpha, a0 + a1);
-                    if (__any_sync(MFD_FULL_MASK, rescale)) {  // O must hold this group's last product
-                        if (done >= 1) {
-                            ok = __all_sync(MFD_FULL_MASK,
-                                            ok & mbar_wait(&bars[L::kPV + grp], ((grp ? x.n_s1 : x.n_s0) + done - 1) & 1, kTries));
-                            tc_fence_after();
-#pragma unroll 1
-                            for (int oc = 0; oc < kD; oc += 32) {
-                                float o[32];
-                                tmem_ld32(o_tm + oc, o);
-#pragma unroll
-                                for (int j = 0; j < 32; ++j) o[j] *= alpha;
-                                tmem_st32(o_tm + oc, o);
-                            }
-                        }
-                    }
+                    l += a0 + a1;
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
                 tc_fence_before();
@@ -321,16 +334,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             // x.alternate: the two groups' (m, l) of a row meet in the raw ring (every code is converted by now), and each
             // group finishes 64 columns
-            float m_fin = m, l_fin = l, f_own = 1.f, f_oth = 0.f;
+            // (l and O come down to the tiles' maximum first: m may be 2^60 below it)
+            const float f_late = m_next > m && m != -INFINITY ? fast_exp2(m - m_next) : 1.f;
+            if (m != -INFINITY) m = fmaxf(m, m_next);
+            l *= f_late;
+            float m_fin = m, l_fin = l, f_own = 1.f, f_oth = 0.f, f_oth_late = 1.f;
             if (x.alternate) {
                 float* xch = reinterpret_cast<float*>(smem + L::kOffRaw);
                 bar_sync<256>(1);  // (a group without a step has waited for nothing: the other's last product has)
                 xch[grp * 128 + rt] = m;
                 xch[256 + grp * 128 + rt] = l;
+                xch[512 + grp * 128 + rt] = f_late;
                 tc_fence_before();
                 bar_sync<256>(1);  // (both groups' products are complete: each waited for its own)
                 tc_fence_after();
                 const float mo = xch[(1 - grp) * 128 + rt], lo = xch[256 + (1 - grp) * 128 + rt];
+                f_oth_late = xch[512 + (1 - grp) * 128 + rt];
                 m_fin = fmaxf(m, mo);
                 f_own = m == -INFINITY ? 0.f : fast_exp2(m - m_fin);
                 f_oth = mo == -INFINITY ? 0.f : fast_exp2(mo - m_fin);
@@ -362,13 +381,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (own_used) {
                         tmem_ld32(o_tm + oc, o);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] *= f_own;
+                        for (int j = 0; j < 32; ++j) o[j] = o[j] * f_late * f_own;
                     }
                     if (oth_used) {
                         float o2[32];
                         tmem_ld32(tmem + lane_off + 128 * (1 - grp) + oc, o2);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] = fmaf(o2[j], f_oth, o[j]);
+                        for (int j = 0; j < 32; ++j) o[j] = fmaf(o2[j] * f_oth_late, f_oth, o[j]);
                     }
                     if (odd && live) {  // rare: infinities and NaNs of the own values the row sees
                         for (int key = own0; key < own1; ++key) {
