@@ -81,6 +81,33 @@ constexpr int kSlotRows(bool pair) { return pair ? 256 : 128; }
 // floats of a partial: m, l per row, then O as float4 chunks, chunk-major (a warp stores 512 contiguous bytes)
 constexpr int64_t kSlotFloats(bool pair) { return (int64_t)kSlotRows(pair) * (2 + kD); }
 
+// One lane of the warp (elected), and the tensor-core instructions issued by it alone while the warp stays together.
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void umma_if(uint32_t leader, uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, l;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 l, %5, 0;\n\t"
+        "@l tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(leader));
+}
+__device__ __forceinline__ void umma_ts_if(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc,
+                                           uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, l;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 l, %5, 0;\n\t"
+        "@l tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc), "r"(leader));
+}
+__device__ __forceinline__ void commit_if(uint32_t leader, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred l;\n\tsetp.ne.b32 l, %1, 0;\n\t"
+        "@l tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)),
+        "r"(leader)
+        : "memory");
+}
+
 // What a piece's tiles are (of 128 keys: cached tokens first, then the nodes' own).
 struct Tiles {
     int hk, rb;       // KV head, block of rows
@@ -161,7 +188,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             x.nsteps = x.alternate ? x.ntiles : 2 * x.ntiles;
             x.n_piece = n_piece, x.n_tile = n_tile, x.n_s0 = n_s[0], x.n_s1 = n_s[1];
             body(pc, x);
-            __syncwarp();  // (the MMA warp's one lane has been apart)
+            __syncwarp();
             if (!ok) *s_failed = 1;
             tc_fence_before();
             bar_sync<kTcThreads>(0);  // the piece is over for every role
@@ -542,47 +569,54 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (uint32_t f = issued > kStages ? issued - kStages : 0u; f < issued; ++f)
                     mbar_wait(&bars[L::kRawFull + f % kStages], (f / kStages) & 1, 1u << 14);
         } else {
-            pieces([&](const Piece& pc, const Tiles& x) {
-                if (lane != 0) return;
-            // ------------------------------------------------------------ MMA issuer
+            // The whole warp walks the steps and one elected lane issues, by predicate: control flow and descriptors stay
+            // uniform, so the operands of an instruction are immediates and uniform registers (a single lane in a branch of
+            // its own spent three times the products' duration on moving them there).
             constexpr uint32_t kIdescS = idesc_bf16(128, kKt, 0);
             constexpr uint32_t kIdescO = idesc_bf16(128, kD, 1);
-            auto scores = [&](int s) {
-                const int i = x.alternate ? s : s >> 1, grp = s & 1;
-                if (x.alternate || grp == 0) {
-                    ok &= mbar_wait(&bars[L::kKFull], (x.n_tile + i) & 1, kTries);
+            const uint32_t leader = elect_one();
+            const uint64_t qd = sdesc(sbase + L::kOffQ, 16, 1024), kd = sdesc(sbase + L::kOffK, 16, 1024);
+            const uint64_t vd = sdesc(sbase + L::kOffV, kTileBytes / 2, 1024);
+            pieces([&](const Piece&, const Tiles& x) {
+                auto wait = [&](int bar, uint32_t parity) {
+                    ok = __all_sync(MFD_FULL_MASK, ok & mbar_wait(&bars[bar], parity, kTries));
                     tc_fence_after();
-                }
-                const uint32_t q = sbase + L::kOffQ + (x.alternate ? 0 : grp * kTileBytes), k = sbase + L::kOffK;
+                };
+                auto scores = [&](int s) {
+                    const int i = x.alternate ? s : s >> 1, grp = s & 1;
+                    if (x.alternate || grp == 0) wait(L::kKFull, (x.n_tile + i) & 1);
+                    if (!ok) return;
+                    const uint64_t q = qd + (uint64_t)(x.alternate || grp == 0 ? 0 : kTileBytes >> 4);
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks)
-                    umma(tmem + 256 + 128 * grp, sw128_desc(q, ks, 128), sw128_desc(k, ks, 128), kIdescS, ks > 0);
-                umma_commit(&bars[L::kSFull + grp]);
-                if (x.alternate || grp == 1) umma_commit(&bars[L::kKEmpty]);
-            };
-            if (x.nsteps > 0) ok &= mbar_wait(&bars[L::kQFull], x.n_piece & 1, kTries);
-            tc_fence_after();
-            if (x.nsteps > 0 && ok) scores(0);
-            if (x.nsteps > 1 && ok) scores(1);
-            for (int s = 0; s < x.nsteps && ok; ++s) {
-                const int i = x.alternate ? s : s >> 1, grp = s & 1;
-                const uint32_t nv = x.n_tile + i;
-                ok &= mbar_wait(&bars[L::kPFull + grp], ((grp ? x.n_s1 : x.n_s0) + (s >> 1)) & 1, kTries);
-                if (x.alternate || grp == 0) ok &= mbar_wait(&bars[L::kVFull + (nv & 1)], (nv >> 1) & 1, kTries);
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t v = sbase + L::kOffV + (nv & 1) * kTileBytes, pt = tmem + 256 + 128 * grp;
+                    for (int ks = 0; ks < 8; ++ks) {
+                        const uint64_t off = (uint64_t)(((ks >> 2) * (kTileBytes / 2) + (ks & 3) * 32) >> 4);
+                        umma_if(leader, tmem + 256 + 128 * grp, q + off, kd + off, kIdescS, ks > 0);
+                    }
+                    commit_if(leader, &bars[L::kSFull + grp]);
+                    if (x.alternate || grp == 1) commit_if(leader, &bars[L::kKEmpty]);
+                };
+                if (x.nsteps > 0) wait(L::kQFull, x.n_piece & 1);
+                if (x.nsteps > 0 && ok) scores(0);
+                if (x.nsteps > 1 && ok) scores(1);
+#pragma unroll 1
+                for (int s = 0; s < x.nsteps && ok; ++s) {
+                    const int i = x.alternate ? s : s >> 1, grp = s & 1;
+                    const uint32_t nv = x.n_tile + i;
+                    if (x.alternate || grp == 0) wait(L::kVFull + (nv & 1), (nv >> 1) & 1);
+                    wait(L::kPFull + grp, ((grp ? x.n_s1 : x.n_s0) + (s >> 1)) & 1);
+                    if (!ok) break;
+                    const uint64_t v = vd + (uint64_t)((nv & 1) * (kTileBytes >> 4));
+                    const uint32_t pt = tmem + 256 + 128 * grp;
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks) {  // 16 keys: hi, then lo
-                    const uint64_t vd = sdesc(v + ks * 2048, kTileBytes / 2, 1024);
-                    const uint32_t pa = pt + 32 * (ks >> 1) + 8 * (ks & 1);
-                    umma_ts(tmem + 128 * grp, pa, vd, kIdescO, (s >= 2 || ks > 0) ? 1u : 0u);
-                    umma_ts(tmem + 128 * grp, pa + 16, vd, kIdescO, 1u);
+                    for (int ks = 0; ks < 8; ++ks) {  // 16 keys: hi, then lo
+                        const uint32_t pa = pt + 32 * (ks >> 1) + 8 * (ks & 1);
+                        umma_ts_if(leader, tmem + 128 * grp, pa, v + (uint64_t)(ks * 128), kIdescO, ks > 0 ? 1u : (uint32_t)(s >= 2));
+                        umma_ts_if(leader, tmem + 128 * grp, pa + 16, v + (uint64_t)(ks * 128), kIdescO, 1u);
+                    }
+                    commit_if(leader, &bars[L::kPV + grp]);
+                    if (x.alternate || grp == 1) commit_if(leader, &bars[L::kVEmpty + (nv & 1)]);
+                    if (s + 2 < x.nsteps) scores(s + 2);
                 }
-                umma_commit(&bars[L::kPV + grp]);
-                if (x.alternate || grp == 1) umma_commit(&bars[L::kVEmpty + (nv & 1)]);
-                if (s + 2 < x.nsteps) scores(s + 2);
-            }
             });
         }
     }
