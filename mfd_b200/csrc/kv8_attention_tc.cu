@@ -13,9 +13,9 @@
 //   single a CTA takes one row tile; group t takes every other key tile and the two (m, l, O) merge at the end
 // In both, step s is group s & 1; the products run PV(s), S(s + 2) in order.
 //
-// Warp roles (512 threads, one CTA an SM; the softmax warps take registers from the others, so that a thread holds its
-// 128 scores: 256 x 184 + 256 x 72 = 512 x 128 registers, what the CTA was launched with):
-//   warps 0-7    softmax, thread = row
+// Warp roles (512 threads, one CTA an SM; the softmax warps take registers from the others: 256 x 152 + 256 x 104 = 512 x
+// 128, what the CTA was launched with):
+//   warps 0-7    softmax, thread = row, 32 scores at a time from TMEM
 //   warps 8-13   converters: raw codes -> bf16 tiles in the 128-byte-swizzled operand layout; the nodes' own keys are
 //                copied there (past the end of a request: zeros, whatever the page holds)
 //   warp 14      producer: page ids and scales, one TMA load per page and tensor into the raw ring (no multicast)
@@ -42,7 +42,7 @@ namespace {
 
 constexpr int kTcThreads = 512;
 constexpr int kConv = 6;                 // converter warps
-constexpr int kSoftmaxRegs = 184, kOtherRegs = 72;
+constexpr int kSoftmaxRegs = 152, kOtherRegs = 104;
 constexpr int kKt = 128;                 // keys per tile
 constexpr int kTileBytes = kKt * kD * 2;  // 32 KB: a bf16 tile, [2 d-halves][128 rows][128 B]
 constexpr int kRawBytes = 2 * kKt * kD;   // 32 KB: the codes of K and V
@@ -474,16 +474,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         const int valid = min(kKt, pc.len - tile * kKt);
                         const unsigned char* src = smem + L::kOffRaw + st * kRawBytes + which * (kRawBytes / 2);
                         const int c = lane & 7, h = c >> 2, q = 2 * (c & 3);
-#pragma unroll 3
-                        for (int j = cw; j < 32; j += kConv) {  // 4 rows of 8 16-byte chunks an instruction
-                            const int r = j * 4 + (lane >> 3);
-                            uint4 cw4 = make_uint4(0u, 0u, 0u, 0u);
-                            if (r < valid) cw4 = *reinterpret_cast<const uint4*>(src + r * kD + c * 16);
+                        constexpr int kMine = (32 + kConv - 1) / kConv;  // groups of 4 rows (8 16-byte chunks each) a warp
+                        uint4 raw[kMine];                                // all loads first: one latency, not six
+#pragma unroll
+                        for (int i = 0; i < kMine; ++i) {
+                            const int r = (cw + kConv * i) * 4 + (lane >> 3);
+                            raw[i] = make_uint4(0u, 0u, 0u, 0u);
+                            if (r < valid) raw[i] = *reinterpret_cast<const uint4*>(src + r * kD + c * 16);
+                        }
+#pragma unroll
+                        for (int i = 0; i < kMine; ++i) {
+                            const int r = (cw + kConv * i) * 4 + (lane >> 3);
+                            if (r >= kKt) break;  // (uniform: whole groups)
                             uint4 y0, y1;
-                            bfloats<FP8>(cw4.x, y0.x, y0.y);
-                            bfloats<FP8>(cw4.y, y0.z, y0.w);
-                            bfloats<FP8>(cw4.z, y1.x, y1.y);
-                            bfloats<FP8>(cw4.w, y1.z, y1.w);
+                            bfloats<FP8>(raw[i].x, y0.x, y0.y);
+                            bfloats<FP8>(raw[i].y, y0.z, y0.w);
+                            bfloats<FP8>(raw[i].z, y1.x, y1.y);
+                            bfloats<FP8>(raw[i].w, y1.z, y1.w);
                             unsigned char* base = dst + h * (kTileBytes / 2) + r * 128;
                             // chunks q and q + 1; the upper half's lanes store them in the other order, so the eight
                             // lanes of a row hit eight different bank groups
@@ -649,12 +656,13 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(const AttnParams p, in
     const int r = blockIdx.y * 32 + lane, row = p.row0 + rb * kRowsU + r;
     if (row - lane >= p.rows) return;
     float mm = -INFINITY;
+#pragma unroll 8
     for (int i = 0; i < pc.pieces; ++i) mm = fmaxf(mm, __ldg(p.part + (int64_t)slot_of(pc, i) * kSlotFloats(PAIR) + r));
     float ll = 0.f;
     float4 v[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
+#pragma unroll 4
     for (int i = 0; i < pc.pieces; ++i) {
         const float* s = p.part + (int64_t)slot_of(pc, i) * kSlotFloats(PAIR);
         const float mi = __ldg(s + r), li = __ldg(s + kRowsU + r);
