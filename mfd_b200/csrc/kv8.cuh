@@ -9,6 +9,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace mfd {
@@ -192,7 +194,7 @@ __device__ __forceinline__ int quotient(int a, int b) {
     return q;
 }
 
-// Work laid end to end over the requests, f(length) * mul of it for each (below 2^31 in all: the entry points check);
+// Work laid end to end over the requests, f(length) * mul (or f(length, request) * mul) of it for each (below 2^31 in all: the entry points check);
 // every warp finds its place by itself.  The lengths of the first 32 requests stay in the lanes' registers.
 struct Lengths {
     const Cache& c;
@@ -205,7 +207,9 @@ struct Lengths {
     __device__ __forceinline__ int part(int b0, F f, int& len) const {
         const int b = b0 + (threadIdx.x & 31);
         len = b0 == 0 ? mine : (b < bs ? seq_len(c, b) : 0);
-        return b < bs ? f(len) : 0;
+        if (b >= bs) return 0;
+        if constexpr (std::is_invocable_v<F, int, int>) return f(len, b);
+        else return f(len);
     }
     // the sum over all requests
     template <class F>

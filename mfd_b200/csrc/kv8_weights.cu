@@ -8,29 +8,27 @@
 //
 // Bound: K's bytes (128 codes a token and KV head); next, instructions: the scores' products of 2 * 128 flop and an
 // exponential per listed row and token.  As in kv8_attention_rows.cu the 16 tokens are the wide operand of the tensor
-// instruction and 8 query rows the narrow one, and the codes come by TMA, a page a copy, into a ring of two 32 KB stages
-// (256 tokens; two CTAs an SM).  A warp turns 32 tokens' codes into operands once and runs all listed rows past them, 8 at a
-// time from shared memory: 32 tokens rather than 16 halve those reads, which would otherwise take as long as the codes.
+// instruction and 8 query rows the narrow one, and every warp copies its own codes asynchronously into a ring of its own
+// (two stages of 32 tokens).  It turns 32 tokens' codes into operands once and runs all listed rows past them, 16 at a time
+// from shared memory: 32 tokens rather than 16 halve those reads, and two row tiles side by side give four independent
+// chains of products.
 //
-// Split: the tiles of all (request, KV head) units are laid end to end and cut into equal ranges, one per CTA, so ragged
-// lengths balance.  Each 16 tokens' sum goes to the workspace; the CTA that finishes a request last adds them up per
+// Split: the tiles of all (request, KV head) units are laid end to end by their cost (tokens, and rows that pass them) and
+// cut into equal ranges, one per CTA, so ragged lengths and counts balance.  Each 16 tokens' sum goes to the workspace; the CTA that finishes a request last adds them up per
 // page, in a fixed order over tokens and heads (no float atomics).
-//
-// Every mbarrier wait is bounded; a CTA whose wait gave up stores NaN sums, so the masses show it.
-#include "kv8_attention.cuh"
-#include "tcgen05.cuh"
+#include "kv8.cuh"
 
 namespace mfd {
 namespace kv8 {
 
 constexpr int kWWarps = 8;
 constexpr int kWThreads = 32 * kWWarps;
-constexpr int kWTile = 256;     // tokens a stage
+constexpr int kWTile = 32 * kWWarps;     // tokens the warps take side by side
 constexpr int kWStages = 2;
-constexpr int kWStageBytes = kWTile * kD;
+constexpr int kWStageBytes = 32 * kD;    // of a warp
+constexpr int kWRingBytes = kWWarps * kWStages * kWStageBytes;
 constexpr int kWRowTiles = 16;  // 8-row tiles staged at a time
 constexpr int kWCtasPerSm = 2;
-constexpr uint32_t kWTries = 1u << 20;
 
 struct WeightParams {
     Cache c;
@@ -53,87 +51,73 @@ struct WeightParams {
 
 template <bool FP8>
 __global__ void __launch_bounds__(kWThreads, kWCtasPerSm)
-    kv8_weights_kernel(const __grid_constant__ CUtensorMap tmk, const WeightParams p) {
-    extern __shared__ __align__(16) unsigned char smem_raw[];
-    unsigned char* ring = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
-    auto s_q = reinterpret_cast<uint2(*)[8][32]>(ring + kWStages * kWStageBytes);  // query operands: tile, step, lane
+    kv8_weights_kernel(const WeightParams p) {
+    extern __shared__ __align__(128) unsigned char ring[];
+    auto s_q = reinterpret_cast<uint2(*)[8][32]>(ring + kWRingBytes);  // query operands: tile, step, lane
     __shared__ __align__(16) float2 s_row[kWRowTiles][8];  // score factor and -log2(e) * log-sum-exp of a row
-    __shared__ float s_scale[kWStages][16];  // K scales of the tile's pages
-    __shared__ uint64_t s_full[kWStages], s_empty[kWStages];
     __shared__ int s_last;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
-    if (tid == 0) {
-        for (int i = 0; i < kWStages; ++i) {
-            mbar_init(&s_full[i], 32);
-            mbar_init(&s_empty[i], kWWarps);
-        }
-        mbar_fence_init();
-    }
     const int Hkv = p.c.Hkv;
+    // a tile's cost: about four row tiles' for its codes, and one for every 8 rows that pass them
     auto tiles_of = [&](int len) { return max(1, (len + kWTile - 1) / kWTile); };
+    auto weight_of = [&](int b) {
+        const int rows = p.counts ? min(max(__ldg(p.counts + b), 0), p.rows) : p.rows;
+        return 4 + min((rows * p.G + 7) >> 3, 60);
+    };
+    auto cost_of = [&](int len, int b) { return tiles_of(len) * weight_of(b); };
     const Lengths lens(p.c, p.bs);
-    const int total = lens.sum(tiles_of) * Hkv;
+    const int total = lens.sum(cost_of) * Hkv;
     const int per = max(1, quotient(total + gridDim.x - 1, gridDim.x));
     int pos = (int)min((int64_t)blockIdx.x * per, (int64_t)total);
     const int end = (int)min((int64_t)total, (int64_t)pos + per);
-    __syncthreads();
 
-    uint32_t n_tile = 0;  // tiles fetched before: the barriers' phases
-    bool ok = true;
     while (pos < end) {
         int before, len;
-        const int b = lens.find(pos, Hkv, tiles_of, before, len);
+        const int b = lens.find(pos, Hkv, cost_of, before, len);
         if (b < 0) return;
-        const int tiles = tiles_of(len);
+        // of the unit (b, hk) the tiles whose cost begins in [pos, end)
+        const int tiles = tiles_of(len), weight = weight_of(b), unit = tiles * weight;
         const int off = pos - before;
-        const int hk = quotient(off, tiles), t0 = off - hk * tiles;
-        const int t1 = min(tiles, t0 + (end - pos));
+        const int hk = quotient(off, unit), u0 = off - hk * unit, u1 = min(unit, u0 + (end - pos));
+        const int t0 = quotient(u0 + weight - 1, weight), t1 = quotient(u1 + weight - 1, weight);
         const int listed = listed_rows(p.path, p.path_stride, p.rows, p.counts, p.n, b);
         const int nrows = listed * p.G;
         float* part = p.part + (int64_t)b * p.groups_max * Hkv + hk;
 
-        // ---- the producer, warp 0: a tile's copies, then its scales; ids two tiles and scales one tile ahead
-        const int ppt = kWTile >> p.c.page_shift;  // at most 16
-        int next = 0, id0 = -1, id1 = -1;
-        float sc = 0.f;
-        auto id_of = [&](int tile) {
-            const int pg = tile * ppt + lane;
-            return lane < ppt && tile < t1 && (pg << p.c.page_shift) < len ? page_id(p.c, b, pg) : -1;
+        // ---- this warp's copies: lane l takes chunk l % 8 of rows l / 8 + 4 i; the page ids are read a tile ahead
+        unsigned char* mine = ring + warp * (kWStages * kWStageBytes);
+        const int64_t lane_off = (int64_t)hk * p.c.sc_h + (int64_t)(lane >> 3) * p.c.sc_t + (lane & 7) * 16;
+        auto key_of = [&](int tile, int q) { return tile * kWTile + 32 * warp + 16 * q; };
+        auto id_of = [&](int tile, int q) {
+            return tile < t1 && key_of(tile, q) < len ? page_id(p.c, b, key_of(tile, q) >> p.c.page_shift) : -1;
         };
-        auto scale_of = [&](int id) { return id < 0 ? 0.f : __ldg(p.c.k_scale + (int64_t)id * Hkv + hk); };
-        auto produce = [&]() {
-            const uint32_t nt = n_tile + next - t0, st = nt % kWStages;
-            if (nt >= (uint32_t)kWStages)
-                ok = __all_sync(MFD_FULL_MASK, ok & mbar_wait(&s_empty[st], (nt / kWStages - 1) & 1, kWTries));
-            if (!ok) return;
-            if (id0 >= 0) {
-                const uint32_t bytes = (uint32_t)(p.c.page * kD);
-                mbar_expect_tx(&s_full[st], bytes);
-                tma_page(smem_addr(ring) + st * kWStageBytes + lane * bytes, &tmk, &s_full[st], hk, id0);
-                s_scale[st][lane] = sc;
+        auto fetch = [&](int tile, const int (&id)[2]) {
+            unsigned char* dst = mine + (tile - t0) % kWStages * kWStageBytes;
+            float2 sc = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                if (id[q] < 0) continue;
+                const uint8_t* src = p.c.k + (int64_t)id[q] * p.c.sc_p + (int64_t)(key_of(tile, q) & (p.c.page - 1)) * p.c.sc_t + lane_off;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    copy16(dst + chunk_at(16 * q + 4 * i + (lane >> 3), lane & 7), src + (int64_t)(4 * i) * p.c.sc_t);
+                (q ? sc.y : sc.x) = __ldg(p.c.k_scale + (int64_t)id[q] * Hkv + hk);
             }
-            __syncwarp();  // lanes without a page (16 .. 31 never have one) arrive last, after every scale is stored
-            if (id0 < 0) mbar_arrive(&s_full[st]);
-            ++next;
-            id0 = id1;
-            sc = scale_of(id0);
-            id1 = id_of(next + 1);
+            copies_commit();
+            return sc;
         };
 
         // one pass in all but extreme cases: 128 rows are staged at a time
 #pragma unroll 1
-        for (int r0 = 0; r0 == 0 || r0 < nrows; r0 += kWRowTiles * 8) {
+        for (int r0 = 0; t0 < t1 && (r0 == 0 || r0 < nrows); r0 += kWRowTiles * 8) {
             const int row_tiles = min(kWRowTiles, (nrows - r0 + 7) / 8);
-            if (warp == 0) {
-                next = t0;
-                id0 = id_of(t0), id1 = id_of(t0 + 1);
-                sc = scale_of(id0);
-                for (int i = 0; i < kWStages && next < t1; ++i) produce();
-            }
+            int id[2] = {id_of(t0, 0), id_of(t0, 1)};
+            float2 sc0 = fetch(t0, id);
+            id[0] = id_of(t0 + 1, 0), id[1] = id_of(t0 + 1, 1);
             // ---- the listed rows as operands: row g of tile w for warp w
 #pragma unroll 1
-            for (int rt = kWWarps - 1 - warp; rt < row_tiles; rt += kWWarps) {  // (warp 0, the producer, last)
+            for (int rt = warp; rt < row_tiles; rt += kWWarps) {
                 const int r = r0 + rt * 8 + g;
                 const bool live = r < nrows;
                 const int i = live ? quotient(r, p.G) : 0;
@@ -178,27 +162,24 @@ __global__ void __launch_bounds__(kWThreads, kWCtasPerSm)
             __syncthreads();
 #pragma unroll 1
             for (int tile = t0; tile < t1; ++tile) {
-                const uint32_t nt = n_tile + tile - t0, st = nt % kWStages;
-                ok = __all_sync(MFD_FULL_MASK, ok & mbar_wait(&s_full[st], (nt / kWStages) & 1, kWTries));
-                if (!ok) break;
-                const int key0 = tile * kWTile + 32 * warp;
+                __syncwarp();  // (every lane has read the stage that the copies below overwrite)
+                const float2 sc1 = fetch(tile + 1, id);
+                id[0] = id_of(tile + 2, 0), id[1] = id_of(tile + 2, 1);
+                copies_wait<1>();
+                __syncwarp();
+                const int key0 = key_of(tile, 0);
+                if (key0 >= len) break;
+                const unsigned char* kt = mine + (tile - t0) % kWStages * kWStageBytes;
                 uint4 raw[2][2][2];  // of 16 tokens each: token g, g + 8; chunks 2 t, 2 t + 1
-                float sk[2];
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const unsigned char* kt = ring + st * kWStageBytes + (32 * warp + 16 * q + g) * kD;
+                for (int q = 0; q < 2; ++q)
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
-                            raw[q][h][i] = *reinterpret_cast<const uint4*>(kt + h * 8 * kD +
-                                                                           (((uint32_t)(2 * t + i) << 4) ^ ((uint32_t)(g & 7) << 4)));
-                    sk[q] = s_scale[st][(32 * warp + 16 * q) >> p.c.page_shift];
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&s_empty[st]);
-                if (warp == 0 && next < t1) produce();
-                if (key0 >= len) continue;
+                            raw[q][h][i] = *reinterpret_cast<const uint4*>(kt + chunk_at(16 * q + 8 * h + g, 2 * t + i));
+                const float sk[2] = {sc0.x, sc0.y};
+                sc0 = sc1;
                 uint32_t a[2][8][4];
 #pragma unroll
                 for (int q = 0; q < 2; ++q)
@@ -212,32 +193,51 @@ __global__ void __launch_bounds__(kWThreads, kWCtasPerSm)
                 float sum[2] = {0.f, 0.f};
                 const bool tail = key0 + 32 > len;
 #pragma unroll 1
-                for (int rt = 0; rt < row_tiles; ++rt) {
-                    float acc[2][4];
+                for (int rt = 0; rt < row_tiles; rt += 2) {
+                    float acc[2][2][4];  // row tile, 16 tokens
 #pragma unroll
-                    for (int q = 0; q < 2; ++q)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[q][e] = 0.f;
-#pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) {
-                        const uint2 x = s_q[rt][ks][lane];
+                    for (int u = 0; u < 2; ++u)
 #pragma unroll
                         for (int q = 0; q < 2; ++q)
-                            mma_f16(acc[q], a[q][ks][0], a[q][ks][1], a[q][ks][2], a[q][ks][3], x.x, x.y);
-                    }
-                    const float4 f = *reinterpret_cast<const float4*>(&s_row[rt][2 * t]);  // rows 2 t and 2 t + 1
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const float fx = f.x * sk[q], fz = f.z * sk[q];
-                        float w[4];
+                            for (int e = 0; e < 4; ++e) acc[u][q][e] = 0.f;
+                    const bool two = rt + 1 < row_tiles;
+                    if (two) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            w[e] = fast_exp2(fmaf(acc[q][e], (e & 1) ? fz : fx, (e & 1) ? f.w : f.y));
-                        if (tail) {
-                            if (key0 + 16 * q + g >= len) w[0] = w[1] = 0.f;
-                            if (key0 + 16 * q + g + 8 >= len) w[2] = w[3] = 0.f;
+                        for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) {
+                                const uint2 x = s_q[rt + u][ks][lane];
+#pragma unroll
+                                for (int q = 0; q < 2; ++q)
+                                    mma_f16(acc[u][q], a[q][ks][0], a[q][ks][1], a[q][ks][2], a[q][ks][3], x.x, x.y);
+                            }
+                    } else {
+#pragma unroll
+                        for (int ks = 0; ks < 8; ++ks) {
+                            const uint2 x = s_q[rt][ks][lane];
+#pragma unroll
+                            for (int q = 0; q < 2; ++q)
+                                mma_f16(acc[0][q], a[q][ks][0], a[q][ks][1], a[q][ks][2], a[q][ks][3], x.x, x.y);
                         }
-                        sum[q] += (w[0] + w[1]) + (w[2] + w[3]);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        if (u == 1 && !two) break;
+                        const float4 f = *reinterpret_cast<const float4*>(&s_row[rt + u][2 * t]);  // rows 2 t and 2 t + 1
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            const float fx = f.x * sk[q], fz = f.z * sk[q];
+                            float w[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                w[e] = fast_exp2(fmaf(acc[u][q][e], (e & 1) ? fz : fx, (e & 1) ? f.w : f.y));
+                            if (tail) {
+                                if (key0 + 16 * q + g >= len) w[0] = w[1] = 0.f;
+                                if (key0 + 16 * q + g + 8 >= len) w[2] = w[3] = 0.f;
+                            }
+                            sum[q] += (w[0] + w[1]) + (w[2] + w[3]);
+                        }
                     }
                 }
 #pragma unroll
@@ -250,20 +250,13 @@ __global__ void __launch_bounds__(kWThreads, kWCtasPerSm)
                     }
                 }
             }
-            if (!ok)
-                for (int i = tid; i < (t1 - t0) * (kWTile / 16); i += kWThreads)
-                    if ((t0 * kWTile + 16 * i) < len) part[(int64_t)(t0 * (kWTile / 16) + i) * Hkv] = NAN;
-            if (!ok && warp == 0)  // copies in flight end before the CTA does (bounded)
-                for (uint32_t f = n_tile + next - t0, i = f > kWStages ? f - kWStages : 0u; i < f; ++i)
-                    mbar_wait(&s_full[i % kWStages], (i / kWStages) & 1, 1u << 14);
-            n_tile += t1 - t0;
-            ok = __syncthreads_and(ok);  // the staged rows are done with
-            if (!ok) break;
+            copies_wait<0>();
+            __syncthreads();  // the staged rows are done with
         }
-        pos += t1 - t0;
+        pos += u1 - u0;
         // ---- the request's last CTA adds up its pages
-        if (pos >= end || pos >= before + tiles * Hkv) {
-            const int pieces = quotient(before + tiles * Hkv - 1, per) - quotient(before, per) + 1;
+        if (pos >= end || pos >= before + unit * Hkv) {
+            const int pieces = quotient(before + unit * Hkv - 1, per) - quotient(before, per) + 1;
             __threadfence();
             __syncthreads();
             if (tid == 0) s_last = pieces == 1 || atomicAdd(p.tickets + b, 1u) == (unsigned)(pieces - 1);
@@ -286,7 +279,6 @@ __global__ void __launch_bounds__(kWThreads, kWCtasPerSm)
                 if (tid == 0 && pieces > 1) p.tickets[b] = 0u;
             }
         }
-        if (!ok) return;
     }
 }
 
@@ -337,7 +329,7 @@ extern "C" int mfd_kv8_page_weights(const void* q, int64_t sq_b, int64_t sq_n, i
         set_error("%s: workspace or tickets too small", who);
         return MFD_ERR_INVALID;
     }
-    if (!kv8::work_fits(bs, num_kv_heads, max_pages, page_size, 256)) {
+    if (!kv8::work_fits(bs, num_kv_heads * 64, max_pages, page_size, 256)) {
         set_error("%s: the requests' capacity is beyond this build's limits", who);
         return MFD_ERR_UNSUPPORTED;
     }
@@ -362,12 +354,7 @@ extern "C" int mfd_kv8_page_weights(const void* q, int64_t sq_b, int64_t sq_n, i
     p.groups_max = (int)(max_pages * (page_size / 16));
     p.tickets = tickets;
     const int grid = kv8::sm_count() * kv8::kWCtasPerSm;
-    constexpr int kSmem = kv8::kWStages * kv8::kWStageBytes + kv8::kWRowTiles * 8 * 32 * 8 + 1024;
-    CUtensorMap tk;
-    if (!kv8::make_page_map(&tk, p.c.k, p.c, true)) {
-        set_error("%s: could not encode the TMA tensor map", who);
-        return MFD_ERR_CUDA;
-    }
+    constexpr int kSmem = kv8::kWRingBytes + kv8::kWRowTiles * 8 * 32 * 8;
     static bool opted[2][64];
     const bool fp8 = code_dtype == MFD_E4M3;
     const void* kernel = fp8 ? (const void*)kv8::kv8_weights_kernel<true> : (const void*)kv8::kv8_weights_kernel<false>;
@@ -376,8 +363,8 @@ extern "C" int mfd_kv8_page_weights(const void* q, int64_t sq_b, int64_t sq_n, i
         set_error("%s: %s", who, cudaGetErrorString(e));
         return MFD_ERR_CUDA;
     }
-    if (fp8) kv8::kv8_weights_kernel<true><<<grid, kv8::kWThreads, kSmem, (cudaStream_t)stream>>>(tk, p);
-    else kv8::kv8_weights_kernel<false><<<grid, kv8::kWThreads, kSmem, (cudaStream_t)stream>>>(tk, p);
+    if (fp8) kv8::kv8_weights_kernel<true><<<grid, kv8::kWThreads, kSmem, (cudaStream_t)stream>>>(p);
+    else kv8::kv8_weights_kernel<false><<<grid, kv8::kWThreads, kSmem, (cudaStream_t)stream>>>(p);
     MFD_CHECK_LAUNCH(who);
     return MFD_OK;
 }
