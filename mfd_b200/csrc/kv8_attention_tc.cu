@@ -205,26 +205,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         pieces([&](const Piece& pc, const Tiles& x) {
             // ------------------------------------------------------------ queries into their operand layout
+            // (asynchronous copies, all in flight together; a rolled loop, since the code is cold)
 #pragma unroll 1
-            for (int r0 = 0; r0 < 128 * x.ntl; r0 += 64) {
-                uint4 qv[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int row = x.row_base + r0 + (tid >> 4) + 16 * j;
+            for (int r = tid >> 4; r < 128 * x.ntl; r += 16) {
+                const int row = x.row_base + r, c = tid & 15;
+                unsigned char* dst = smem + L::kOffQ + (r >> 7) * kTileBytes + sw128_offset(r & 127, c * 8, 128);
+                if (row < p.rows) {
                     const int node = quotient(row, p.G);
-                    qv[j] = make_uint4(0u, 0u, 0u, 0u);
-                    if (row < p.rows)
-                        qv[j] = __ldg(reinterpret_cast<const uint4*>(p.q + (int64_t)pc.b * p.sq_b + (int64_t)node * p.sq_n +
-                                                                     (int64_t)(x.hk * p.G + row - node * p.G) * p.sq_h +
-                                                                     (tid & 15) * 8));
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int r = r0 + (tid >> 4) + 16 * j;
-                    *reinterpret_cast<uint4*>(smem + L::kOffQ + (r >> 7) * kTileBytes +
-                                              sw128_offset(r & 127, (tid & 15) * 8, 128)) = qv[j];
+                    copy16(dst, p.q + (int64_t)pc.b * p.sq_b + (int64_t)node * p.sq_n +
+                                    (int64_t)(x.hk * p.G + row - node * p.G) * p.sq_h + c * 8);
+                } else {
+                    *reinterpret_cast<uint4*>(dst) = make_uint4(0u, 0u, 0u, 0u);
                 }
             }
+            copies_commit();
+            copies_wait<0>();
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars[L::kQFull]);

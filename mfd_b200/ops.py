@@ -594,26 +594,28 @@ _KV8_CODES = {torch.int8: MFD_I8, torch.float8_e4m3fn: MFD_E4M3}
 
 
 def _kv8_check(what: str, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens):
-    """The cache's checks; its shape, strides and code type."""
+    """The cache's checks; its shape, strides and code type, and the table's shape."""
     shape, strides = k_cache.shape, k_cache.stride()
     code = _KV8_CODES.get(k_cache.dtype)
     if code is None:
         raise RuntimeError(f"{what}: cache codes must be int8 or float8_e4m3fn, got {k_cache.dtype}")
     if len(shape) != 4 or strides[3] != 1:
         raise RuntimeError(f"{what}: caches must be [pages, KV heads, page_size, D] with a contiguous last dim")
-    if v_cache is not None and (v_cache.shape != shape or v_cache.dtype != k_cache.dtype
-                                or v_cache.stride() != strides):
+    if v_cache is not None and (v_cache.shape != shape or v_cache.stride() != strides
+                                or v_cache.dtype != k_cache.dtype):
         raise RuntimeError(f"{what}: k_cache and v_cache need the same dtype, shape and strides")
-    pages = shape[:2]
-    if (k_scale.dtype != torch.float32 or k_scale.shape != pages or not k_scale.is_contiguous()
-            or (v_scale is not None and (v_scale.dtype != torch.float32 or v_scale.shape != pages
-                                         or not v_scale.is_contiguous()))):
+    # (a contiguous [pages, KV heads] has these strides whatever its sizes)
+    pages, rows = (shape[0], shape[1]), (shape[1], 1)
+    if k_scale.dtype != torch.float32 or k_scale.shape != pages or k_scale.stride() != rows or (
+            v_scale is not None and (v_scale.dtype != torch.float32 or v_scale.shape != pages
+                                     or v_scale.stride() != rows)):
         raise RuntimeError(f"{what}: scales must be contiguous float32 [pages, KV heads]")
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1:
+    table = page_table.shape
+    if page_table.dtype != torch.int32 or len(table) != 2 or page_table.stride(1) != 1:
         raise RuntimeError(f"{what}: page_table must be int32 [bs, max_pages] with a contiguous last dim")
-    if seq_lens.dtype != torch.int32 or seq_lens.shape != page_table.shape[:1] or not seq_lens.is_contiguous():
+    if seq_lens.dtype != torch.int32 or seq_lens.shape != table[:1] or not seq_lens.is_contiguous():
         raise RuntimeError(f"{what}: seq_lens must be contiguous int32 [bs]")
-    return shape, strides, code
+    return shape, strides, code, table
 
 
 def _kv8_rows(what: str, rows: torch.Tensor, name: str, shape):
@@ -654,8 +656,8 @@ def kv8_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tens
     counts as accept's "commit_lens"; None: all).  Returns the new lengths (a tensor of their own)."""
     dev = device_index(k_cache, v_cache, k_scale, v_scale, k_new, v_new, page_table, seq_lens, path, counts, new_lens,
                        status)
-    (pages, hkv, page, d), sc, code = _kv8_check("kv8_append", k_cache, v_cache, k_scale, v_scale, page_table, seq_lens)
-    bs, width = page_table.shape
+    (pages, hkv, page, d), sc, code, (bs, width) = _kv8_check("kv8_append", k_cache, v_cache, k_scale, v_scale,
+                                                             page_table, seq_lens)
     n = k_new.shape[1]
     sn = _kv8_new("kv8_append", k_new, v_new, (bs, n, hkv, d))
     path_stride, rows = _kv8_path("kv8_append", bs, n, path, counts)
@@ -703,9 +705,8 @@ def kv8_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     n = 1 is a decode step.  Returns out [bs, n, H, 128] bf16, or (out, lse) with lse f32 [bs, n, H] the natural
     log-sum-exp of every row's scaled scores.  Rows that see nothing give 0 and -inf."""
     dev = device_index(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, k_new, v_new, anc, out)
-    (pages, hkv, page, d), sc, code = _kv8_check("kv8_attention", k_cache, v_cache, k_scale, v_scale, page_table,
-                                                 seq_lens)
-    bs, width = page_table.shape
+    (pages, hkv, page, d), sc, code, (bs, width) = _kv8_check("kv8_attention", k_cache, v_cache, k_scale, v_scale,
+                                                             page_table, seq_lens)
     shape = q.shape
     if len(shape) != 4 or shape[0] != bs or shape[3] != d:
         raise RuntimeError(f"kv8_attention: q must be [bs, n, H, D] for {bs} requests, D = {d}; got {tuple(shape)}")
@@ -722,7 +723,7 @@ def kv8_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
             raise RuntimeError("kv8_attention: anc must be contiguous int64 [bs, n, words]")
         ab, words = anc.data_ptr(), anc.shape[2]
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         so = (n * H * d, H * d, d)
     else:
         so = _kv8_rows("kv8_attention", out, "out", shape)
@@ -764,9 +765,8 @@ def kv8_page_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, 
     the page's tokens; 0 past a request's pages.  lse f32 [bs, n, H] from kv8_attention on the same cache (before the
     nodes are appended); mass f32 [bs, max_pages]; out may be mass.  The sums run in a fixed order."""
     dev = device_index(q, lse, k_cache, k_scale, page_table, seq_lens, mass, path, counts, out)
-    (pages, hkv, page, d), sc, code = _kv8_check("kv8_page_weights", k_cache, None, k_scale, None, page_table,
-                                                 seq_lens)
-    table_shape = page_table.shape
+    (pages, hkv, page, d), sc, code, table_shape = _kv8_check("kv8_page_weights", k_cache, None, k_scale, None,
+                                                             page_table, seq_lens)
     bs, width = table_shape
     shape = q.shape
     if len(shape) != 4 or shape[0] != bs or shape[3] != d:
