@@ -55,7 +55,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     // the warps' rings; at a piece's end [kWarps][kRows][kRowStride] floats, then the merge weights
     extern __shared__ __align__(128) unsigned char ring[];
     float* smem = reinterpret_cast<float*>(ring);
-    __shared__ float s_own[kRows][kMaxOwn];    // scores of the nodes' own keys (log2), -inf where not visible
+    __shared__ float s_own[kRows][kMaxOwn];     // scores (log2) of the own keys a row sees, then their weights
+    __shared__ uint8_t s_key[kRows][kMaxOwn];   // which keys they are
+    __shared__ int s_seen[kRows];               // how many
     __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows], s_mm[kRows], s_ll[kRows];
     __shared__ uint2 s_q[NT][8][32];  // query operands, the same for every warp (in registers they would spill)
     __shared__ int s_last;
@@ -198,46 +200,48 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         };
 
         // ---- scores of the nodes' own keys, while the first tiles are on their way: few products, on the CUDA cores (a
-        // second set of tensor instructions for them cost more in instruction fetches than in arithmetic).  The weights meet the
-        // values in the merge below.
+        // second set of tensor instructions for them cost more in instruction fetches than in arithmetic).  A warp takes a
+        // row, lists the keys it sees (of a tree's nodes a row sees its ancestors) and gives each eight lanes, 16 columns a
+        // lane.  The weights meet the values in the merge below.
         const int live_rows = min(16, p.rows - base);
         const int own = pc.g1 == pc.of ? p.nn : 0;  // of a unit's last piece
-        auto score = [&](int r, int key, float dot) {
-            const int nd = quotient(base + r, p.G);
-            const bool sees = (visible_word(p, pc.b, nd, key >> 6) >> (key & 63)) & 1ull;
-            s_own[r][key] = sees ? dot * p.scale_log2 : -INFINITY;
-        };
-        auto pair_dot = [&](int r, int key, int c, int chunks) {  // of 8-column chunks c ..
-            const int nd = quotient(base + r, p.G), hd = hk * p.G + base + r - nd * p.G;
-            const uint4* qp = reinterpret_cast<const uint4*>(p.q + (int64_t)pc.b * p.sq_b + (int64_t)nd * p.sq_n +
-                                                             (int64_t)hd * p.sq_h) + c;
-            const uint4* kp = reinterpret_cast<const uint4*>(p.kn + (int64_t)pc.b * p.sn_b + (int64_t)key * p.sn_n +
-                                                             (int64_t)hk * p.sn_h) + c;
-            float dot = 0.f;
-#pragma unroll 2
-            for (int i = 0; i < chunks; ++i) {
-                const uint4 x = __ldg(qp + i), y = __ldg(kp + i);
-                const uint32_t u[4] = {x.x, x.y, x.z, x.w}, v[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll 1
+        for (int r = warp; r < kRows; r += kWarps) {
+            int seen = 0;
+            if (r < live_rows && own > 0) {
+                const int nd = quotient(base + r, p.G), hd = hk * p.G + base + r - nd * p.G;
+#pragma unroll 1
+                for (int j0 = 0; j0 < own; j0 += 32) {
+                    const bool sees = (visible_word(p, pc.b, nd, j0 >> 6) >> ((j0 & 63) + lane)) & 1ull;
+                    const uint32_t m = __ballot_sync(MFD_FULL_MASK, sees);
+                    if (sees) s_key[r][seen + __popc(m & ((1u << lane) - 1u))] = (uint8_t)(j0 + lane);
+                    seen += __popc(m);
+                }
+                __syncwarp();
+                const int c = lane & 7;
+                const uint4* qp = reinterpret_cast<const uint4*>(p.q + (int64_t)pc.b * p.sq_b + (int64_t)nd * p.sq_n +
+                                                                 (int64_t)hd * p.sq_h + 16 * c);
+                const __nv_bfloat16* kn = p.kn + (int64_t)pc.b * p.sn_b + (int64_t)hk * p.sn_h + 16 * c;
+                const uint4 q0 = __ldg(qp), q1 = __ldg(qp + 1);
+#pragma unroll 1
+                for (int k0 = 0; k0 < seen; k0 += 4) {
+                    const int k = min(k0 + (lane >> 3), seen - 1);
+                    const uint4* kp = reinterpret_cast<const uint4*>(kn + (int64_t)s_key[r][k] * p.sn_n);
+                    const uint4 y0 = __ldg(kp), y1 = __ldg(kp + 1);
+                    const uint32_t u[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
+                    const uint32_t v[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
+                    float dot = 0.f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 f = bf2(u[j]), h = bf2(v[j]);
-                    dot = fmaf(f.x, h.x, fmaf(f.y, h.y, dot));
+                    for (int j = 0; j < 8; ++j) {
+                        const float2 f = bf2(u[j]), h = bf2(v[j]);
+                        dot = fmaf(f.x, h.x, fmaf(f.y, h.y, dot));
+                    }
+#pragma unroll
+                    for (int d = 1; d < 8; d <<= 1) dot += __shfl_xor_sync(MFD_FULL_MASK, dot, d);
+                    if (c == 0) s_own[r][k] = dot * p.scale_log2;
                 }
             }
-            return dot;
-        };
-        // eight lanes a (row, key) pair, or (the last rows of a tree, whose own keys are all its nodes) a thread
-        const int lanes = own > 16 ? 1 : 8;
-#pragma unroll 1
-        for (int e0 = tid / lanes; e0 - (lane / lanes) < live_rows * own; e0 += kThreads / lanes) {
-            const int e = min(e0, live_rows * own - 1);
-            const int key = quotient(e, live_rows), r = e - key * live_rows, c = lane & (lanes - 1);
-            float dot = pair_dot(r, key, 2 * c, 16 / lanes);
-            if (lanes > 1) {
-#pragma unroll 1
-                for (int d = 1; d < 8; d <<= 1) dot += __shfl_xor_sync(MFD_FULL_MASK, dot, d);
-            }
-            if (c == 0) score(r, key, dot);
+            if (lane == 0) s_seen[r] = seen;
         }
 
         // ---- cached tokens
@@ -341,7 +345,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 #pragma unroll 1
         for (int r = warp; r < kRows; r += kWarps) {  // a warp a row: the warps' (m, l), then the own keys
             float mm = lane < kWarps ? s_m[lane][r] : -INFINITY;
-            for (int j = lane; j < own; j += 32) mm = fmaxf(mm, s_own[r][j]);
+            const int seen = s_seen[r];
+            for (int j = lane; j < seen; j += 32) mm = fmaxf(mm, s_own[r][j]);
             mm = warp_max_f32(mm);
             float ll = 0.f;
             if (lane < kWarps) {
@@ -349,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                 ll = s_l[lane][r] * a;  // (a NaN sum stays one)
                 s_m[lane][r] = a;
             }
-            for (int j = lane; j < own; j += 32) {
+            for (int j = lane; j < seen; j += 32) {
                 const float a = s_own[r][j] == -INFINITY ? 0.f : fast_exp2(s_own[r][j] - mm);
                 ll += a;
                 s_own[r][j] = a;
@@ -390,12 +395,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                                                                   (c4 & 3) * 4);
                 v.x = fmaf(a, x.x, v.x), v.y = fmaf(a, x.y, v.y), v.z = fmaf(a, x.z, v.z), v.w = fmaf(a, x.w, v.w);
             }
-#pragma unroll 8
-            for (int j = 0; j < own; ++j) {
+            const __nv_bfloat16* vn = p.vn + (int64_t)pc.b * p.sn_b + (int64_t)hk * p.sn_h + 4 * c4;
+#pragma unroll 4
+            for (int j = 0; j < s_seen[r]; ++j) {
                 const float a = s_own[r][j];
-                uint2 y = __ldg(reinterpret_cast<const uint2*>(p.vn + (int64_t)pc.b * p.sn_b + (int64_t)j * p.sn_n +
-                                                               (int64_t)hk * p.sn_h + 4 * c4));
-                if (a == 0.f) y = make_uint2(0u, 0u);  // what the row does not see has no effect, an infinite value neither
+                const uint2 y = __ldg(reinterpret_cast<const uint2*>(vn + (int64_t)s_key[r][j] * p.sn_n));
                 const float2 f = bf2(y.x), h = bf2(y.y);
                 v.x = fmaf(a, f.x, v.x), v.y = fmaf(a, f.y, v.y), v.z = fmaf(a, h.x, v.z), v.w = fmaf(a, h.y, v.w);
             }
