@@ -210,6 +210,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             int seen = 0;
             if (r < live_rows && own > 0) {
                 const int nd = quotient(base + r, p.G), hd = hk * p.G + base + r - nd * p.G;
+                const int c = lane & 7;
+                const uint4* qp = reinterpret_cast<const uint4*>(p.q + (int64_t)pc.b * p.sq_b + (int64_t)nd * p.sq_n +
+                                                                 (int64_t)hd * p.sq_h + 16 * c);
+                const uint4 q0 = __ldg(qp), q1 = __ldg(qp + 1);
 #pragma unroll 1
                 for (int j0 = 0; j0 < own; j0 += 32) {
                     const bool sees = (visible_word(p, pc.b, nd, j0 >> 6) >> ((j0 & 63) + lane)) & 1ull;
@@ -218,27 +222,35 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                     seen += __popc(m);
                 }
                 __syncwarp();
-                const int c = lane & 7;
-                const uint4* qp = reinterpret_cast<const uint4*>(p.q + (int64_t)pc.b * p.sq_b + (int64_t)nd * p.sq_n +
-                                                                 (int64_t)hd * p.sq_h + 16 * c);
                 const __nv_bfloat16* kn = p.kn + (int64_t)pc.b * p.sn_b + (int64_t)hk * p.sn_h + 16 * c;
-                const uint4 q0 = __ldg(qp), q1 = __ldg(qp + 1);
+                const __nv_bfloat16* vn = p.vn + (int64_t)pc.b * p.sn_b + (int64_t)hk * p.sn_h + 16 * c;
 #pragma unroll 1
-                for (int k0 = 0; k0 < seen; k0 += 4) {
-                    const int k = min(k0 + (lane >> 3), seen - 1);
-                    const uint4* kp = reinterpret_cast<const uint4*>(kn + (int64_t)s_key[r][k] * p.sn_n);
-                    const uint4 y0 = __ldg(kp), y1 = __ldg(kp + 1);
-                    const uint32_t u[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
-                    const uint32_t v[8] = {y0.x, y0.y, y0.z, y0.w, y1.x, y1.y, y1.z, y1.w};
-                    float dot = 0.f;
+                for (int k0 = 0; k0 < seen; k0 += 16) {  // sixteen keys' loads in flight: their latency is the cost
+                    uint4 y[4][2];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float2 f = bf2(u[j]), h = bf2(v[j]);
-                        dot = fmaf(f.x, h.x, fmaf(f.y, h.y, dot));
+                    for (int i = 0; i < 4; ++i) {
+                        const int64_t off = (int64_t)s_key[r][min(k0 + 4 * i + (lane >> 3), seen - 1)] * p.sn_n;
+                        const uint4* kp = reinterpret_cast<const uint4*>(kn + off);
+                        y[i][0] = __ldg(kp), y[i][1] = __ldg(kp + 1);
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(vn + off));  // for the merge
                     }
 #pragma unroll
-                    for (int d = 1; d < 8; d <<= 1) dot += __shfl_xor_sync(MFD_FULL_MASK, dot, d);
-                    if (c == 0) s_own[r][k] = dot * p.scale_log2;
+                    for (int i = 0; i < 4; ++i) {
+                        const int k = k0 + 4 * i + (lane >> 3);
+                        const uint32_t u[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
+                        const uint32_t v[8] = {y[i][0].x, y[i][0].y, y[i][0].z, y[i][0].w,
+                                               y[i][1].x, y[i][1].y, y[i][1].z, y[i][1].w};
+                        float dot = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float2 f = bf2(u[j]), h = bf2(v[j]);
+                            dot = fmaf(f.x, h.x, fmaf(f.y, h.y, dot));
+                        }
+#pragma unroll
+                        for (int d = 1; d < 8; d <<= 1) dot += __shfl_xor_sync(MFD_FULL_MASK, dot, d);
+                        if (c == 0 && k < seen) s_own[r][k] = dot * p.scale_log2;
+                        if (k0 + 4 * i + 4 >= seen) break;  // (uniform)
+                    }
                 }
             }
             if (lane == 0) s_seen[r] = seen;
@@ -396,12 +408,20 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                 v.x = fmaf(a, x.x, v.x), v.y = fmaf(a, x.y, v.y), v.z = fmaf(a, x.z, v.z), v.w = fmaf(a, x.w, v.w);
             }
             const __nv_bfloat16* vn = p.vn + (int64_t)pc.b * p.sn_b + (int64_t)hk * p.sn_h + 4 * c4;
-#pragma unroll 4
-            for (int j = 0; j < s_seen[r]; ++j) {
-                const float a = s_own[r][j];
-                const uint2 y = __ldg(reinterpret_cast<const uint2*>(vn + (int64_t)s_key[r][j] * p.sn_n));
-                const float2 f = bf2(y.x), h = bf2(y.y);
-                v.x = fmaf(a, f.x, v.x), v.y = fmaf(a, f.y, v.y), v.z = fmaf(a, h.x, v.z), v.w = fmaf(a, h.y, v.w);
+            const int seen = s_seen[r];
+#pragma unroll 1
+            for (int j0 = 0; j0 < seen; j0 += 8) {
+                uint2 y[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    y[j] = __ldg(reinterpret_cast<const uint2*>(vn + (int64_t)s_key[r][min(j0 + j, seen - 1)] * p.sn_n));
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (j0 + j >= seen) break;
+                    const float a = s_own[r][j0 + j];
+                    const float2 f = bf2(y[j].x), h = bf2(y[j].y);
+                    v.x = fmaf(a, f.x, v.x), v.y = fmaf(a, f.y, v.y), v.z = fmaf(a, h.x, v.z), v.w = fmaf(a, h.y, v.w);
+                }
             }
             if (whole) {
                 store(r, 4 * c4, v, s_mm[r], s_ll[r]);
