@@ -20,8 +20,9 @@
 //                copied there (past the end of a request: zeros, whatever the page holds)
 //   warp 14      producer: page ids and scales, one TMA load per page and tensor into the raw ring (no multicast)
 //   warp 15      MMA issuer
-// Shared memory: Q (32 KB a row tile), K tile 32 KB, V tiles 2 x 32 KB, raw ring 32 KB a stage.  K needs one buffer: it
-// is free from the last S of its tile to the end of the next PV, and the PV of hi + lo is the longer product.
+// Shared memory: Q (32 KB a row tile), two K and two V tiles of 32 KB, raw codes 32 KB a stage (K's and V's halves filled
+// and freed on their own).  With a second raw stage in the second K tile's place 32 trees of 65 nodes take 401 us, this
+// way 388: the next tile's conversion waits neither for the last S nor the next S for it.
 //
 // Bound: the tensor pipe and shared memory together.  A key tile of 128 costs a pair of row tiles 4 S and 8 PV
 // products of 128 x 128 x 64, 3072 cycles of the tensor pipe at its bf16 rate, and about the same of the
@@ -46,29 +47,29 @@ constexpr int kSoftmaxRegs = 152, kOtherRegs = 104;
 constexpr int kKt = 128;                 // keys per tile
 constexpr int kTileBytes = kKt * kD * 2;  // 32 KB: a bf16 tile, [2 d-halves][128 rows][128 B]
 constexpr int kRawBytes = 2 * kKt * kD;   // 32 KB: the codes of K and V
-constexpr int kRing = 8;                 // tiles of page constants kept
 constexpr uint32_t kTries = 1u << 20;
 
 template <bool PAIR>
 struct Layout {
     static constexpr int kRowTiles = PAIR ? 2 : 1;
-    static constexpr int kStages = PAIR ? 2 : 3;
+    static constexpr int kStages = PAIR ? 1 : 2;  // of raw codes; K's and V's halves are filled and freed on their own
+    static constexpr int kRing = 8;  // tiles of page constants kept (the producer is at most kStages + 3 ahead of a softmax warp)
     static constexpr int kOffQ = 0;
     static constexpr int kOffK = kOffQ + kRowTiles * kTileBytes;
-    static constexpr int kOffV = kOffK + kTileBytes;
+    static constexpr int kOffV = kOffK + 2 * kTileBytes;
     static constexpr int kOffRaw = kOffV + 2 * kTileBytes;
     static constexpr int kOffConst = kOffRaw + kStages * kRawBytes;  // [kRing][8 groups][4] floats: c, d, 1 / sv
     static constexpr int kOffBar = kOffConst + kRing * 8 * 4 * 4;
     static constexpr int kUsed = kOffBar + 512;
     static constexpr int kBytes = kUsed + 1024;  // the base is aligned to 1024 by hand
     static_assert(kBytes <= 227 * 1024, "shared memory");
-    // barriers
+    // barriers; two of each kind that follows the K and V halves of a stage or two buffers
     static constexpr int kQFull = 0;
-    static constexpr int kRawFull = 1;
-    static constexpr int kRawEmpty = kRawFull + kStages;
-    static constexpr int kKFull = kRawEmpty + kStages;
-    static constexpr int kKEmpty = kKFull + 1;
-    static constexpr int kVFull = kKEmpty + 1;
+    static constexpr int kRawFull = 1;  // + 2 stage + (0: K, 1: V)
+    static constexpr int kRawEmpty = kRawFull + 2 * kStages;
+    static constexpr int kKFull = kRawEmpty + 2 * kStages;
+    static constexpr int kKEmpty = kKFull + 2;
+    static constexpr int kVFull = kKEmpty + 2;
     static constexpr int kVEmpty = kVFull + 2;
     static constexpr int kSFull = kVEmpty + 2;
     static constexpr int kPFull = kSFull + 2;
@@ -137,13 +138,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
     if (tid == 0) {
         mbar_init(&bars[L::kQFull], 8);
-        for (int i = 0; i < kStages; ++i) {
+        for (int i = 0; i < 2 * kStages; ++i) {
             mbar_init(&bars[L::kRawFull + i], 32);
             mbar_init(&bars[L::kRawEmpty + i], kConv);
         }
-        mbar_init(&bars[L::kKFull], kConv);
-        mbar_init(&bars[L::kKEmpty], 1);
         for (int i = 0; i < 2; ++i) {
+            mbar_init(&bars[L::kKFull + i], kConv);
+            mbar_init(&bars[L::kKEmpty + i], 1);
             mbar_init(&bars[L::kVFull + i], kConv);
             mbar_init(&bars[L::kVEmpty + i], 1);
             mbar_init(&bars[L::kSFull + i], 1);
@@ -253,7 +254,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 ok = __all_sync(MFD_FULL_MASK, ok & mbar_wait(&bars[L::kSFull + grp], ((grp ? x.n_s1 : x.n_s0) + done) & 1, kTries));
                 tc_fence_after();
                 if (quarter_live && ok) {
-                    const float4* cst = consts + (size_t)((x.n_tile + tile - pc.g0) & (kRing - 1)) * 8;
+                    const float4* cst = consts + (size_t)((x.n_tile + tile - pc.g0) % L::kRing) * 8;
                     // visibility of the tile's keys, 32 a word
                     const int valid = pc.len - tile * kKt;
                     const bool masked = tile >= x.tp || valid < kKt;
@@ -450,19 +451,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             for (int i = 0; i < x.ntiles && ok; ++i) {
                 const int tile = pc.g0 + i;
                 const uint32_t nr = x.n_tile + i, st = nr % kStages;
-                ok &= mbar_wait(&bars[L::kRawFull + st], (nr / kStages) & 1, kTries);
 #pragma unroll 1
-                for (int which = 0; which < 2 && ok; ++which) {
-                    unsigned char* dst;
-                    if (which == 0) {
-                        const uint32_t n = x.n_tile + i;
-                        if (n >= 1) ok &= mbar_wait(&bars[L::kKEmpty], (n - 1) & 1, kTries);
-                        dst = smem + L::kOffK;
-                    } else {
-                        const uint32_t n = x.n_tile + i;
-                        if (n >= 2) ok &= mbar_wait(&bars[L::kVEmpty + (n & 1)], ((n >> 1) - 1) & 1, kTries);
-                        dst = smem + L::kOffV + (n & 1) * kTileBytes;
-                    }
+                for (int which = 0; which < 2 && ok; ++which) {  // K, then V
+                    ok &= mbar_wait(&bars[L::kRawFull + 2 * st + which], (nr / kStages) & 1, kTries);
+                    const int buf = which * 2 + (int)(nr & 1);
+                    if (nr >= 2) ok &= mbar_wait(&bars[(which ? L::kVEmpty : L::kKEmpty) + (nr & 1)], ((nr >> 1) - 1) & 1, kTries);
+                    unsigned char* dst = smem + L::kOffK + buf * kTileBytes;
                     ok = __all_sync(MFD_FULL_MASK, ok);
                     if (!ok) break;
                     if (tile < x.tp) {
@@ -519,8 +513,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
-                        mbar_arrive(which == 0 ? &bars[L::kKFull] : &bars[L::kVFull + ((x.n_tile + i) & 1)]);
-                        if (which == 1) mbar_arrive(&bars[L::kRawEmpty + st]);
+                        mbar_arrive(&bars[(which ? L::kVFull : L::kKFull) + (nr & 1)]);
+                        mbar_arrive(&bars[L::kRawEmpty + 2 * st + which]);
                     }
                 }
             }
@@ -539,37 +533,41 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const int tile = pc.g0 + i;
                 const uint32_t nr = x.n_tile + i, st = nr % kStages;
                 const int id_next = i + 1 < x.ntiles ? id_of(tile + 1) : -1;
-                if (nr >= (uint32_t)kStages) {
-                    ok &= mbar_wait(&bars[L::kRawEmpty + st], (nr / kStages - 1) & 1, kTries);
-                    ok = __all_sync(MFD_FULL_MASK, ok);
+                float4* cst = consts + (size_t)(nr % L::kRing) * 8;
+#pragma unroll 1
+                for (int which = 0; which < 2; ++which) {
+                    uint64_t* bar = &bars[L::kRawFull + 2 * st + which];
+                    if (nr >= (uint32_t)kStages)
+                        ok = __all_sync(MFD_FULL_MASK, ok & mbar_wait(&bars[L::kRawEmpty + 2 * st + which], (nr / kStages - 1) & 1, kTries));
                     if (!ok) break;
+                    if (id >= 0) {
+                        const uint32_t bytes = (uint32_t)(p.c.page * kD);
+                        mbar_expect_tx(bar, bytes);
+                        tma_page(sbase + L::kOffRaw + st * kRawBytes + which * (kRawBytes / 2) + lane * bytes, which ? &tmv : &tmk,
+                                 bar, x.hk, id);
+                    }
+                    if (which == 0 && lane < ppt) {
+                        float4 k = make_float4(p.scale_log2, 0.f, 1.f, 0.f);  // own keys, or behind the request's end
+                        if (id >= 0) {
+                            const float sk = __ldg(p.c.k_scale + (int64_t)id * p.c.Hkv + x.hk);
+                            const float sv = fmaxf(__ldg(p.c.v_scale + (int64_t)id * p.c.Hkv + x.hk), kScaleFloor);
+                            k = make_float4(sk * p.scale_log2, __log2f(sv), __frcp_rn(sv), 0.f);
+                        }
+                        for (int g = 0; g < gpp; ++g) cst[lane * gpp + g] = k;
+                    }
+                    // the lanes without a page arrive last (lanes 8 .. 31 never have one), after every constant is stored
+                    __syncwarp();
+                    if (id < 0) mbar_arrive(bar);
                 }
-                float4* cst = consts + (size_t)(nr & (kRing - 1)) * 8;
-                uint64_t* bar = &bars[L::kRawFull + st];
-                if (id >= 0) {
-                    const uint32_t half = (uint32_t)(p.c.page * kD);
-                    const uint32_t dst = sbase + L::kOffRaw + st * kRawBytes + lane * half;
-                    mbar_expect_tx(bar, 2 * half);
-                    tma_page(dst, &tmk, bar, x.hk, id);
-                    tma_page(dst + kRawBytes / 2, &tmv, bar, x.hk, id);
-                    const float sk = __ldg(p.c.k_scale + (int64_t)id * p.c.Hkv + x.hk);
-                    const float sv = fmaxf(__ldg(p.c.v_scale + (int64_t)id * p.c.Hkv + x.hk), kScaleFloor);
-                    const float4 k = make_float4(sk * p.scale_log2, __log2f(sv), __frcp_rn(sv), 0.f);
-                    for (int g = 0; g < gpp; ++g) cst[lane * gpp + g] = k;
-                } else if (lane < ppt) {
-                    const float4 k = make_float4(p.scale_log2, 0.f, 1.f, 0.f);  // own keys, or behind the request's end
-                    for (int g = 0; g < gpp; ++g) cst[lane * gpp + g] = k;
-                }
-                // the lanes without a page arrive last (lanes 8 .. 31 never have one), after every constant is stored
-                __syncwarp();
-                if (id < 0) mbar_arrive(bar);
+                if (!ok) break;
                 id = id_next;
                 issued = nr + 1;
             }
             });
             if (*s_failed)  // copies in flight end before the CTA does (bounded)
                 for (uint32_t f = issued > kStages ? issued - kStages : 0u; f < issued; ++f)
-                    mbar_wait(&bars[L::kRawFull + f % kStages], (f / kStages) & 1, 1u << 14);
+                    for (int which = 0; which < 2; ++which)
+                        mbar_wait(&bars[L::kRawFull + 2 * (f % kStages) + which], (f / kStages) & 1, 1u << 14);
         } else {
             // The whole warp walks the steps and one elected lane issues, by predicate: control flow and descriptors stay
             // uniform, so the operands of an instruction are immediates and uniform registers (a single lane in a branch of
@@ -586,16 +584,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 };
                 auto scores = [&](int s) {
                     const int i = x.alternate ? s : s >> 1, grp = s & 1;
-                    if (x.alternate || grp == 0) wait(L::kKFull, (x.n_tile + i) & 1);
+                    const uint32_t nk = x.n_tile + i;
+                    if (x.alternate || grp == 0) wait(L::kKFull + (nk & 1), (nk >> 1) & 1);
                     if (!ok) return;
+                    const uint64_t k = kd + (uint64_t)((nk & 1) * (kTileBytes >> 4));
                     const uint64_t q = qd + (uint64_t)(x.alternate || grp == 0 ? 0 : kTileBytes >> 4);
 #pragma unroll
                     for (int ks = 0; ks < 8; ++ks) {
                         const uint64_t off = (uint64_t)(((ks >> 2) * (kTileBytes / 2) + (ks & 3) * 32) >> 4);
-                        umma_if(leader, tmem + 256 + 128 * grp, q + off, kd + off, kIdescS, ks > 0);
+                        umma_if(leader, tmem + 256 + 128 * grp, q + off, k + off, kIdescS, ks > 0);
                     }
                     commit_if(leader, &bars[L::kSFull + grp]);
-                    if (x.alternate || grp == 1) commit_if(leader, &bars[L::kKEmpty]);
+                    if (x.alternate || grp == 1) commit_if(leader, &bars[L::kKEmpty + (nk & 1)]);
                 };
                 if (x.nsteps > 0) wait(L::kQFull, x.n_piece & 1);
                 if (x.nsteps > 0 && ok) scores(0);
