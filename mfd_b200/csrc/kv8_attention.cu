@@ -126,13 +126,17 @@ extern "C" int mfd_kv8_attention(const void* q, int64_t sq_b, int64_t sq_n, int6
     p.tickets = tickets;
     const int sms = kv8::sm_count(), rows = p.rows;
     cudaStream_t s = (cudaStream_t)stream;
-    if (rows <= kRowsAlone && p.nn <= kv8::kRowsMaxOwn) return kv8::launch_rows(p, sms, s);
-    // pairs of 128-row tiles; a remainder of a few rows goes to the register kernel instead of a tile of padding
+    if (rows <= kRowsAlone) return kv8::launch_rows(p, sms, s);
+    // Pairs of 128-row tiles; a remainder of a few rows goes to the register kernel instead of a tile of padding (32
+    // requests of 4096 tokens, 65 nodes x 4 heads: 309 against 362 us).
     const int rest = rows % 256;
     const bool tail = rows > 256 && rest > 0 && rest <= kRowsAlone && p.nn <= kv8::kRowsMaxOwn;
-    // With few units a second and a third launch cost more than the padding: one row tile a CTA, the last one mostly
-    // empty (65 nodes x 4 heads over 4096 tokens: 33 against 62 us at 1 request, 46 against 64 at 2).
-    if (tail && bs * num_kv_heads * ((rows + 255) / 256) <= sms / 4) return kv8::launch_tc(p, false, sms, s);
+    // With few units one row tile a CTA.  In place of a second and a third launch the last tile is mostly empty (65 nodes
+    // x 4 heads over 4096 tokens: 32 against 60 us at 1 request of 8 KV heads, 43 against 60 at 2, 77 against 76 at 4); in
+    // place of pairs more CTAs share the keys (64 nodes x 4 heads, 1 request: 29 against 36 us over 4096 tokens, 53
+    // against 58 over 16384; at 2 requests 39 against 39 and 90 against 77).
+    const int64_t pairs = bs * num_kv_heads * ((rows + 255) / 256);
+    if (pairs <= sms / (tail ? 4 : 16)) return kv8::launch_tc(p, false, sms, s);
     if (tail) p.rows = rows - rest;
     st = kv8::launch_tc(p, rows > 128, sms, s);
     if (st != MFD_OK || !tail) return st;

@@ -43,6 +43,7 @@ constexpr int kRingBytes = kWarps * kStages * kStageBytes;
 constexpr int kDBlock = 20, kRowStride = 8 * kDBlock + 4;
 constexpr int kSlot = 16 * (kD + 2);  // floats of a partial: m[16], l[16], O[16][128]
 constexpr int kCtasPerSm = 2;
+constexpr int kMaxPieces = 512;   // of a unit: at most one a CTA
 constexpr float kLift = 12.f;  // the largest weights are 2^12, and up to 2^15 before the reference moves
 constexpr float kLazy = 3.f;
 constexpr int kMaxOwn = kRowsMaxOwn;  // own keys a request
@@ -440,46 +441,54 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             if (s_last) {
                 __threadfence();
                 auto record = [&](int i) { return p.part + (int64_t)slot_of(pc, i) * kSlot; };
-                float* wgt = smem;  // [pieces][16] weights
-                constexpr int kBatch = 512;
-                float4 v[2];
-                v[0] = v[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                float* wgt = smem;  // [pieces][16]: the pieces' m, then their weights
+                float* sum = smem + kMaxPieces * 16;  // and l
+                const int held = pc.pieces * 16;
+#pragma unroll 2
+                for (int e = tid; e < held; e += kThreads) {
+                    const float* rec = record(e >> 4) + (e & 15);
+                    wgt[e] = __ldcg(rec), sum[e] = __ldcg(rec + 16);  // (rows that are not live: never used)
+                }
+                __syncthreads();
+#pragma unroll 1
                 for (int r = warp; r < live_rows; r += kWarps) {
-                    float mm = -INFINITY;
-                    for (int i = lane; i < pc.pieces; i += 32) mm = fmaxf(mm, __ldcg(record(i) + r));
+                    float mm = -INFINITY, ll = 0.f;
+                    for (int i = lane; i < pc.pieces; i += 32) mm = fmaxf(mm, wgt[i * 16 + r]);
                     mm = warp_max_f32(mm);
-                    float ll = 0.f;
                     for (int i = lane; i < pc.pieces; i += 32) {
-                        const float mi = __ldcg(record(i) + r);
-                        const float a = mi == -INFINITY ? 0.f : fast_exp2(mi - mm);
-                        if (i < kBatch) wgt[i * 16 + r] = a;
-                        ll += a * __ldcg(record(i) + 16 + r);
+                        const float mi = wgt[i * 16 + r], a = mi == -INFINITY ? 0.f : fast_exp2(mi - mm);
+                        wgt[i * 16 + r] = a;
+                        ll += a * sum[i * 16 + r];
                     }
 #pragma unroll
                     for (int d = 16; d; d >>= 1) ll += __shfl_xor_sync(MFD_FULL_MASK, ll, d);
                     if (lane == 0) s_mm[r] = mm, s_ll[r] = ll;
                 }
-                __syncthreads();
+                __syncwarp();
+                // (a warp's rows are the same here: warp, and warp + 8)
+                if (warp < live_rows) {
+                    float4 v[NT];
+                    int row[NT];
 #pragma unroll
-                for (int u = 0; u < kRows * 32 / kThreads; ++u) {
-                    const int e = tid + u * kThreads;
-                    const int r = e >> 5, c4 = e & 31;
-                    if (r < live_rows) {
-#pragma unroll 4
-                        for (int i = 0; i < pc.pieces; ++i) {
-                            const float* sl = record(i);
-                            float a;
-                            if (i < kBatch) {
-                                a = wgt[i * 16 + r];
-                            } else {
-                                const float mi = __ldcg(sl + r);
-                                a = mi == -INFINITY ? 0.f : fast_exp2(mi - s_mm[r]);
-                            }
-                            const float4 x = __ldcg(reinterpret_cast<const float4*>(sl + 32 + r * kD + 4 * c4));
+                    for (int u = 0; u < NT; ++u) {
+                        v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        row[u] = min(warp + u * kWarps, live_rows - 1);
+                    }
+#pragma unroll 8
+                    for (int i = 0; i < pc.pieces; ++i) {
+                        const float* rec = record(i) + 32 + 4 * lane;
+#pragma unroll
+                        for (int u = 0; u < NT; ++u) {
+                            const float a = wgt[i * 16 + row[u]];
+                            const float4 x = __ldcg(reinterpret_cast<const float4*>(rec + row[u] * kD));
                             v[u].x = fmaf(a, x.x, v[u].x), v[u].y = fmaf(a, x.y, v[u].y);
                             v[u].z = fmaf(a, x.z, v[u].z), v[u].w = fmaf(a, x.w, v[u].w);
                         }
-                        store(r, 4 * c4, v[u], s_mm[r], s_ll[r]);
+                    }
+#pragma unroll
+                    for (int u = 0; u < NT; ++u) {
+                        const int r = warp + u * kWarps;
+                        if (r < live_rows) store(r, 4 * lane, v[u], s_mm[r], s_ll[r]);
                     }
                 }
                 if (tid == 0) *ticket = 0u;
@@ -494,14 +503,15 @@ size_t rows_workspace(int sms) { return (size_t)sms * kCtasPerSm * 2 * kSlot * s
 
 template <bool FP8, int NT>
 static int launch_one(const AttnParams& p, int sms, cudaStream_t stream) {
-    static_assert(kWarps * 8 * NT * kRowStride * 4 <= kRingBytes && 512 * 16 * 4 <= kRingBytes, "the merge fits the ring");
+    static_assert(kWarps * 8 * NT * kRowStride * 4 <= kRingBytes && kMaxPieces * 2 * 16 * 4 <= kRingBytes, "the merge fits the ring");
     static bool opted[64];
     cudaError_t e = opt_in_smem((const void*)kv8_rows_kernel<FP8, NT>, kRingBytes, opted);
     if (e != cudaSuccess) {
         set_error("mfd_kv8_attention: %s", cudaGetErrorString(e));
         return MFD_ERR_CUDA;
     }
-    kv8_rows_kernel<FP8, NT><<<sms * kCtasPerSm, kThreads, kRingBytes, stream>>>(p);
+    const int ctas = sms * kCtasPerSm < kMaxPieces ? sms * kCtasPerSm : kMaxPieces;
+    kv8_rows_kernel<FP8, NT><<<ctas, kThreads, kRingBytes, stream>>>(p);
     MFD_CHECK_LAUNCH("mfd_kv8_attention");
     return MFD_OK;
 }
