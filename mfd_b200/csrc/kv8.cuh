@@ -137,22 +137,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                         uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ uint4 ldg_stream_u4(const void* p) {
-    uint4 r;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-                 : "l"(p));
-    return r;
-}
-
 // One asynchronous 16-byte copy into shared memory, and the groups they are waited for in.
 __device__ __forceinline__ void copy16(void* dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
@@ -194,8 +178,8 @@ __device__ __forceinline__ int quotient(int a, int b) {
     return q;
 }
 
-// Work laid end to end over the requests, f(length) * mul (or f(length, request) * mul) of it for each (below 2^31 in all: the entry points check);
-// every warp finds its place by itself.  The lengths of the first 32 requests stay in the lanes' registers.
+// Work laid end to end over the requests, f(length) * mul (or f(length, request) * mul) of it for each (below 2^31 in all:
+// the entry points check); every warp finds its place by itself.  The lengths of the first 32 requests stay in the lanes' registers.
 struct Lengths {
     const Cache& c;
     int bs, mine;

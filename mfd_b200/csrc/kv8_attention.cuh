@@ -30,8 +30,8 @@ struct AttnParams {
     int* status;
 };
 
-// TMA map of a cache tensor's codes: (128, page, KV heads, pages), one page of one head a box (swizzle: 128-byte)
-bool make_page_map(CUtensorMap* m, const uint8_t* base, const Cache& c, bool swizzle);
+// TMA map of a cache tensor's codes: (128, page, KV heads, pages), one page of one head a box
+bool make_page_map(CUtensorMap* m, const uint8_t* base, const Cache& c);
 __device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int head, int page) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
@@ -44,7 +44,7 @@ __device__ __forceinline__ void bar_sync(int id) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
 }
 
-// Own keys the register kernel takes (more rows' trees go to the tensor-core kernel).
+// Own keys a request the register kernel holds in shared memory (larger trees go to the tensor-core kernel).
 constexpr int kRowsMaxOwn = 128;
 // rows [p.row0, p.rows) with the register kernel (16 rows a unit)
 int launch_rows(const AttnParams& p, int sms, cudaStream_t stream);

@@ -687,7 +687,7 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(const AttnParams p, in
 template <bool FP8, bool PAIR>
 int launch_tc_one(const AttnParams& p, int sms, cudaStream_t stream) {
     CUtensorMap tk, tv;
-    if (!make_page_map(&tk, p.c.k, p.c, false) || !make_page_map(&tv, p.c.v, p.c, false)) {
+    if (!make_page_map(&tk, p.c.k, p.c) || !make_page_map(&tv, p.c.v, p.c)) {
         set_error("mfd_kv8_attention: could not encode the TMA tensor maps");
         return MFD_ERR_CUDA;
     }

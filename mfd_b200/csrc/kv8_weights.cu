@@ -14,8 +14,14 @@
 // chains of products.
 //
 // Split: the tiles of all (request, KV head) units are laid end to end by their cost (tokens, and rows that pass them) and
-// cut into equal ranges, one per CTA, so ragged lengths and counts balance.  Each 16 tokens' sum goes to the workspace; the CTA that finishes a request last adds them up per
-// page, in a fixed order over tokens and heads (no float atomics).
+// cut into equal ranges, one per CTA, so ragged lengths and counts balance.  Each 16 tokens' sum goes to the workspace; the
+// CTA that finishes a request last adds them up per page, in a fixed order over tokens and heads (no float atomics).
+//
+// Measured (H 32 over 8 KV heads, paths of 17 of 65 nodes: 68 rows a KV head): one request of 4096 tokens 14.4 us, where
+// launch, prologue and the last CTA's sum are nearly all; 32 requests of 1K - 8K tokens 64 us, 2.2 TB/s of codes.  There one
+// listed row takes 43 of the 64 us of 68 rows (32 requests of 4096 tokens): the rest is the products at the legacy tensor
+// rate.  The same on tcgen05 (keys as rows of a 128-wide product, codes to bf16 tiles by warps of their own) ran 69 us
+// with two CTAs an SM and 81 with one: turning the codes into operand tiles took what the products gave.
 #include "kv8.cuh"
 
 namespace mfd {
@@ -266,12 +272,21 @@ __global__ void __launch_bounds__(kWThreads, kWCtasPerSm)
                 const int pages = (len + p.c.page - 1) >> p.c.page_shift, groups = (len + 15) / 16;
                 const int gpp = p.c.page / 16;
                 const float* src = p.part + (int64_t)b * p.groups_max * Hkv;
+                const bool wide = (gpp * Hkv) % 4 == 0;
                 for (int i = tid; i < p.c.max_pages; i += kWThreads) {
                     float v = 0.f;
                     if (i < pages) {
-                        const int n0 = i * gpp * Hkv, n1 = min((i + 1) * gpp, groups) * Hkv;
+                        int e = i * gpp * Hkv;
+                        const int stop = min((i + 1) * gpp, groups) * Hkv;
+                        if (wide) {  // (the page's sums are contiguous: one latency for 32 of them)
 #pragma unroll 8
-                        for (int e = n0; e < n1; ++e) v += __ldcg(src + e);
+                            for (; e + 4 <= stop; e += 4) {
+                                const float4 x = __ldcg(reinterpret_cast<const float4*>(src + e));
+                                v += (x.x + x.y) + (x.z + x.w);
+                            }
+                        }
+#pragma unroll 8
+                        for (; e < stop; ++e) v += __ldcg(src + e);
                         v = fmaf(p.mass[(int64_t)b * p.mass_stride + i], p.decay, v);  // (out may be mass)
                     }
                     p.out[(int64_t)b * p.mass_stride + i] = v;
