@@ -310,9 +310,9 @@ __device__ __forceinline__ bool next_piece(const Lengths& lens, F f, const Cut& 
 __device__ __forceinline__ int slot_of(const Piece& pc, int i) {
     return 2 * (pc.first + i) + (pc.second && i == 0 ? 1 : 0);
 }
-// whether all requests at their capacity are less than 2^31 pieces of work of `tokens` each (host)
+// whether all requests at their capacity are less than 2^31 pieces of work of `tokens` each, and a few a unit (host)
 inline bool work_fits(int64_t bs, int64_t per_req, int64_t max_pages, int64_t page, int64_t tokens) {
-    const double all = (double)bs * (double)per_req * ((double)max_pages * (double)page / (double)tokens + 2.0);
+    const double all = (double)bs * (double)per_req * ((double)max_pages * (double)page / (double)tokens + 16.0);
     return all < 2147483648.0;
 }
 

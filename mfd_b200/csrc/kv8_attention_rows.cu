@@ -7,7 +7,8 @@
 // and float32 sums: codes are exact there, and so is the query row divided by a power of two.  The weights go in as
 // float16 hi + lo, two tensor instructions, lifted to at most 2^15: 22 bits of a weight, down to 2^-37 of the row's
 // largest.  (One float16 or bf16 weight would err by a good part of the output's own rounding.)  The nodes' own bf16
-// keys and values take bf16 operands, the weights hi + lo as well.  All sums and statistics are float32.
+// keys and values are few: float32 products on the CUDA cores, of the keys a row sees, joined at the piece's merge.  All
+// sums and statistics are float32.
 //
 // Bound: bytes (256 codes a token and KV head for 4 G n multiply-adds each); next, instructions: turning the codes into
 // operands.  The codes are the wide operand of the tensor instruction and the query rows, which are few, the narrow one,
@@ -27,6 +28,11 @@
 // ragged lengths balance and one long request fills the GPU; the lengths are read on the device.  The nodes' own keys
 // belong to a unit's last piece.  A unit cut into pieces is merged by the CTA that finishes last (its partial (m, l, O) in
 // the workspace, a ticket per unit; the pieces are added in their order, so the result does not depend on who merges).
+// It reads all pieces of its rows together: one after another they took 8 us of the 21 of a request of 4096 tokens (now
+// 12.5).
+//
+// Measured (H 32 over 8 KV heads, one node): a request of 1000 tokens 10 us, launch and latency; 131072 tokens 62 us, 4.3 TB/s;
+// 64 requests of 1K - 8K tokens 126 us, 5.1 TB/s of codes, 0.79 of a copy's bandwidth.
 #include "kv8_attention.cuh"
 #include "tcgen05.cuh"
 
@@ -44,6 +50,10 @@ constexpr int kDBlock = 20, kRowStride = 8 * kDBlock + 4;
 constexpr int kSlot = 16 * (kD + 2);  // floats of a partial: m[16], l[16], O[16][128]
 constexpr int kCtasPerSm = 2;
 constexpr int kMaxPieces = 512;   // of a unit: at most one a CTA
+// What a unit's start and merge, and its own keys, take in tiles (below).  Without them the CTAs that get several short
+// requests end last: 64 requests of 1K - 8K tokens 139 us, with them 126; the 4 rows over the pairs of 32 trees of 65 nodes 103
+// and 77.
+constexpr int kUnitTiles = 4, kOwnTiles = 6;
 constexpr float kLift = 12.f;  // the largest weights are 2^12, and up to 2^15 before the reference moves
 constexpr float kLazy = 3.f;
 constexpr int kMaxOwn = kRowsMaxOwn;  // own keys a request
@@ -67,7 +77,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     const int nrows = p.rows - p.row0;
     const int RB = (nrows + 15) / 16;
     // ---- this CTA's share of the work, in tiles
-    auto tiles_of = [](int len) { return max(1, (len + kTile - 1) / kTile); };  // (one, for the own keys or to write zeros)
+    // (at least one, for the own keys or to write zeros; of many units, which share CTAs, each counts kUnitTiles more for
+    // its start and merge and kOwnTiles for its own keys)
+    const int more = p.bs * p.c.Hkv * RB > (int)gridDim.x / 2 ? kUnitTiles + max(0, min(p.nn - 1, kOwnTiles)) : 0;
+    auto tiles_of = [&](int len) { return max(1, (len + kTile - 1) / kTile) + more; };
     const Lengths lens(p.c, p.bs);
     const Cut cut = make_cut(lens, tiles_of, p.c.Hkv * RB, gridDim.x);
     int pos, end;
@@ -206,6 +219,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         // lane.  The weights meet the values in the merge below.
         const int live_rows = min(16, p.rows - base);
         const int own = pc.g1 == pc.of ? p.nn : 0;  // of a unit's last piece
+        auto own_words = [&](int r) {  // lane w: word w of what the row sees
+            return lane < kMaxOwn / 64 ? visible_word(p, pc.b, quotient(base + r, p.G), lane) : 0ull;
+        };
 #pragma unroll 1
         for (int r = warp; r < kRows; r += kWarps) {
             int seen = 0;
@@ -215,9 +231,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                 const uint4* qp = reinterpret_cast<const uint4*>(p.q + (int64_t)pc.b * p.sq_b + (int64_t)nd * p.sq_n +
                                                                  (int64_t)hd * p.sq_h + 16 * c);
                 const uint4 q0 = __ldg(qp), q1 = __ldg(qp + 1);
+                const uint64_t word = own_words(r);
 #pragma unroll 1
                 for (int j0 = 0; j0 < own; j0 += 32) {
-                    const bool sees = (visible_word(p, pc.b, nd, j0 >> 6) >> ((j0 & 63) + lane)) & 1ull;
+                    const uint64_t v = __shfl_sync(MFD_FULL_MASK, word, j0 >> 6);
+                    const bool sees = (v >> ((j0 & 63) + lane)) & 1ull;
                     const uint32_t m = __ballot_sync(MFD_FULL_MASK, sees);
                     if (sees) s_key[r][seen + __popc(m & ((1u << lane) - 1u))] = (uint8_t)(j0 + lane);
                     seen += __popc(m);
@@ -411,13 +429,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             const __nv_bfloat16* vn = p.vn + (int64_t)pc.b * p.sn_b + (int64_t)hk * p.sn_h + 4 * c4;
             const int seen = s_seen[r];
 #pragma unroll 1
-            for (int j0 = 0; j0 < seen; j0 += 8) {
-                uint2 y[8];
+            for (int j0 = 0; j0 < seen; j0 += 16) {
+                uint2 y[16];
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
+                for (int j = 0; j < 16; ++j)
                     y[j] = __ldg(reinterpret_cast<const uint2*>(vn + (int64_t)s_key[r][min(j0 + j, seen - 1)] * p.sn_n));
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
+                for (int j = 0; j < 16; ++j) {
                     if (j0 + j >= seen) break;
                     const float a = s_own[r][j0 + j];
                     const float2 f = bf2(y[j].x), h = bf2(y[j].y);

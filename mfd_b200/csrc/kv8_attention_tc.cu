@@ -26,7 +26,13 @@
 //
 // Bound: the tensor pipe and shared memory together.  A key tile of 128 costs a pair of row tiles 4 S and 8 PV
 // products of 128 x 128 x 64, 3072 cycles of the tensor pipe at its bf16 rate, and about the same of the
-// 128 B/clk shared-memory port (operands 256 KB, conversion 96 KB, raw codes 32 KB); the exponentials are 2048.
+// 128 B/clk shared-memory port (operands 256 KB, conversion 96 KB, raw codes 32 KB); the exponentials are 2048.  A tile
+// takes about 6000: the products of a group, its softmax and the next products follow one another, and two groups fill
+// half of the gaps.  Sixteen softmax warps instead of eight (two a row quarter) ran 5% slower, and so did loads of the next
+// scores ahead of the exponentials.
+//
+// Measured (H 32 over 8 KV heads): 64 nodes, 32 requests of 1K - 8K tokens 250 us with the combination, 0.59 PFLOP/s of
+// 4 D flop a score (0.89 with the second product of the weights); 65 nodes, one request of 4096 tokens 32 us.
 //
 // Split: as in kv8_attention_rows.cu, in key tiles of 128: equal ranges of all units' tiles laid end to end, or at most
 // one piece a CTA when there are few units.  Pieces leave (m, l, O) and kv8_combine_kernel adds them in order, spread
@@ -48,6 +54,13 @@ constexpr int kKt = 128;                 // keys per tile
 constexpr int kTileBytes = kKt * kD * 2;  // 32 KB: a bf16 tile, [2 d-halves][128 rows][128 B]
 constexpr int kRawBytes = 2 * kKt * kD;   // 32 KB: the codes of K and V
 constexpr uint32_t kTries = 1u << 20;
+// Tiles of a unit as the cut counts them.  Many units share CTAs, and there a unit counts kUnitTiles more than it has, for
+// its queries and its epilogue: otherwise the CTAs that get several short requests end last (32 trees of 65 nodes over 1K
+// - 8K tokens 273 us, this way 237).
+constexpr int kUnitTiles = 3;
+__device__ __forceinline__ int counted_tiles(const AttnParams& p, int len, int units, int ctas) {
+    return max(1, (len + kKt - 1) / kKt + (p.nn + kKt - 1) / kKt) + (units > ctas / 2 ? kUnitTiles : 0);
+}
 
 template <bool PAIR>
 struct Layout {
@@ -165,7 +178,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t tmem = *tmem_slot;
     // TMEM columns: O of group t at 128 t, S of group t at 256 + 128 t
     const int RB = (p.rows - p.row0 + 128 * L::kRowTiles - 1) / (128 * L::kRowTiles);
-    auto tiles_of = [&](int len) { return max(1, (len + kKt - 1) / kKt + (p.nn + kKt - 1) / kKt); };
+    auto tiles_of = [&](int len) { return counted_tiles(p, len, p.bs * p.c.Hkv * RB, gridDim.x); };
     const Lengths lens(p.c, p.bs);
     const Cut cut = make_cut(lens, tiles_of, p.c.Hkv * RB, gridDim.x);
     int pos, end;
@@ -181,7 +194,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             Tiles x;
             x.hk = pc.u / RB, x.rb = pc.u % RB;
             x.tp = (pc.len + kKt - 1) / kKt;
-            x.t1 = min(pc.g1, x.tp + (p.nn + kKt - 1) / kKt);  // (a unit without keys has one empty tile)
+            x.t1 = min(pc.g1, x.tp + (p.nn + kKt - 1) / kKt);  // (counted tiles that there are not are empty)
             x.ntiles = max(0, x.t1 - pc.g0);
             x.row_base = p.row0 + x.rb * 128 * L::kRowTiles;
             x.ntl = PAIR ? (p.rows - x.row_base > 128 ? 2 : 1) : 1;
@@ -639,7 +652,7 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(const AttnParams p, in
     constexpr int kRowsU = kSlotRows(PAIR);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
     const int RB = (p.rows - p.row0 + kRowsU - 1) / kRowsU;
-    auto tiles_of = [&](int len) { return max(1, (len + kKt - 1) / kKt + (p.nn + kKt - 1) / kKt); };
+    auto tiles_of = [&](int len) { return counted_tiles(p, len, p.bs * p.c.Hkv * RB, ctas); };
     const Lengths lens(p.c, p.bs);
     const Cut cut = make_cut(lens, tiles_of, p.c.Hkv * RB, ctas);
     int pos, end;
