@@ -391,6 +391,13 @@ int mfd_kv8_evict(const int32_t* page_table, const float* mass, const int32_t* s
                   int32_t* table_out, float* mass_out, int32_t* new_lens, int32_t* freed, int32_t* freed_counts,
                   void* stream);
 
+/*
+ * One of the four operators above with its arguments in an array: count 64-bit words in the order of the operator's
+ * parameters, pointers and integers as such, floats as doubles.  For callers that pay for each argument of a foreign call.
+ */
+enum { MFD_KV8_APPEND = 0, MFD_KV8_ATTENTION = 1, MFD_KV8_PAGE_WEIGHTS = 2, MFD_KV8_EVICT = 3 };
+int mfd_kv8_call(int op, const void* words, int64_t count);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,7 +9,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._lib import MFD_BF16, MFD_E4M3, MFD_F32, MFD_I8, MFD_I32, MFD_I64, Workspace, check, device_index, ptr, raw_stream, require_cuda, stream_ptr
+from ._lib import (MFD_BF16, MFD_E4M3, MFD_F32, MFD_I8, MFD_I32, MFD_I64, Workspace, address, check, device_index, packed,
+                   ptr, raw_stream, require_cuda, stream_ptr)
 
 
 def _ids_code(dtype: torch.dtype) -> int:
@@ -592,6 +593,10 @@ def conv_commit(conv_states, xs, window) -> None:
 
 _KV8_CODES = {torch.int8: MFD_I8, torch.float8_e4m3fn: MFD_E4M3}
 
+# (in the order of include/mfd_b200.h)
+_kv8_append_c, _kv8_attention_c, _kv8_page_weights_c, _kv8_evict_c = (
+    packed("mfd_kv8_" + name, op) for op, name in enumerate(("append", "attention", "page_weights", "evict")))
+
 
 def _kv8_check(what: str, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens):
     """The cache's checks; its shape, strides and code type, and the table's shape."""
@@ -665,11 +670,11 @@ def kv8_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tens
         new_lens = torch.empty_like(seq_lens)
     elif new_lens.dtype != torch.int32 or new_lens.shape != seq_lens.shape or not new_lens.is_contiguous():
         raise RuntimeError("kv8_append: new_lens must be contiguous int32 [bs]")
-    rc = _lib.lib().mfd_kv8_append(k_cache.data_ptr(), v_cache.data_ptr(), sc[0], sc[1], sc[2], code,
-                                   k_scale.data_ptr(), v_scale.data_ptr(), pages, page, page_table.data_ptr(),
-                                   page_table.stride(0), width, seq_lens.data_ptr(), k_new.data_ptr(),
-                                   v_new.data_ptr(), sn[0], sn[1], sn[2], n, ptr(path), path_stride, rows, ptr(counts),
-                                   bs, hkv, d, new_lens.data_ptr(), ptr(status), raw_stream(dev))
+    rc = _kv8_append_c(k_cache.data_ptr(), v_cache.data_ptr(), sc[0], sc[1], sc[2], code, k_scale.data_ptr(),
+                       v_scale.data_ptr(), pages, page, page_table.data_ptr(), page_table.stride(0), width,
+                       seq_lens.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), sn[0], sn[1], sn[2], n, address(path),
+                       path_stride, rows, address(counts), bs, hkv, d, new_lens.data_ptr(), address(status),
+                       raw_stream(dev))
     check(rc, "mfd_kv8_append")
     return new_lens
 
@@ -712,12 +717,12 @@ def kv8_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
         raise RuntimeError(f"kv8_attention: q must be [bs, n, H, D] for {bs} requests, D = {d}; got {tuple(shape)}")
     _, n, H, _ = shape
     sq = _kv8_rows("kv8_attention", q, "q", shape)
-    sn, kn, vn = (0, 0, 0), None, None
+    sn, kn, vn = (0, 0, 0), 0, 0
     if k_new is not None and v_new is not None:
         sn, kn, vn = _kv8_new("kv8_attention", k_new, v_new, (bs, n, hkv, d)), k_new.data_ptr(), v_new.data_ptr()
     elif k_new is not v_new:
         raise RuntimeError("kv8_attention: k_new and v_new come together")
-    ab, words = None, 0
+    ab, words = 0, 0
     if anc is not None:
         if anc.dtype != torch.int64 or anc.dim() != 3 or anc.shape[:2] != shape[:2] or not anc.is_contiguous():
             raise RuntimeError("kv8_attention: anc must be contiguous int64 [bs, n, words]")
@@ -727,19 +732,19 @@ def kv8_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
         so = (n * H * d, H * d, d)
     else:
         so = _kv8_rows("kv8_attention", out, "out", shape)
-    lse, lse_ptr = None, None
+    lse, lse_ptr = None, 0
     if return_lse:
-        lse = torch.empty((bs, n, H), dtype=torch.float32, device=q.device)
+        lse = torch.empty_strided(shape[:3], (n * H, H, 1), dtype=torch.float32, device=q.device)
         lse_ptr = lse.data_ptr()
     L = _lib.lib()
     stream = raw_stream(dev)
     scratch = _kv8_scratch(q.device, stream, "kv8_attn", (bs, n, H, hkv),
                            lambda: (L.mfd_kv8_attention_workspace(bs, n, H, hkv),
                                     L.mfd_kv8_attention_tickets(bs, n, H, hkv)))
-    rc = L.mfd_kv8_attention(q.data_ptr(), sq[0], sq[1], sq[2], k_cache.data_ptr(), v_cache.data_ptr(), sc[0], sc[1],
-                             sc[2], code, k_scale.data_ptr(), v_scale.data_ptr(), pages, page, page_table.data_ptr(),
-                             page_table.stride(0), width, seq_lens.data_ptr(), kn, vn, sn[0], sn[1], sn[2], ab, words,
-                             bs, n, H, hkv, d, scale, out.data_ptr(), so[0], so[1], so[2], lse_ptr, *scratch, stream)
+    rc = _kv8_attention_c(q.data_ptr(), sq[0], sq[1], sq[2], k_cache.data_ptr(), v_cache.data_ptr(), sc[0], sc[1],
+                          sc[2], code, k_scale.data_ptr(), v_scale.data_ptr(), pages, page, page_table.data_ptr(),
+                          page_table.stride(0), width, seq_lens.data_ptr(), kn, vn, sn[0], sn[1], sn[2], ab, words, bs,
+                          n, H, hkv, d, scale, out.data_ptr(), so[0], so[1], so[2], lse_ptr, *scratch, stream)
     check(rc, "mfd_kv8_attention")
     return (out, lse) if return_lse else out
 
@@ -786,11 +791,10 @@ def kv8_page_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, 
     stream = raw_stream(dev)
     scratch = _kv8_scratch(q.device, stream, "kv8_weights", (bs, width, page, hkv),
                            lambda: (L.mfd_kv8_page_weights_workspace(bs, width, page, hkv), bs))
-    rc = L.mfd_kv8_page_weights(q.data_ptr(), sq[0], sq[1], sq[2], lse.data_ptr(), k_cache.data_ptr(), sc[0], sc[1],
-                                sc[2], code, k_scale.data_ptr(), pages, page, page_table.data_ptr(),
-                                page_table.stride(0), width, seq_lens.data_ptr(), ptr(path), path_stride, rows,
-                                ptr(counts), bs, n, H, hkv, d, scale, decay, mass.data_ptr(), out.data_ptr(), width, *scratch,
-                                stream)
+    rc = _kv8_page_weights_c(q.data_ptr(), sq[0], sq[1], sq[2], lse.data_ptr(), k_cache.data_ptr(), sc[0], sc[1],
+                             sc[2], code, k_scale.data_ptr(), pages, page, page_table.data_ptr(), page_table.stride(0),
+                             width, seq_lens.data_ptr(), address(path), path_stride, rows, address(counts), bs, n, H,
+                             hkv, d, scale, decay, mass.data_ptr(), out.data_ptr(), width, *scratch, stream)
     check(rc, "mfd_kv8_page_weights")
     return out
 
@@ -816,8 +820,8 @@ def kv8_evict(page_table: torch.Tensor, mass: torch.Tensor, seq_lens: torch.Tens
     freed = torch.empty_like(page_table)
     lens = torch.empty_like(seq_lens)
     counts = torch.empty_like(seq_lens)
-    rc = _lib.lib().mfd_kv8_evict(page_table.data_ptr(), mass.data_ptr(), seq_lens.data_ptr(), bs, width, page_size,
-                                  keep_pages, sink_pages, recent_pages, table.data_ptr(), kept.data_ptr(),
-                                  lens.data_ptr(), freed.data_ptr(), counts.data_ptr(), raw_stream(dev))
+    rc = _kv8_evict_c(page_table.data_ptr(), mass.data_ptr(), seq_lens.data_ptr(), bs, width, page_size, keep_pages,
+                      sink_pages, recent_pages, table.data_ptr(), kept.data_ptr(), lens.data_ptr(), freed.data_ptr(),
+                      counts.data_ptr(), raw_stream(dev))
     check(rc, "mfd_kv8_evict")
     return table, kept, lens, freed, counts
