@@ -229,6 +229,19 @@ def test_attention_many_requests(bs, n):
     Case(bs, rng.integers(0, 90, bs).tolist(), n=n, heads=4, kv=1, page=16, dtype="e4m3").check()
 
 
+@pytest.mark.parametrize("n", [1, 3, 20, 65])
+def test_attention_many_units_of_very_unequal_lengths(n):
+    # more units than half the CTAs of either kernel, so CTAs' ranges begin and end inside units, and in what a unit is
+    # counted for beside its tiles
+    Case(23 + n, [3000, 0, 1, 2, 0, 129, 16, 0, 1700, 5, 0, 0, 127, 128, 1, 640] * 3, n=n, heads=16, kv=4, page=16).check()
+
+
+@pytest.mark.parametrize("n", [1, 4])
+@pytest.mark.parametrize("tokens", [129, 4096, 40000])
+def test_attention_one_request_in_many_pieces(n, tokens):
+    Case(29 + n, [tokens], n=n, heads=4, kv=1, page=64).check()
+
+
 @pytest.mark.parametrize("n", [1, 12, 65])
 def test_attention_long_requests_are_split_and_merged(n):
     """One long request over the whole GPU, next to short ones; and the same bits every time."""
