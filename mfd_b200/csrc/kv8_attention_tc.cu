@@ -32,7 +32,7 @@
 // scores ahead of the exponentials.
 //
 // Measured (H 32 over 8 KV heads): 64 nodes, 32 requests of 1K - 8K tokens 250 us with the combination, 0.59 PFLOP/s of
-// 4 D flop a score (0.89 with the second product of the weights); 65 nodes, one request of 4096 tokens 32 us.
+// 4 D flop a score (0.89 with the second product of the weights); 65 nodes, one request of 4096 tokens 31 us, 21 of them here.
 //
 // Split: as in kv8_attention_rows.cu, in key tiles of 128: equal ranges of all units' tiles laid end to end, or at most
 // one piece a CTA when there are few units.  Pieces leave (m, l, O) and kv8_combine_kernel adds them in order, spread
@@ -176,6 +176,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the combination may be set up (it waits for this grid's end)
     // TMEM columns: O of group t at 128 t, S of group t at 256 + 128 t
     const int RB = (p.rows - p.row0 + 128 * L::kRowTiles - 1) / (128 * L::kRowTiles);
     auto tiles_of = [&](int len) { return counted_tiles(p, len, p.bs * p.c.Hkv * RB, gridDim.x); };
@@ -646,7 +647,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
 // Adds up the pieces of every unit that was cut, in their order.  Block x is the CTA boundary (range cut: the first one
 // inside its unit; split: the unit's first piece) that answers for a unit, block y 32 of its rows; a warp takes 16
-// columns of them, lane = row, so every load of a piece is 512 contiguous bytes.
+// columns of them, lane = row, so every load of a piece is 512 contiguous bytes.  It is launched while the attention runs and
+// waits for its end after finding its unit (2 us of a call less).
 template <bool PAIR>
 __global__ void __launch_bounds__(256) kv8_combine_kernel(const AttnParams p, int ctas) {
     constexpr int kRowsU = kSlotRows(PAIR);
@@ -658,14 +660,18 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(const AttnParams p, in
     int pos, end;
     cut_range(cut, cta, pos, end);
     Piece pc;
-    if (!next_piece(lens, tiles_of, cut, cta, pos, end, pc)) return;
+    const bool any = next_piece(lens, tiles_of, cut, cta, pos, end, pc);
+    // The pieces are complete and visible from here.  (Every CTA waits, so that this grid never ends before the attention's:
+    // the next launch waits for this one.)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!any) return;
     if (cut.split ? (pc.first != cta || pc.pieces == 1) : (pc.g0 == 0 || pc.first != cta - 1)) return;
     const int hk = pc.u / RB, rb = pc.u % RB;
     const int r = blockIdx.y * 32 + lane, row = p.row0 + rb * kRowsU + r;
     if (row - lane >= p.rows) return;
     float mm = -INFINITY;
 #pragma unroll 8
-    for (int i = 0; i < pc.pieces; ++i) mm = fmaxf(mm, __ldg(p.part + (int64_t)slot_of(pc, i) * kSlotFloats(PAIR) + r));
+    for (int i = 0; i < pc.pieces; ++i) mm = fmaxf(mm, __ldcg(p.part + (int64_t)slot_of(pc, i) * kSlotFloats(PAIR) + r));
     float ll = 0.f;
     float4 v[4];
 #pragma unroll
@@ -673,12 +679,12 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(const AttnParams p, in
 #pragma unroll 4
     for (int i = 0; i < pc.pieces; ++i) {
         const float* s = p.part + (int64_t)slot_of(pc, i) * kSlotFloats(PAIR);
-        const float mi = __ldg(s + r), li = __ldg(s + kRowsU + r);
+        const float mi = __ldcg(s + r), li = __ldcg(s + kRowsU + r);
         const float a = mi == -INFINITY ? 0.f : fast_exp2(mi - mm);
         ll = fmaf(a, li, ll);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            const float4 o = __ldg(reinterpret_cast<const float4*>(s + 2 * kRowsU) + (int64_t)(4 * warp + c) * kRowsU + r);
+            const float4 o = __ldcg(reinterpret_cast<const float4*>(s + 2 * kRowsU) + (int64_t)(4 * warp + c) * kRowsU + r);
             v[c].x = fmaf(a, o.x, v[c].x), v[c].y = fmaf(a, o.y, v[c].y);
             v[c].z = fmaf(a, o.z, v[c].z), v[c].w = fmaf(a, o.w, v[c].w);
         }
@@ -713,7 +719,20 @@ int launch_tc_one(const AttnParams& p, int sms, cudaStream_t stream) {
     kv8_tc_kernel<FP8, PAIR><<<sms, kTcThreads, Layout<PAIR>::kBytes, stream>>>(tk, tv, p);
     MFD_CHECK_LAUNCH("mfd_kv8_attention");
     const int rows = p.rows - p.row0 < kSlotRows(PAIR) ? p.rows - p.row0 : kSlotRows(PAIR);
-    kv8_combine_kernel<PAIR><<<dim3((unsigned)sms, (unsigned)((rows + 31) / 32)), 256, 0, stream>>>(p, sms);
+    // the combination's launch overlaps the attention (programmatic dependent launch)
+    cudaLaunchAttribute overlap;
+    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    overlap.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)sms, (unsigned)((rows + 31) / 32));
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cfg.attrs = &overlap, cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kv8_combine_kernel<PAIR>, p, sms);
+    if (e != cudaSuccess) {
+        set_error("mfd_kv8_attention: %s", cudaGetErrorString(e));
+        return MFD_ERR_CUDA;
+    }
     MFD_CHECK_LAUNCH("mfd_kv8_attention (combination)");
     return MFD_OK;
 }
