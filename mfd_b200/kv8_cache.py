@@ -35,23 +35,21 @@ class KV8Cache:
         self._pages = [0] * batch  # pages a request owns
 
     def reserve(self, tokens: int) -> None:
-        """Give every request pages for `tokens` more tokens.  Reads the lengths back."""
-        lens = self.seq_lens.tolist()
-        rows, cols, ids = [], [], []
-        for b, t in enumerate(lens):
-            need = -(-(t + tokens) // self.page_size)
-            if need > self.page_table.shape[1]:
-                raise RuntimeError(f"KV8Cache: request {b} needs {need} pages, its table holds {self.page_table.shape[1]}")
-            while self._pages[b] < need:
-                if not self._free:
-                    raise RuntimeError("KV8Cache: no free page")
-                rows.append(b)
-                cols.append(self._pages[b])
-                ids.append(self._free.pop())
-                self._pages[b] += 1
-        if ids:
-            at = torch.tensor([rows, cols, ids], device=self.page_table.device)
-            self.page_table[at[0], at[1]] = at[2].to(torch.int32)
+        """Give every request pages for `tokens` more tokens.  Reads the lengths back.  All or nothing: where it raises,
+        no request has got a page."""
+        need = [-(-(t + tokens) // self.page_size) for t in self.seq_lens.tolist()]
+        for b, n in enumerate(need):
+            if n > self.page_table.shape[1]:
+                raise RuntimeError(f"KV8Cache: request {b} needs {n} pages, its table holds {self.page_table.shape[1]}")
+        places = [(b, i) for b, n in enumerate(need) for i in range(self._pages[b], n)]
+        if len(places) > len(self._free):
+            raise RuntimeError(f"KV8Cache: no free page for {len(places) - len(self._free)} of the {len(places)} wanted")
+        if places:
+            ids = self._free[-len(places):]
+            at = torch.tensor(places, device=self.page_table.device).t()
+            self.page_table[at[0], at[1]] = torch.tensor(ids, dtype=torch.int32, device=self.page_table.device)
+            del self._free[-len(places):]
+            self._pages = [max(p, n) for p, n in zip(self._pages, need)]
 
     def append(self, k_new: torch.Tensor, v_new: torch.Tensor, path: torch.Tensor | None = None,
                counts: torch.Tensor | None = None) -> None:
