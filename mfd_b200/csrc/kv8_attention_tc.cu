@@ -62,6 +62,13 @@ __device__ __forceinline__ int counted_tiles(const AttnParams& p, int len, int u
     return max(1, (len + kKt - 1) / kKt + (p.nn + kKt - 1) / kKt) + (units > ctas / 2 ? kUnitTiles : 0);
 }
 
+// What the producer says of a tile beside its page constants.
+struct TileConst {
+    float factor[8];  // score factors of its 8 groups, where not all are positive (their constants say 1 then)
+    int turned;       // whether that is so
+    int pad[3];
+};
+
 template <bool PAIR>
 struct Layout {
     static constexpr int kRowTiles = PAIR ? 2 : 1;
@@ -72,7 +79,8 @@ struct Layout {
     static constexpr int kOffV = kOffK + 2 * kTileBytes;
     static constexpr int kOffRaw = kOffV + 2 * kTileBytes;
     static constexpr int kOffConst = kOffRaw + kStages * kRawBytes;  // [kRing][8 groups][4] floats: c, d, 1 / sv
-    static constexpr int kOffBar = kOffConst + kRing * 8 * 4 * 4;
+    static constexpr int kOffTile = kOffConst + kRing * 8 * 4 * 4;  // [kRing] TileConst
+    static constexpr int kOffBar = kOffTile + kRing * (int)sizeof(TileConst);
     static constexpr int kUsed = kOffBar + 512;
     static constexpr int kBytes = kUsed + 1024;  // the base is aligned to 1024 by hand
     static_assert(kBytes <= 227 * 1024, "shared memory");
@@ -147,6 +155,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     volatile int* s_failed = reinterpret_cast<volatile int*>(smem + L::kOffBar + 8 * L::kBars + 4);
     volatile int* s_odd = s_failed + 1;  // a non-finite own value was met in this piece
     float4* consts = reinterpret_cast<float4*>(smem + L::kOffConst);
+    TileConst* tile_consts = reinterpret_cast<TileConst*>(smem + L::kOffTile);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
@@ -269,6 +278,20 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 tc_fence_after();
                 if (quarter_live && ok) {
                     const float4* cst = consts + (size_t)((x.n_tile + tile - pc.g0) % L::kRing) * 8;
+                    const TileConst& tc = tile_consts[(x.n_tile + tile - pc.g0) % L::kRing];
+                    if (tc.turned) {
+                        // rare: a factor that is not positive (a K scale of 0, a softmax scale of 0 or below) goes in before the
+                        // maximum, which it would turn over, and before the mask, which it would turn into NaN (-inf * 0)
+#pragma unroll 1
+                        for (int c = 0; c < 4; ++c) {
+                            float v[32];
+                            tmem_ld32(s_tm + 32 * c, v);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] *= tc.factor[2 * c + (j >> 4)];
+                            tmem_st32(s_tm + 32 * c, v);
+                        }
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    }
                     // visibility of the tile's keys, 32 a word
                     const int valid = pc.len - tile * kKt;
                     const bool masked = tile >= x.tp || valid < kKt;
@@ -560,14 +583,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         tma_page(sbase + L::kOffRaw + st * kRawBytes + which * (kRawBytes / 2) + lane * bytes, which ? &tmv : &tmk,
                                  bar, x.hk, id);
                     }
-                    if (which == 0 && lane < ppt) {
+                    if (which == 0) {
                         float4 k = make_float4(p.scale_log2, 0.f, 1.f, 0.f);  // own keys, or behind the request's end
                         if (id >= 0) {
                             const float sk = __ldg(p.c.k_scale + (int64_t)id * p.c.Hkv + x.hk);
                             const float sv = fmaxf(__ldg(p.c.v_scale + (int64_t)id * p.c.Hkv + x.hk), kScaleFloor);
                             k = make_float4(sk * p.scale_log2, __log2f(sv), __frcp_rn(sv), 0.f);
                         }
-                        for (int g = 0; g < gpp; ++g) cst[lane * gpp + g] = k;
+                        TileConst& tc = tile_consts[nr % L::kRing];
+                        const bool turned = __any_sync(MFD_FULL_MASK, !(k.x > 0.f));
+                        const float factor = k.x;
+                        if (turned) k.x = 1.f;
+                        if (lane < ppt)
+                            for (int g = 0; g < gpp; ++g) {
+                                cst[lane * gpp + g] = k;
+                                if (turned) tc.factor[lane * gpp + g] = factor;
+                            }
+                        if (lane == 0) tc.turned = turned;
                     }
                     // the lanes without a page arrive last (lanes 8 .. 31 never have one), after every constant is stored
                     __syncwarp();

@@ -1,0 +1,43 @@
+"""The 8-bit cache attention where scales and scores leave their usual ranges, in both kernels (up to 16 rows of a KV head,
+and more).  References and tolerances are those of test_gpu_kv8.py, whose terms hold here too: the scores are sums of 128
+float32 products, and an output is compared in units of sum p |v|, which scales with the values."""
+import pytest
+import torch
+
+from test_gpu_kv8 import Case
+
+pytestmark = pytest.mark.gpu
+ROWS = [1, 4, 5, 9, 40, 65]  # nodes, of 4 heads to a KV head: the last row counts of one kernel and the first of the other
+
+
+def _last_pages(c):
+    return [int(c.table[b, (t - 1) // c.page]) for b, t in enumerate(c.lens) if t]
+
+
+@pytest.mark.parametrize("dtype", ["int8", "e4m3"])
+@pytest.mark.parametrize("n", ROWS)
+def test_key_scales_of_zero_in_partial_pages(n, dtype):
+    """A page of zero keys may have the scale 0: its tokens score 0, and what lies behind the length stays hidden."""
+    c = Case(101 + n, [0, 5, 33, 64, 290], n=n, heads=8, kv=2, page=32, dtype=dtype)
+    c.ks[_last_pages(c), 0] = 0.0
+    c.ks[int(c.table[4, 2])] = 0.0
+    c.check()
+    c.check(own=False)
+
+
+@pytest.mark.parametrize("n", ROWS)
+@pytest.mark.parametrize("scale", [0.0, -0.0, -128 ** -0.5, -1.0])
+def test_scales_of_zero_and_below(n, scale):
+    """Softmax scales that are not positive; with -1 the scores reach 130 to either side (log2), which no float32 weight spans
+    unless the reference is their maximum."""
+    c = Case(111 + n, [0, 7, 150, 333], n=n, heads=8, kv=2, page=16, dtype="int8")
+    c.scale = scale
+    biggest = max(float((c.v.float() * c.vs[:, :, None, None]).nan_to_num().abs().max()), float(c.vn.float().abs().max()))
+    for anc in (True, False):
+        out, lse = c.run(anc=anc)
+        ref, rl, size = c.attention(anc=anc)
+        # (weights below 2^-37 of a row's largest may be lost in the kernel for few rows, as it states)
+        assert bool(((out.double() - ref).abs() <= 1.05 * 2 ** -8 * size + 2.0 ** -36 * biggest).all())
+        live = torch.isfinite(rl)
+        assert torch.equal(lse.double()[~live], rl[~live])
+        assert float(((lse.double() - rl).abs() - 2e-6 * rl.abs())[live].max()) <= 2e-5
