@@ -130,6 +130,9 @@ __device__ __forceinline__ void commit_if(uint32_t leader, uint64_t* bar) {
         : "memory");
 }
 
+// A TMEM store is asynchronous: whoever reads what it wrote (a later load of the same warp too) waits for it first.
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
 // What a piece's tiles are (of 128 keys: cached tokens first, then the nodes' own).
 struct Tiles {
     int hk, rb;       // KV head, block of rows
@@ -271,6 +274,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     for (int j = 0; j < 32; ++j) o[j] *= alpha;
                     tmem_st32(o_tm + oc, o);
                 }
+                tmem_st_wait();  // (a second rescaling in the step reads O again)
             };
             for (int s = grp; s < x.nsteps; s += 2, ++done) {
                 const int tile = pc.g0 + (x.alternate ? s : s >> 1);
@@ -290,7 +294,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             for (int j = 0; j < 32; ++j) v[j] *= tc.factor[2 * c + (j >> 4)];
                             tmem_st32(s_tm + 32 * c, v);
                         }
-                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                        tmem_st_wait();
                     }
                     // visibility of the tile's keys, 32 a word
                     const int valid = pc.len - tile * kKt;
@@ -346,6 +350,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             acc[0] = mul2(acc[0], dup2(alpha)), acc[1] = mul2(acc[1], dup2(alpha));
                             if (done >= 1) rescale_o(alpha);
                             const __nv_bfloat162 a2 = __float2bfloat162_rn(alpha);
+                            tmem_st_wait();  // the weights of the chunks before are read again
 #pragma unroll 1
                             for (int d = 0; d < c; ++d) {
                                 uint32_t w[1][32];
@@ -380,7 +385,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     float a0, a1;
                     upk2(add2(acc[0], acc[1]), a0, a1);
                     l += a0 + a1;
-                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    tmem_st_wait();
                 }
                 tc_fence_before();
                 __syncwarp();

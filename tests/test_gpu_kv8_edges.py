@@ -4,7 +4,7 @@ float32 products, and an output is compared in units of sum p |v|, which scales 
 import pytest
 import torch
 
-from test_gpu_kv8 import Case
+from test_gpu_kv8 import DEV, Case
 
 pytestmark = pytest.mark.gpu
 ROWS = [1, 4, 5, 9, 40, 65]  # nodes, of 4 heads to a KV head: the last row counts of one kernel and the first of the other
@@ -41,3 +41,23 @@ def test_scales_of_zero_and_below(n, scale):
         live = torch.isfinite(rl)
         assert torch.equal(lse.double()[~live], rl[~live])
         assert float(((lse.double() - rl).abs() - 2e-6 * rl.abs())[live].max()) <= 2e-5
+
+
+@pytest.mark.parametrize("dtype", ["int8", "e4m3"])
+@pytest.mark.parametrize("n", ROWS)
+@pytest.mark.parametrize("leap", [9.0, 50.0])
+def test_references_that_move_at_every_chunk_and_tile(leap, n, dtype):
+    """Scores that rise by `leap` every 32 keys over three tiles: past 2^60 a chunk, the weights already written and O are
+    scaled again within the step, several times; past 2^8 a tile, O alone at its start.  (A value read back before its store had
+    finished would be a raw score, or a stale O.)"""
+    c = Case(141 + n, [384, 384, 300, 130], n=n, heads=8, kv=2, page=16, dtype=dtype, stale=False)
+    c.k = torch.zeros(c.k.shape, device=DEV).to(c.k.dtype)
+    c.k[..., 0] = torch.full(c.k.shape[:3], 64.0, device=DEV).to(c.k.dtype)
+    c.q.zero_()
+    c.q[..., 0] = 1.0
+    c.scale = 1.0
+    for b, t in enumerate(c.lens):
+        for i in range(-(-t // 16)):
+            c.ks[int(c.table[b, i])] = (i // 2) * leap / 64.0
+    c.check(own=False)
+    c.check()
