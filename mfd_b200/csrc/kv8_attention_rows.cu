@@ -2,8 +2,10 @@
 //
 // The mathematics, for a row with query q over keys j (page P(j), codes a_j and c_j, scales sk and sv):
 //   score  s_j = sk (q . a_j) scale log2(e),      w_j = s_j + log2(sv),      m = max_j w_j - 12
-//   O = sum_j 2^(w_j - m) c_j,   l = sum_j 2^(w_j - m) / sv,                 out = O / l,  lse = ln2 (m + log2 l)
-// so the value scale rides in the exponent and no code is multiplied by its scale.  The products have float16 operands
+//   O = sum_j 2^(w_j - m) c_j,   l = sum_j 2^(w_j - m - u) / sv,             out = O 2^-u / l,  lse = ln2 (m + u + log2 l)
+// so the value scale rides in the exponent and no code is multiplied by its scale.  1 / sv goes from 2^-121 (the largest
+// bf16 values) to 2^100 (a page of zeros), the weights to 2^15: with u = 18 no sum of 2^30 of them leaves float32, and one
+// key of the largest values is still 22 bits.  The products have float16 operands
 // and float32 sums: codes are exact there, and so is the query row divided by a power of two.  The weights go in as
 // float16 hi + lo, two tensor instructions, lifted to at most 2^15: 22 bits of a weight, down to 2^-37 of the row's
 // largest.  (One float16 or bf16 weight would err by a good part of the output's own rounding.)  The nodes' own bf16
@@ -56,6 +58,7 @@ constexpr int kMaxPieces = 512;   // of a unit: at most one a CTA
 constexpr int kUnitTiles = 4, kOwnTiles = 6;
 constexpr float kLift = 12.f;  // the largest weights are 2^12, and up to 2^15 before the reference moves
 constexpr float kLazy = 3.f;
+constexpr float kUnit = 3.814697265625e-06f, kUnitLog2 = 18.f;  // 2^-u and u
 constexpr int kMaxOwn = kRowsMaxOwn;  // own keys a request
 
 // NT: 8-row tiles a unit
@@ -209,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
                     const float mr = m[n][e] == -INFINITY ? 0.f : m[n][e];
                     w[n][e] = fast_exp2(w[n][e] - mr);
                     w[n][2 + e] = fast_exp2(w[n][2 + e] - mr);
-                    l[n][e] = fmaf(w[n][e] + w[n][2 + e], inv_sv, l[n][e]);
+                    l[n][e] = fmaf((w[n][e] + w[n][2 + e]) * kUnit, inv_sv, l[n][e]);
                 }
         };
 
@@ -387,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             }
             for (int j = lane; j < seen; j += 32) {
                 const float a = s_own[r][j] == -INFINITY ? 0.f : fast_exp2(s_own[r][j] - mm);
-                ll += a;
+                ll = fmaf(a, kUnit, ll);
                 s_own[r][j] = a;
             }
 #pragma unroll 1
@@ -408,12 +411,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         const bool whole = pc.pieces == 1;
         float* slot = p.part + (int64_t)pc.slot * kSlot;
         auto store = [&](int r, int col, float4 v, float mm, float ll) {  // columns col .. col + 3 of row r, and lse
-            const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
+            const float inv = ll > 0.f ? kUnit / ll : (ll == 0.f ? 0.f : ll);
             const int row = base + r, nd = row / p.G, hd = hk * p.G + row % p.G;
             *reinterpret_cast<uint2*>(p.out + (int64_t)pc.b * p.so_b + (int64_t)nd * p.so_n + (int64_t)hd * p.so_h + col) =
                 make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
             if (p.lse && col == 0)
-                p.lse[((int64_t)pc.b * p.n + nd) * p.H + hd] = ll == 0.f ? -INFINITY : 0.6931471805599453f * (mm + log2f(ll));
+                p.lse[((int64_t)pc.b * p.n + nd) * p.H + hd] = ll == 0.f ? -INFINITY : 0.6931471805599453f * (mm + (kUnitLog2 + log2f(ll)));
         };
 #pragma unroll 1
         for (int e = tid; e < live_rows * 32; e += kThreads) {

@@ -4,7 +4,7 @@
 // The mathematics is that of kv8_attention_rows.cu, with every operand in bf16 (the codes, the queries and the nodes'
 // own keys and values are exact there; the weights go in as hi + lo, 16 bits of each):
 //   S = Q K8^T,  w = sk scale log2(e) S + log2(sv),  P = 2^(w - m) = P_hi + P_lo,  O = P_hi V8 + P_lo V8,
-//   l = sum P / sv,  out = O / l.
+//   l = sum P 2^-u / sv,  out = O 2^-u / l.
 //
 // Rows r = node * G + g of a (request, KV head) in tiles of 128 (one row per TMEM lane).  Two softmax groups of four
 // warps, each with its own S buffer and O accumulator in TMEM, so one group's softmax runs while the other's products
@@ -54,6 +54,11 @@ constexpr int kKt = 128;                 // keys per tile
 constexpr int kTileBytes = kKt * kD * 2;  // 32 KB: a bf16 tile, [2 d-halves][128 rows][128 B]
 constexpr int kRawBytes = 2 * kKt * kD;   // 32 KB: the codes of K and V
 constexpr uint32_t kTries = 1u << 20;
+// How far (log2) a score may pass its row's reference within a tile, and the unit of l, 2^u.  1 / sv goes up to 2^100 (a page
+// of zeros): the 128 weights of a tile sum to at most 2^(7 + 30 + 100 - 12), those of 2^30 keys in all, within 2^8 of their
+// references, to 2^(30 + 8 + 100 - 12), and a key of the largest bf16 values still counts with 16 bits.
+constexpr float kFar = 30.f;
+constexpr float kUnit = 0.000244140625f, kUnitLog2 = 12.f;  // 2^-u and u
 // Tiles of a unit as the cut counts them.  Many units share CTAs, and there a unit counts kUnitTiles more than it has, for
 // its queries and its epilogue: otherwise the CTAs that get several short requests end last (32 trees of 65 nodes over 1K
 // - 8K tokens 273 us, this way 237).
@@ -78,7 +83,7 @@ struct Layout {
     static constexpr int kOffK = kOffQ + kRowTiles * kTileBytes;
     static constexpr int kOffV = kOffK + 2 * kTileBytes;
     static constexpr int kOffRaw = kOffV + 2 * kTileBytes;
-    static constexpr int kOffConst = kOffRaw + kStages * kRawBytes;  // [kRing][8 groups][4] floats: c, d, 1 / sv
+    static constexpr int kOffConst = kOffRaw + kStages * kRawBytes;  // [kRing][8 groups][4] floats: c, d, 2^-u / sv
     static constexpr int kOffTile = kOffConst + kRing * 8 * 4 * 4;  // [kRing] TileConst
     static constexpr int kOffBar = kOffTile + kRing * (int)sizeof(TileConst);
     static constexpr int kUsed = kOffBar + 512;
@@ -262,7 +267,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const uint32_t s_tm = tmem + lane_off + 256 + 128 * grp, o_tm = tmem + lane_off + 128 * grp;
             // O and l are relative to 2^m; m_next is what m should be (the tiles' maxima).  A tile's weights are formed
             // in one pass against the m of the tiles before it, which bf16's range allows: m only follows when the
-            // maximum has passed it by 2^8, before the next tile, and at once where a chunk passes it by 2^60.
+            // maximum has passed it by 2^8, before the next tile, and at once where a chunk passes it by 2^kFar.
             float m = -INFINITY, m_next = -INFINITY, l = 0.f;
             int done = 0;  // steps of this group
             auto rescale_o = [&](float alpha) {  // (S of this step is there, so the group's last product is complete)
@@ -339,7 +344,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         const float mx = fmaxf(top[0] == -INFINITY ? top[0] : fmaf(top[0], k0.x, k0.y),
                                                top[1] == -INFINITY ? top[1] : fmaf(top[1], k1.x, k1.y));
                         m_next = fmaxf(m_next, mx);
-                        const bool far = mx > m + 60.f;
+                        const bool far = mx > m + kFar;
                         if (__any_sync(MFD_FULL_MASK, far)) {
                             // a row's first keys, or scores that leap: the reference moves now, by a power of two, so that the
                             // weights already written scale exactly
@@ -399,7 +404,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             // x.alternate: the two groups' (m, l) of a row meet in the raw ring (every code is converted by now), and each
             // group finishes 64 columns
-            // (l and O come down to the tiles' maximum first: m may be 2^60 below it)
+            // (l and O come down to the tiles' maximum first: m may be 2^kFar below it)
             const float f_late = m_next > m && m != -INFINITY ? fast_exp2(m - m_next) : 1.f;
             if (m != -INFINITY) m = fmaxf(m, m_next);
             l *= f_late;
@@ -425,7 +430,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const bool odd = *s_odd != 0;
             const int own0 = max(pc.g0 - x.tp, 0) * kKt, own1 = min(p.nn, (x.t1 - x.tp) * kKt);  // own keys of this piece
             if (quarter_live && ok) {
-                const float inv = l_fin > 0.f ? 1.f / l_fin : (l_fin == 0.f ? 0.f : l_fin);
+                const float inv = l_fin > 0.f ? kUnit / l_fin : (l_fin == 0.f ? 0.f : l_fin);
                 const int c_lo = x.alternate ? 64 * grp : 0, c_hi = x.alternate ? c_lo + 64 : kD;
                 float* slot = p.part + (int64_t)pc.slot * kSlotFloats(PAIR);
                 const int srow = (x.alternate ? 0 : 128 * grp) + rt;
@@ -435,7 +440,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         slot[kSlotRows(PAIR) + srow] = l_fin;
                     } else if (live && p.lse) {
                         p.lse[((int64_t)pc.b * p.n + node) * p.H + x.hk * p.G + row % p.G] =
-                            l_fin == 0.f ? -INFINITY : 0.6931471805599453f * (m_fin + log2f(l_fin));
+                            l_fin == 0.f ? -INFINITY : 0.6931471805599453f * (m_fin + (kUnitLog2 + log2f(l_fin)));
                     }
                 }
 #pragma unroll 1
@@ -589,11 +594,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                  bar, x.hk, id);
                     }
                     if (which == 0) {
-                        float4 k = make_float4(p.scale_log2, 0.f, 1.f, 0.f);  // own keys, or behind the request's end
+                        float4 k = make_float4(p.scale_log2, 0.f, kUnit, 0.f);  // own keys, or behind the request's end
                         if (id >= 0) {
                             const float sk = __ldg(p.c.k_scale + (int64_t)id * p.c.Hkv + x.hk);
                             const float sv = fmaxf(__ldg(p.c.v_scale + (int64_t)id * p.c.Hkv + x.hk), kScaleFloor);
-                            k = make_float4(sk * p.scale_log2, __log2f(sv), __frcp_rn(sv), 0.f);
+                            k = make_float4(sk * p.scale_log2, __log2f(sv), __frcp_rn(sv) * kUnit, 0.f);
                         }
                         TileConst& tc = tile_consts[nr % L::kRing];
                         const bool turned = __any_sync(MFD_FULL_MASK, !(k.x > 0.f));
@@ -727,7 +732,7 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(const AttnParams p, in
         }
     }
     if (row >= p.rows) return;
-    const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);
+    const float inv = ll > 0.f ? kUnit / ll : (ll == 0.f ? 0.f : ll);
     const int node = row / p.G, head = hk * p.G + row % p.G;
     uint4* dst = reinterpret_cast<uint4*>(p.out + (int64_t)pc.b * p.so_b + (int64_t)node * p.so_n + (int64_t)head * p.so_h +
                                           16 * warp);
@@ -737,7 +742,7 @@ __global__ void __launch_bounds__(256) kv8_combine_kernel(const AttnParams p, in
                             pack_bf16(v[2 * c + 1].x * inv, v[2 * c + 1].y * inv),
                             pack_bf16(v[2 * c + 1].z * inv, v[2 * c + 1].w * inv));
     if (p.lse && warp == 0)
-        p.lse[((int64_t)pc.b * p.n + node) * p.H + head] = ll == 0.f ? -INFINITY : 0.6931471805599453f * (mm + log2f(ll));
+        p.lse[((int64_t)pc.b * p.n + node) * p.H + head] = ll == 0.f ? -INFINITY : 0.6931471805599453f * (mm + (kUnitLog2 + log2f(ll)));
 }
 
 template <bool FP8, bool PAIR>
