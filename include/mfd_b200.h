@@ -31,6 +31,10 @@ enum mfd_dtype { MFD_F32 = 0, MFD_BF16 = 1, MFD_I32 = 2, MFD_I64 = 3, MFD_I8 = 4
 
 /* Thread-local message of the last failed call ("" if none). */
 const char* mfd_last_error(void);
+
+/* The capture that `stream` records into: *id receives a number of its own for every capture of the process, 0 when the
+ * stream records into none.  (Scratch of recorded calls belongs to one capture.) */
+int mfd_capture_id(void* stream, uint64_t* id);
 /* ABI version of this library. */
 int mfd_abi_version(void);
 
@@ -343,10 +347,13 @@ int mfd_kv8_append(void* k_cache, void* v_cache, int64_t sc_p, int64_t sc_h, int
  * lse [bs, n, H] float32 (optional): the natural log of the sum of exp(score * scale).  A row that sees nothing gives
  * zeros and lse -inf.  A non-finite key or value a row does not see has no effect on it.  n = 1 is a decode step.
  * Limits: head_dim 128, H a multiple of Hkv, n <= 4096.
- * Workspace: mfd_kv8_attention_workspace() bytes, zeroed before its first use, any sizes in turn; its first int32 is a
- * sticky device status, 1 once a bounded wait in the kernel gave up.  Tickets: mfd_kv8_attention_tickets(bs, n, H,
- * Hkv) zeroed words of a ticket-only buffer, left zero again.
+ * Workspace: mfd_kv8_attention_workspace() bytes, any sizes in turn; its first int32 (256-byte aligned) becomes 1 once a
+ * bounded wait in a kernel gave up, and is written at no other time (zero it before its first use to read it).  Tickets:
+ * mfd_kv8_attention_tickets(bs, n, H, Hkv) zeroed words of a ticket-only buffer, left zero again.
+ * mfd_kv8_attention_status: the same status for all calls on the current device, whatever their workspaces (waits for
+ * `stream`).
  */
+int mfd_kv8_attention_status(int* status, void* stream);
 size_t mfd_kv8_attention_workspace(int64_t bs, int64_t n, int64_t num_heads, int64_t num_kv_heads);
 int64_t mfd_kv8_attention_tickets(int64_t bs, int64_t n, int64_t num_heads, int64_t num_kv_heads);
 int mfd_kv8_attention(const void* q, int64_t sq_b, int64_t sq_n, int64_t sq_h, const void* k_cache,

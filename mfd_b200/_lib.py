@@ -71,6 +71,8 @@ _SIGS = {
     "mfd_kv8_append": (c_int, [c_vp, c_vp, c_i64, c_i64, c_i64, c_int, c_vp, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64,
                                c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64,
                                c_i64, c_vp, c_vp, c_vp]),
+    "mfd_capture_id": (c_int, [c_vp, c_vp]),
+    "mfd_kv8_attention_status": (c_int, [c_vp, c_vp]),
     "mfd_kv8_attention_workspace": (c_size, [c_i64, c_i64, c_i64, c_i64]),
     "mfd_kv8_attention_tickets": (c_i64, [c_i64, c_i64, c_i64, c_i64]),
     "mfd_kv8_attention": (c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i64, c_int, c_vp, c_vp, c_i64,
@@ -165,6 +167,18 @@ def raw_stream(idx: int) -> int:
     return _raw_stream(idx) if _raw_stream is not None else torch.cuda.current_stream(idx).cuda_stream
 
 
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+
+
+def capture_id(stream: int) -> int:
+    """The number of the CUDA graph capture that the current stream (`stream`) records into; 0 when it records none."""
+    if not _capturing():
+        return 0
+    number = ctypes.c_uint64()
+    check(lib().mfd_capture_id(stream, ctypes.byref(number)), "mfd_capture_id")
+    return number.value
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
@@ -215,3 +229,51 @@ class Workspace:
             buf = torch.zeros(size, dtype=torch.uint8, device=device)
             cls._cache[key] = buf
         return buf
+
+
+class CaptureScratch:
+    """Scratch of calls that are recorded into a CUDA graph: its own for each capture, purpose and stream.
+
+    The workspace is allocated while the graph is captured, so it belongs to the graph's memory pool and lives as long as
+    the graph.  The tickets, which have to be zero, are words of a buffer that an earlier plain call zeroed and that is never
+    given back (each capture keeps its words); where there is none, or it is used up, a node of the graph zeroes some in
+    front of the first call (2 us of a replay).  So a replay depends on no other call, and graphs share no scratch.  (Workspaces
+    captured into one pool may overlap: PyTorch wants such graphs replayed in order.)"""
+
+    SPARE = 1 << 22  # bytes of zeroed tickets a device
+    _held: dict = {}  # (device index, purpose, stream) -> (capture id, workspace, its bytes, tickets, their bytes)
+    _spare: dict = {}  # device index -> (zeroed buffer, bytes taken)
+
+    @classmethod
+    def prepare(cls, device: torch.device) -> None:
+        """Zero the spare tickets of a device, once; not while capturing.  They are zero when this returns."""
+        if device.index not in cls._spare:
+            cls._spare[device.index] = torch.zeros(cls.SPARE, dtype=torch.uint8, device=device), 0
+            if device.type == "cuda":
+                torch.cuda.current_stream(device).synchronize()
+
+    @classmethod
+    def _zeroed(cls, device: torch.device, nbytes: int) -> torch.Tensor:
+        spare, taken = cls._spare.get(device.index, (None, 0))
+        if spare is None or taken + nbytes > spare.numel():
+            return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        cls._spare[device.index] = spare, taken + nbytes
+        return spare[taken:taken + nbytes]
+
+    @classmethod
+    def get(cls, device: torch.device, purpose: str, stream: int, capture: int, nbytes: int, words: int):
+        """(workspace, its bytes, tickets, their words), as addresses."""
+        key = (device.index, purpose, stream)
+        held = cls._held.get(key)
+        if held is not None and held[0] != capture:  # (an ended capture's memory stays with its graph)
+            del cls._held[key]
+            held = None
+        if held is None or held[2] < nbytes or held[4] < 4 * words:
+            _, ws, had, tk, had_tk = held if held is not None else (0, None, 0, None, 0)
+            if had_tk < 4 * words:
+                had_tk = -(-4 * words // 256) * 256
+                tk = cls._zeroed(device, had_tk)
+            if had < nbytes:
+                ws, had = torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
+            held = cls._held[key] = capture, ws, had, tk, had_tk
+        return held[1].data_ptr(), held[2], held[3].data_ptr(), held[4] // 4

@@ -47,6 +47,8 @@ namespace kv8 {
 
 namespace {
 
+__device__ int gave_up;  // sticky, of all calls on the device
+
 constexpr int kTcThreads = 512;
 constexpr int kConv = 6;                 // converter warps
 constexpr int kSoftmaxRegs = 152, kOtherRegs = 104;
@@ -678,7 +680,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             });
         }
     }
-    if (*s_failed && tid == 0) atomicExch(p.status, 1);
+    if (*s_failed && tid == 0) atomicExch(p.status, 1), atomicExch(&gave_up, 1);
     tc_fence_before();
     __syncthreads();
     if (warp == 15) {
@@ -790,3 +792,15 @@ int launch_tc(const AttnParams& p, bool pair, int sms, cudaStream_t stream) {
 
 }  // namespace kv8
 }  // namespace mfd
+
+extern "C" int mfd_kv8_attention_status(int* status, void* stream) {
+    cudaError_t e = status ? cudaSuccess : cudaErrorInvalidValue;
+    if (e == cudaSuccess)
+        e = cudaMemcpyFromSymbolAsync(status, mfd::kv8::gave_up, sizeof(int), 0, cudaMemcpyDeviceToHost, (cudaStream_t)stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize((cudaStream_t)stream);
+    if (e != cudaSuccess) {
+        mfd::set_error("mfd_kv8_attention_status: %s", cudaGetErrorString(e));
+        return MFD_ERR_CUDA;
+    }
+    return MFD_OK;
+}

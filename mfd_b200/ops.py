@@ -6,11 +6,13 @@ tree_logits.py, ddtree_utils.py (SGLang), mode_attention.py, tree_gdn_kernel.py 
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
-from ._lib import (MFD_BF16, MFD_E4M3, MFD_F32, MFD_I8, MFD_I32, MFD_I64, Workspace, address, check, device_index, packed,
-                   ptr, raw_stream, require_cuda, stream_ptr)
+from ._lib import (MFD_BF16, MFD_E4M3, MFD_F32, MFD_I8, MFD_I32, MFD_I64, CaptureScratch, Workspace, address, capture_id,
+                   check, device_index, packed, ptr, raw_stream, require_cuda, stream_ptr)
 
 
 def _ids_code(dtype: torch.dtype) -> int:
@@ -683,9 +685,10 @@ _KV8_SIZES: dict = {}
 
 
 def _kv8_scratch(dev: torch.device, stream: int, purpose: str, sizes: tuple, size_of):
-    """(workspace, its bytes, ticket words, their number) of one stream, as addresses: calls on different streams may
-    overlap on the GPU, so the operators of the 8-bit cache share no scratch between streams.  size_of() -> (bytes,
-    tickets) is asked once for each tuple of sizes."""
+    """(workspace, its bytes, ticket words, their number), as addresses: those of the stream, or of the graph that it
+    records into.  Calls on different streams may overlap on the GPU, and so may a graph's replays and other calls, so the
+    operators of the 8-bit cache share no scratch between them.  size_of() -> (bytes, tickets) is asked once for each
+    tuple of sizes."""
     key = (purpose, dev.index, *sizes)
     need = _KV8_SIZES.get(key)
     if need is None:
@@ -694,6 +697,11 @@ def _kv8_scratch(dev: torch.device, stream: int, purpose: str, sizes: tuple, siz
         if len(_KV8_SIZES) >= 4096:
             _KV8_SIZES.clear()
         _KV8_SIZES[key] = need
+        if not capture_id(stream):
+            CaptureScratch.prepare(dev)
+    capture = capture_id(stream)
+    if capture:
+        return CaptureScratch.get(dev, purpose, stream, capture, *need)
     ws = Workspace.get(dev, (purpose, stream), need[0])
     tk = Workspace.get(dev, (purpose, "tickets", stream), 4 * need[1])
     return ws.data_ptr(), ws.numel(), tk.data_ptr(), tk.numel() // 4
@@ -750,15 +758,13 @@ def kv8_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
 
 
 def kv8_attention_status(device=None) -> int:
-    """The sticky status word of kv8_attention's workspace for the current stream: 0, or 1 once a bounded wait in a
-    kernel gave up.  0 when no such call has run on the stream."""
+    """The sticky status of kv8_attention on a device: 0, or 1 once a bounded wait in a kernel gave up, in a call on
+    whatever stream or in a graph's replay.  Waits for the current stream, so the calls before it there are in."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    idx = dev.index if dev.index is not None else torch.cuda.current_device()
-    ws = Workspace._cache.get((idx, ("kv8_attn", stream_ptr(dev))))
-    if ws is None:
-        return 0
-    off = (-ws.data_ptr()) % 256
-    return int(ws[off:off + 4].view(torch.int32).item())
+    with torch.cuda.device(dev):
+        status = ctypes.c_int()
+        check(_lib.lib().mfd_kv8_attention_status(ctypes.byref(status), stream_ptr(dev)), "mfd_kv8_attention_status")
+    return status.value
 
 
 def kv8_page_weights(q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor, k_scale: torch.Tensor,
