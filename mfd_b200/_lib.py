@@ -202,9 +202,12 @@ def packed(name: str, op: int):
 class Workspace:
     """Per-device, per-purpose scratch, grown on demand, plus one per-device ticket buffer.  Tickets live only in
     the ticket buffer, which starts zeroed and which every ticketed kernel leaves zeroed; scratch needs no
-    initialisation.  Calls that share them must be ordered on one stream (as the current-stream launches are)."""
+    initialisation.  Calls that share them must be ordered on one stream (as the current-stream launches are).  A buffer
+    that was outgrown stays allocated, since a CUDA graph may hold its address (each is at least twice the one before, so
+    all of them take less than the last)."""
 
     _cache: dict = {}
+    _outgrown: list = []
 
     @classmethod
     def tickets(cls, device: torch.device, n: int) -> torch.Tensor:
@@ -214,6 +217,7 @@ class Workspace:
             size = max(int(n), 1024)
             if buf is not None:
                 size = max(size, 2 * buf.numel())
+                cls._outgrown.append(buf)
             buf = torch.zeros(size, dtype=torch.int32, device=device)
             cls._cache[key] = buf
         return buf
@@ -226,6 +230,7 @@ class Workspace:
             size = max(int(nbytes), 256)
             if buf is not None:
                 size = max(size, 2 * buf.numel())
+                cls._outgrown.append(buf)
             buf = torch.zeros(size, dtype=torch.uint8, device=device)
             cls._cache[key] = buf
         return buf
