@@ -170,6 +170,10 @@ def raw_stream(idx: int) -> int:
 _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 
 
+def _recording() -> bool:
+    return torch.cuda.is_initialized() and _capturing()
+
+
 def capture_id(stream: int) -> int:
     """The number of the CUDA graph capture that the current stream (`stream`) records into; 0 when it records none."""
     if not _capturing():
@@ -204,35 +208,33 @@ class Workspace:
     the ticket buffer, which starts zeroed and which every ticketed kernel leaves zeroed; scratch needs no
     initialisation.  Calls that share them must be ordered on one stream (as the current-stream launches are).  A buffer
     that was outgrown stays allocated, since a CUDA graph may hold its address (each is at least twice the one before, so
-    all of them take less than the last)."""
+    all of them take less than the last).  One that is made while a graph is captured is zeroed by that graph's replays
+    alone, and is left to it."""
 
     _cache: dict = {}
     _outgrown: list = []
 
     @classmethod
     def tickets(cls, device: torch.device, n: int) -> torch.Tensor:
-        key = (device.index if device.index is not None else torch.cuda.current_device(), "__tickets__")
-        buf = cls._cache.get(key)
-        if buf is None or buf.numel() < n:
-            size = max(int(n), 1024)
-            if buf is not None:
-                size = max(size, 2 * buf.numel())
-                cls._outgrown.append(buf)
-            buf = torch.zeros(size, dtype=torch.int32, device=device)
-            cls._cache[key] = buf
-        return buf
+        return cls._buffer(device, "__tickets__", int(n), 1024, torch.int32)
 
     @classmethod
     def get(cls, device: torch.device, purpose: str, nbytes: int) -> torch.Tensor:
+        return cls._buffer(device, purpose, int(nbytes), 256, torch.uint8)
+
+    @classmethod
+    def _buffer(cls, device: torch.device, purpose, n: int, least: int, dtype: torch.dtype) -> torch.Tensor:
         key = (device.index if device.index is not None else torch.cuda.current_device(), purpose)
         buf = cls._cache.get(key)
-        if buf is None or buf.numel() < nbytes:
-            size = max(int(nbytes), 256)
-            if buf is not None:
-                size = max(size, 2 * buf.numel())
-                cls._outgrown.append(buf)
-            buf = torch.zeros(size, dtype=torch.uint8, device=device)
-            cls._cache[key] = buf
+        if buf is not None and buf.numel() >= n:
+            return buf
+        if _recording():
+            return torch.zeros(max(n, least), dtype=dtype, device=device)
+        size = max(n, least)
+        if buf is not None:
+            size = max(size, 2 * buf.numel())
+            cls._outgrown.append(buf)
+        buf = cls._cache[key] = torch.zeros(size, dtype=dtype, device=device)
         return buf
 
 
