@@ -305,6 +305,10 @@ extern "C" int mfd_kv8_append(void* k_cache, void* v_cache, int64_t sc_p, int64_
         set_error("%s: new rows need strides that are multiples of 8 elements and 16-byte aligned bases", who);
         return MFD_ERR_INVALID;
     }
+    if ((uintptr_t)status % sizeof(int)) {
+        set_error("%s: status is not aligned to an int", who);
+        return MFD_ERR_INVALID;
+    }
     if (n > 0x3fffffff || rows > 0x3fffffff) {
         set_error("%s: too many rows", who);
         return MFD_ERR_UNSUPPORTED;

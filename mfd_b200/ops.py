@@ -660,7 +660,8 @@ def kv8_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tens
     k_cache, v_cache [pages, Hkv, page_size, 128] int8 or float8_e4m3fn; k_scale, v_scale [pages, Hkv] f32: a value is
     code * scale.  page_table int32 [bs, max_pages], seq_lens int32 [bs] (before the call).  Request b appends the
     nodes path[b, :counts[b]] (path int64 [bs, rows], as accept's "accepted", ended by -1; None: rows 0 .. counts - 1;
-    counts as accept's "commit_lens"; None: all).  Returns the new lengths (a tensor of their own)."""
+    counts as accept's "commit_lens"; None: all).  status int32 [1]: set to 4 where a row found no place (mfd_kv8_append).
+    Returns the new lengths (a tensor of their own)."""
     dev = device_index(k_cache, v_cache, k_scale, v_scale, k_new, v_new, page_table, seq_lens, path, counts, new_lens,
                        status)
     (pages, hkv, page, d), sc, code, (bs, width) = _kv8_check("kv8_append", k_cache, v_cache, k_scale, v_scale,
@@ -672,6 +673,8 @@ def kv8_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tens
         new_lens = torch.empty_like(seq_lens)
     elif new_lens.dtype != torch.int32 or new_lens.shape != seq_lens.shape or not new_lens.is_contiguous():
         raise RuntimeError("kv8_append: new_lens must be contiguous int32 [bs]")
+    if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
+        raise RuntimeError("kv8_append: status must be int32 with at least one element")
     rc = _kv8_append_c(k_cache.data_ptr(), v_cache.data_ptr(), sc[0], sc[1], sc[2], code, k_scale.data_ptr(),
                        v_scale.data_ptr(), pages, page, page_table.data_ptr(), page_table.stride(0), width,
                        seq_lens.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), sn[0], sn[1], sn[2], n, address(path),
