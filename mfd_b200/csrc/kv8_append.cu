@@ -57,8 +57,10 @@ __device__ __forceinline__ uint32_t encode2(float a, float b) {  // two values a
 }
 // The codes of 8 finite bf16 values x / s, given r, the float32 nearest to 1 / s: the product x r and one correction by its
 // exact remainder (Markstein's theorem on the correctly rounded quotient), two values an instruction.  The result is the
-// IEEE quotient for every bf16 x and every scale that comes from a bf16 maximum (tests/test_kv8_quotient.py goes through
-// all of them), at a fifth of the instructions of a division.
+// IEEE quotient for every bf16 x and every scale whose reciprocal is normal and whose remainders are exact, at a fifth of
+// the instructions of a division.  (2^23 significands of the scale times 128 of x: none differs.  Below 2^-90 a remainder may be
+// subnormal: 1.9999999 * 2^-100 and x = 2^-109 give another e4m3 code.)  Blocks of other scales divide.
+constexpr float kFastScaleLo = 5.421010862427522e-20f, kFastScaleHi = 8.507059173023462e+37f;  // 2^-64 and 2^126
 template <bool FP8>
 __device__ __forceinline__ uint2 encode8(const uint4& x, float s, float r) {
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
@@ -181,13 +183,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(PAGE)) kv8_append_kernel
         for (int w = 0; w < kThreads / 32; ++w) mx = fmaxf(mx, warp_max[w]);
     }
     const float s = fmaxf(fmaxf(__fmul_rn(mx, 1.f / qmax), open), kScaleFloor), r = __frcp_rn(s);
+    const bool fast = finite && s >= kFastScaleLo && s <= kFastScaleHi;
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
         const int slot = r0 + kRowsPerPass * i;
         uint2* dst = reinterpret_cast<uint2*>(page + (int64_t)slot * p.sc_t);
-        if (slot >= lo && slot < hi && finite) {
+        if (slot >= lo && slot < hi && fast) {
             *dst = encode8<FP8>(x[i], s, r);
-        } else if (slot < hi && (slot >= lo || s != open)) {  // rare: rows already there whose scale grows, non-finite blocks
+        } else if (slot < hi && (slot >= lo || s != open)) {  // rare: rows already there whose scale grows, non-finite blocks, extreme scales
             float f[8];
             if (slot >= lo) {
                 const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
