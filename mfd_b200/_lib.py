@@ -150,15 +150,21 @@ def stream_ptr(device: torch.device | None = None) -> int:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
 def device_index(first: torch.Tensor, *rest: torch.Tensor | None) -> int:
     """require_cuda for calls whose host time matters: the CUDA device index all the tensors share, without the
-    runtime queries (a CUDA tensor implies a device)."""
+    runtime queries (a CUDA tensor implies a device).  It has to be the current device, on which the kernel runs."""
     idx = first.get_device()
     if idx < 0:
         require_cuda(first)
     for t in rest:
         if t is not None and t.get_device() != idx:
             require_cuda(first, t)
+    current = _current_device()
+    if idx != current:
+        raise RuntimeError(f"mfd_b200: tensors on cuda:{idx} while cuda:{current} is the current device")
     return idx
 
 
