@@ -237,7 +237,7 @@ bool check_cache(const char* who, const void* k, const void* v, int64_t sc_p, in
                  int code_dtype, int64_t num_pages, int64_t page_size, const int32_t* table, int64_t max_pages,
                  const int32_t* lens, int64_t bs, int64_t hkv, int64_t head_dim, int* status) {
     *status = MFD_ERR_INVALID;
-    if (!k || !v || !table || !lens) {
+    if (!k || !v || (bs > 0 && (!table || !lens))) {  // (the tensors of an empty batch have no memory)
         set_error("%s: null pointer", who);
         return false;
     }
@@ -298,7 +298,7 @@ extern "C" int mfd_kv8_append(void* k_cache, void* v_cache, int64_t sc_p, int64_
     if (!kv8::check_cache(who, k_cache, v_cache, sc_p, sc_h, sc_t, code_dtype, num_pages, page_size, page_table,
                           max_pages, seq_lens, bs, num_kv_heads, head_dim, &st))
         return st;
-    if (!k_scale || !v_scale || !k_new || !v_new || !new_lens || new_lens == seq_lens || n <= 0 || rows < 0 ||
+    if (!k_scale || !v_scale || (bs > 0 && (!k_new || !v_new || !new_lens || new_lens == seq_lens)) || n <= 0 || rows < 0 ||
         (!path && rows > n)) {
         set_error("%s: null pointer, new_lens over seq_lens, or invalid sizes (n %lld, rows %lld)", who, (long long)n,
                   (long long)rows);

@@ -72,7 +72,7 @@ extern "C" int mfd_kv8_attention(const void* q, int64_t sq_b, int64_t sq_n, int6
     if (!kv8::check_cache(who, k_cache, v_cache, sc_p, sc_h, sc_t, code_dtype, num_pages, page_size, page_table,
                           max_pages, seq_lens, bs, num_kv_heads, head_dim, &st))
         return st;
-    if (!q || !out || !k_scale || !v_scale || !workspace || !tickets || (k_new == nullptr) != (v_new == nullptr)) {
+    if ((bs > 0 && (!q || !out)) || !k_scale || !v_scale || !workspace || !tickets || (k_new == nullptr) != (v_new == nullptr)) {
         set_error("%s: null pointer", who);
         return MFD_ERR_INVALID;
     }

@@ -161,8 +161,8 @@ extern "C" int mfd_kv8_evict(const int32_t* page_table, const float* mass, const
                              int64_t recent_pages, int32_t* table_out, float* mass_out, int32_t* new_lens,
                              int32_t* freed, int32_t* freed_counts, void* stream) {
     const char* who = "mfd_kv8_evict";
-    if (!page_table || !mass || !seq_lens || !table_out || !mass_out || !new_lens || !freed || !freed_counts ||
-        table_out == page_table || mass_out == mass || freed == page_table) {
+    if (bs > 0 && (!page_table || !mass || !seq_lens || !table_out || !mass_out || !new_lens || !freed || !freed_counts ||
+                   table_out == page_table || mass_out == mass || freed == page_table)) {
         set_error("%s: null or overlapping pointers", who);
         return MFD_ERR_INVALID;
     }

@@ -322,7 +322,7 @@ extern "C" int mfd_kv8_page_weights(const void* q, int64_t sq_b, int64_t sq_n, i
     if (!kv8::check_cache(who, k_cache, k_cache, sc_p, sc_h, sc_t, code_dtype, num_pages, page_size, page_table,
                           max_pages, seq_lens, bs, num_kv_heads, head_dim, &st))
         return st;
-    if (!q || !lse || !k_scale || !mass || !out || !workspace || !tickets) {
+    if ((bs > 0 && (!q || !lse || !mass || !out)) || !k_scale || !workspace || !tickets) {
         set_error("%s: null pointer", who);
         return MFD_ERR_INVALID;
     }

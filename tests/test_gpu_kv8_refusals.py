@@ -16,3 +16,15 @@ def test_append_refuses_a_status_that_is_no_int32(status):
     with pytest.raises(RuntimeError, match="status"):
         ops.kv8_append(c.k, c.v, c.ks, c.vs, c.kn, c.vn, c.table, c.seq, status=status.to(DEV))
     assert torch.equal(c.k, before[0]) and torch.equal(c.v, before[1])
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_an_empty_batch_gives_empty_results(n):
+    c = Case(302, [20, 3], n=n, heads=4, kv=2, page=16, dtype="int8")
+    none = dict(k_new=c.kn[:0], v_new=c.vn[:0])
+    out, lse = ops.kv8_attention(c.q[:0], c.k, c.v, c.ks, c.vs, c.table[:0], c.seq[:0], 1.0, **none, return_lse=True)
+    assert out.shape == (0, n, 4, 128) and lse.shape == (0, n, 4)
+    mass = torch.zeros(c.table.shape, device=DEV)[:0]
+    assert ops.kv8_page_weights(c.q[:0], lse, c.k, c.ks, c.table[:0], c.seq[:0], 1.0, mass).shape == mass.shape
+    assert ops.kv8_append(c.k, c.v, c.ks, c.vs, *none.values(), c.table[:0], c.seq[:0]).shape == (0,)
+    assert [tuple(t.shape) for t in ops.kv8_evict(c.table[:0], mass, c.seq[:0], 16, 4, 1, 1)][2:] == [(0,), mass.shape, (0,)]
