@@ -637,7 +637,9 @@ def _kv8_rows(what: str, rows: torch.Tensor, name: str, shape):
 
 def _kv8_new(what: str, k_new: torch.Tensor, v_new: torch.Tensor, shape):
     strides = _kv8_rows(what, k_new, "k_new", shape)
-    if v_new.stride() != strides or v_new.shape != shape or v_new.dtype != torch.bfloat16:
+    if v_new.shape != shape or v_new.dtype != torch.bfloat16 or (
+            v_new.stride() != strides  # (a stride of one row or request addresses nothing)
+            and any(size > 1 and a != b for size, a, b in zip(shape, strides, v_new.stride()))):
         raise RuntimeError(f"{what}: v_new must be bfloat16 {tuple(shape)} with the strides of k_new")
     return strides
 

@@ -28,3 +28,29 @@ def test_an_empty_batch_gives_empty_results(n):
     assert ops.kv8_page_weights(c.q[:0], lse, c.k, c.ks, c.table[:0], c.seq[:0], 1.0, mass).shape == mass.shape
     assert ops.kv8_append(c.k, c.v, c.ks, c.vs, *none.values(), c.table[:0], c.seq[:0]).shape == (0,)
     assert [tuple(t.shape) for t in ops.kv8_evict(c.table[:0], mass, c.seq[:0], 16, 4, 1, 1)][2:] == [(0,), mass.shape, (0,)]
+
+
+@pytest.mark.parametrize("bs,n", [(1, 1), (1, 3), (2, 1)])
+def test_keys_and_values_whose_strides_differ_where_it_does_not_matter(bs, n):
+    """A decode step's rotated keys are a tensor of their own, its values a slice of the fused projection: a batch of one, or
+    one node, has strides that address nothing."""
+    c = Case(303, [70] * bs, n=n, heads=4, kv=2, page=16, dtype="int8", spare=8)
+    want = c.run()
+    if bs == 1:
+        c.vn = torch.cat([c.vn, c.vn], 1)[:, :n]
+    else:
+        c.kn, c.vn = c.kn.transpose(0, 1).contiguous().transpose(0, 1), c.vn.as_strided(c.vn.shape, (256, 9 * 256, 128, 1))
+        c.kn = c.kn.as_strided(c.kn.shape, (256, 7 * 256, 128, 1))
+    assert c.kn.stride() != c.vn.stride()
+    got = c.run()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    ops.kv8_append(c.k, c.v, c.ks, c.vs, c.kn, c.vn, c.table, c.seq)
+
+
+def test_keys_and_values_whose_strides_differ_where_it_matters():
+    c = Case(304, [70, 3], n=2, heads=4, kv=2, page=16, dtype="int8", spare=8)
+    c.vn = torch.cat([c.vn, c.vn], 1)[:, :2]
+    with pytest.raises(RuntimeError, match="strides"):
+        c.run()
+    with pytest.raises(RuntimeError, match="strides"):
+        ops.kv8_append(c.k, c.v, c.ks, c.vs, c.kn, c.vn, c.table, c.seq)
