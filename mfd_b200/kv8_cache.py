@@ -37,6 +37,7 @@ class KV8Cache:
     def reserve(self, tokens: int) -> None:
         """Give every request pages for `tokens` more tokens.  Reads the lengths back.  All or nothing: where it raises,
         no request has got a page."""
+        self._check_status()
         need = [-(-(t + tokens) // self.page_size) for t in self.seq_lens.tolist()]
         for b, n in enumerate(need):
             if n > self.page_table.shape[1]:
@@ -51,10 +52,16 @@ class KV8Cache:
             del self._free[-len(places):]
             self._pages = [max(p, n) for p, n in zip(self._pages, need)]
 
+    def _check_status(self) -> None:
+        if int(self.status):
+            raise RuntimeError("KV8Cache: an append found no page for some of its rows, which the lengths count (set seq_lens to "
+                               "what the pages hold and status to 0 to go on)")
+
     def append(self, k_new: torch.Tensor, v_new: torch.Tensor, path: torch.Tensor | None = None,
                counts: torch.Tensor | None = None) -> None:
         """Quantise rows of k_new, v_new [bs, n, Hkv, D] into the cache: a prompt (counts rows each), or the accepted
-        path of a tree.  The pages must be there (reserve); self.status becomes nonzero when one was not."""
+        path of a tree.  The pages must be there (reserve).  Where one was not, its rows are lost, though the length counts
+        them, self.status becomes nonzero, and reserve() and evict() raise."""
         self.seq_lens = ops.kv8_append(self.k, self.v, self.k_scale, self.v_scale, k_new, v_new, self.page_table,
                                        self.seq_lens, path=path, counts=counts, status=self.status)
 
@@ -73,6 +80,7 @@ class KV8Cache:
     def evict(self, keep_pages: int, sink_pages: int = 1, recent_pages: int = 2) -> list[list[int]]:
         """Drop the pages of least mass of every request that fills more than keep_pages; they return to the pool.
         Returns the dropped page ids per request.  Pages that are reserved but still empty stay with their request."""
+        self._check_status()
         table, mass, lens, freed, counts = ops.kv8_evict(self.page_table, self.mass, self.seq_lens, self.page_size,
                                                          keep_pages, sink_pages, recent_pages)
         n = counts.tolist()
