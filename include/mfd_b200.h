@@ -316,7 +316,9 @@ int mfd_conv_commit(const uint64_t* conv_states, const uint64_t* x, int64_t elem
  * 8-bit paged K/V cache of one layer.  k_cache, v_cache: pages of page_size (16, 32, 64 or 128) tokens for every KV
  * head, row (page p, KV head h, token t) at byte offset p * sc_p + h * sc_h + t * sc_t (K and V alike; 128 contiguous
  * codes a row, strides and bases multiples of 16); code_dtype MFD_I8 or MFD_E4M3.  k_scale, v_scale
- * [num_pages, Hkv] float32: a value is code * scale.  Request b holds seq_lens[b] tokens (int32, on the device),
+ * [num_pages, Hkv] float32: a value is code * scale.  Scales are finite; V's are not negative (below 2^-100 they count as
+ * that), and those of the pages that a row sees lie within 2^100 of one another (farther apart, its log-sum-exp may miss
+ * keys of the pages with the least).  Request b holds seq_lens[b] tokens (int32, on the device),
  * token j in page page_table[b * table_stride + j / page_size] (int32), slot j % page_size.  Lengths are clamped to
  * [0, max_pages * page_size] and page ids to [0, num_pages), so no table makes a kernel read outside the cache.
  */

@@ -120,8 +120,9 @@ __device__ __forceinline__ float2 bf2(uint32_t w) {
 }
 
 // the power of two 2^-e that brings a row of largest magnitude mx into (-2, 2), and 2^e.  Both are exact, so a bf16
-// query row becomes float16 without loss except below 2^-24 of its largest element, whose products vanish against
-// the row's own rounding.  (A zero or non-finite row is left as it is.)
+// query row becomes float16 without loss down to 2^-17 of its largest element (8 bits, the last of them 2^-24, where
+// float16 ends); smaller ones lose up to 2^-25 of it, which vanishes against the row's own rounding.  (A zero or non-finite
+// row is left as it is.)
 __device__ __forceinline__ void row_power(float mx, float& down, float& up) {
     int e = (int)((__float_as_uint(mx) >> 23) & 0xffu) - 127;
     if (mx == 0.f || e == 128) e = 0;

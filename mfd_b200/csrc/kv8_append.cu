@@ -99,7 +99,8 @@ __device__ __forceinline__ float finite_abs(float x) {
 
 // CTAs an SM the registers are cut for.  A CTA waits for its rows, then for its maximum, then writes, so the others keep the
 // memory busy: two prompts of 8192 tokens in pages of 128 take 27 us with 4 (what 64 registers allow), 24.4 with 5 and
-// 29 with 8 (rows in local memory); in pages of 64 24.7 with 5, 23.9 with 6 and 22.7 with 8.
+// 29 with 8 (rows in local memory); in pages of 64 24.7 with 5, 23.9 with 6 and 22.7 with 8.  Pages of 16 take 32 registers,
+// which is 8, uncut (30.9 either way); pages of 32 take 40 uncut (26.7, and 24.7 with 8).  Paths of 17 rows: no difference.
 constexpr int ctas_per_sm(int page) { return page == 128 ? 5 : (page == 64 ? 8 : 1); }
 
 // PAGE: tokens per page, kItems rows of 16 lanes a thread

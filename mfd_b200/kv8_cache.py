@@ -8,6 +8,16 @@ the attention weight of the accepted nodes per page (weigh), quantises their key
 
 Which request owns which page is decided on the host: reserve() and evict() read a few integers back (they
 synchronise); attention(), weigh() and append() only launch.
+
+What it does not do:
+- Pages come back through evict() alone.  A request that has finished keeps its pages, and reserve() makes room for as many
+  tokens in every request: a server that admits and retires requests keeps its own tables and calls the operators.
+- append() and evict() bind seq_lens (and evict() page_table and mass) to new tensors, so a CUDA graph of a whole step is built
+  from the operators, with tensors that stay.
+- After an eviction seq_lens counts the tokens that are held, not those that were seen.  The position of the next token, for
+  rotary embeddings, is the caller's to keep.
+- Pages enter with mass 0, a prompt's too, and the attention among a step's own nodes is credited to no page: mass is what later
+  steps gave a page through weigh().
 """
 
 from __future__ import annotations
