@@ -330,6 +330,7 @@ int mfd_conv_commit(const uint64_t* conv_states, const uint64_t* x, int64_t elem
  * becomes max(its old scale if it already holds tokens of the request, max |finite new value| * r, 2^-100), r the
  * float32 nearest to 1 / 127 (int8) or 1 / 448 (e4m3); codes are value / scale rounded to nearest even; tokens already in the page are rounded
  * again when its scale grows.  An infinite value becomes +-127 or +-448, NaN becomes 0, and neither counts for the scale.
+ * (A zero's sign is not kept.)
  * Every product, quotient and rounding is the IEEE float32 one, so the codes do not depend on the launch.  new_lens
  * [bs] int32 (must not be seq_lens) receives seq_lens + the rows appended.  Rows past max_pages * page_size, and rows
  * of a page whose table entry is outside [0, num_pages), are dropped and status (optional device int) receives

@@ -59,7 +59,7 @@ __device__ __forceinline__ uint32_t encode2(float a, float b) {  // two values a
 // exact remainder (Markstein's theorem on the correctly rounded quotient), two values an instruction.  The result is the
 // IEEE quotient for every bf16 x and every scale whose reciprocal is normal and whose remainders are exact, at a fifth of
 // the instructions of a division.  (2^23 significands of the scale times 128 of x: none differs.  Below 2^-90 a remainder may be
-// subnormal: 1.9999999 * 2^-100 and x = 2^-109 give another e4m3 code.)  Blocks of other scales divide.
+// subnormal: 1.9999999 * 2^-100 and x = 2^-109 give another e4m3 code.)  Blocks of other scales divide, unless all their values are zero.
 constexpr float kFastScaleLo = 5.421010862427522e-20f, kFastScaleHi = 8.507059173023462e+37f;  // 2^-64 and 2^126
 template <bool FP8>
 __device__ __forceinline__ uint2 encode8(const uint4& x, float s, float r) {
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(PAGE)) kv8_append_kernel
         for (int w = 0; w < kThreads / 32; ++w) mx = fmaxf(mx, warp_max[w]);
     }
     const float s = fmaxf(fmaxf(__fmul_rn(mx, 1.f / qmax), open), kScaleFloor), r = __frcp_rn(s);
-    const bool fast = finite && s >= kFastScaleLo && s <= kFastScaleHi;
+    const bool fast = finite && s <= kFastScaleHi && (s >= kFastScaleLo || mx == 0.f);  // (zeros are 0 in any scale)
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
         const int slot = r0 + kRowsPerPass * i;

@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+from mfd_b200 import ops
 from test_gpu_kv8 import DEV, Case, _check_append
 
 pytestmark = pytest.mark.gpu
@@ -28,3 +29,20 @@ def test_codes_behind_an_open_page_of_any_scale(scale, dtype):
     rows = x.bfloat16()[None, :, None].expand(2, n, 2, 128).contiguous()
     _check_append(c, rows, -rows, [list(range(n))] * 2, [n, n])
     assert c.ks[int(c.table[0, 0])].tolist() == [torch.tensor(scale, dtype=torch.float32).item()] * 2
+
+
+@pytest.mark.parametrize("dtype", ["int8", "e4m3"])
+@pytest.mark.parametrize("scale", [2.0 ** -100, 1.0, 2.0 ** 126])
+def test_zeros_of_both_signs_are_zero(scale, dtype):
+    """Behind an open page, and in pages of their own, whose scale is the least."""
+    c = Case(402, [5, 0], n=20, kv=2, page=16, dtype=dtype, spare=20, stale=False)
+    c.ks[int(c.table[0, 0])] = scale
+    rows = torch.zeros(2, 20, 2, 128, device=DEV).bfloat16()
+    rows[:, ::2] = -0.0
+    before = c.k[int(c.table[0, 0]), :, :5].view(torch.uint8).clone()
+    lens = ops.kv8_append(c.k, c.v, c.ks, c.vs, rows, rows, c.table, c.seq)
+    c.lens = lens.tolist()
+    assert c.lens == [25, 20]
+    assert bool((c.rows(0, "k")[:, 5:] == 0).all()) and bool((c.rows(1, "k") == 0).all()) and bool((c.rows(1, "v") == 0).all())
+    assert torch.equal(c.k[int(c.table[0, 0]), :, :5].view(torch.uint8), before) and c.ks[int(c.table[0, 0])].tolist() == [scale] * 2
+    assert c.ks[c.table[1, :2].long()].unique().tolist() == [2.0 ** -100]
